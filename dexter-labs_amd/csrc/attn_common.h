@@ -86,10 +86,12 @@ __device__ __forceinline__ void prefetch_args(const AttnArgs& a) {
 // Block start i, read through the constant address space: the list does not
 // change while a kernel runs, and that lets the compiler use scalar loads
 // (counted by lgkmcnt) instead of vector loads, whose waits would also wait
-// for every tile load in flight.
+// for every tile load in flight. (Args, here and below: AttnArgs, or other
+// launch arguments with its mask fields.)
 typedef __attribute__((address_space(4))) const int32_t const_i32;
 typedef __attribute__((address_space(4))) const int64_t const_i64;
-__device__ __forceinline__ int load_start(const AttnArgs& a, int i) {
+template <typename Args>
+__device__ __forceinline__ int load_start(const Args& a, int i) {
   // A generic pointer to device memory is its global address: convert it
   // through the integer value.
   const uint64_t p = reinterpret_cast<uint64_t>(a.starts);
@@ -104,8 +106,8 @@ __device__ __forceinline__ int slice_at(int x, int n) { return x < 0 ? max(x + n
 // slicing, current keys [0, min(hi, Lq))). The starts are read 16 (+1) at a
 // time as independent scalar loads, so each batch is one memory round trip
 // instead of a chain of dependent ones; fn(lo, hi) sees every pair in order.
-template <typename Fn>
-__device__ __forceinline__ void for_each_block(const AttnArgs& a, Fn&& fn) {
+template <typename Args, typename Fn>
+__device__ __forceinline__ void for_each_block(const Args& a, Fn&& fn) {
   const int nb = a.n_blocks;
   for (int base = 0; base < nb; base += 16) {
     int st[17];
@@ -133,7 +135,8 @@ __device__ __forceinline__ int pair_end(int hi, int cache_len, int Lq) {
 // pair_end among them, 0 when no pair holds i (such a row sees only the
 // cache). For ascending starts this is the end of i's own block, and rows
 // before the first start see no current key.
-__device__ __forceinline__ int visible_end(const AttnArgs& a, int i, int cache_len) {
+template <typename Args>
+__device__ __forceinline__ int visible_end(const Args& a, int i, int cache_len) {
   if (a.causal) return i + 1;
   if (a.n_blocks == 0) return a.Lk;
   int e = 0;
@@ -151,7 +154,8 @@ __device__ __forceinline__ int visible_end(const AttnArgs& a, int i, int cache_l
 // the widest bounds, [0, Lq]: every current tile is visited and masked per
 // key, so results stay exact and only the whole-tile skipping is lost.
 struct EndBounds { int lo, hi; };
-__device__ __forceinline__ EndBounds end_bounds(const AttnArgs& a, int q_first, int q_last) {
+template <typename Args>
+__device__ __forceinline__ EndBounds end_bounds(const Args& a, int q_first, int q_last) {
   if (a.causal || a.n_blocks == 0)
     return {__builtin_amdgcn_readfirstlane(visible_end(a, q_first, 0)),
             __builtin_amdgcn_readfirstlane(visible_end(a, q_last, 0))};

@@ -26,6 +26,13 @@ and calls it, exactly as dexter's dispatchers do (``python/dexter/ops/__init__.p
   (reference ``ops/__init__.py:39-49``; same arguments and default eps)
 * ``gated_residual``             -> ``select("norm", "gated_residual", x, y, gate)``
   (reference ``ops/__init__.py:52-54``)
+* ``kv_page_append``             -> ``select("cache", "page_append", pages, k, v)``,
+  ``kv_page_copy``               -> ``select("cache", "page_copy", pools)``,
+  ``paged_attention``            -> ``select("attention", "paged", q, k, v)``,
+  ``shared_prefix_attention``    -> ``select("attention", "shared_prefix", q, k, v)``
+  (no counterpart in the reference, whose cache is one contiguous history per
+  sequence, ``models/dreamzero/model.py:35-65``: a cache in pages that
+  sequences can share, and attention over it)
 
 Importing this module registers the gfx950 HIP kernels. Nothing else is
 registered, so on a machine without an MI355X every call raises
@@ -34,6 +41,8 @@ registered, so on a machine without an MI355X every call raises
 
 from __future__ import annotations
 
+from collections.abc import Sequence
+
 import torch
 
 from ..registry import select
@@ -41,7 +50,8 @@ from ..registry import select
 __all__ = ["qk_norm_rope", "blockwise_causal_attention", "kv_cache_append",
            "qk_norm_rope_append", "blockwise_causal_attention_varlen",
            "adaln_modulate", "gated_residual", "qkv_norm_rope", "qk_norm_rope_attention",
-           "linear_chunk"]
+           "linear_chunk", "kv_page_append", "kv_page_copy", "paged_attention",
+           "shared_prefix_attention"]
 
 
 def qkv_norm_rope(
@@ -239,6 +249,90 @@ def qk_norm_rope_append(
     """
     return select("rope", "qk_norm_rope_append", q, k, v, cache)(
         q, k, v, q_weight, k_weight, cos, sin, cache, start, eps, interleaved, status)
+
+
+def kv_page_append(pages: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                   block_table: torch.Tensor, starts: torch.Tensor,
+                   status: torch.Tensor | None = None) -> None:
+    """Write ``k``/``v`` ``[B, n, H, D]`` into the batch's pages: row ``starts[b] + t``
+    of sequence ``b`` is row ``r % R`` of page ``block_table[b, r // R]`` of ``pages``
+    ``[2, P, R, H, D]``.
+
+    ``block_table`` ``[B, W]`` and ``starts`` ``[B]`` are int32 on the device, read by
+    the kernel when it runs. A row without a page (past the table, a start below 0, an
+    entry outside ``[0, P)``) is not written, and ``status`` (one int32, optional) set
+    to 1. Sequences that write one page's same row in one call leave either's.
+    """
+    return select("cache", "page_append", pages, k, v)(pages, k, v, block_table, starts, status)
+
+
+def kv_page_copy(pages: torch.Tensor | Sequence[torch.Tensor], src: Sequence[int],
+                 dst: Sequence[int]) -> None:
+    """``pages[:, dst[i]] = pages[:, src[i]]`` for every ``i``: what a fork (the partly
+    filled last page) and compaction need. ``pages`` is a pool ``[2, P, R, H, D]`` or one
+    per layer, all of one shape, copied in one launch (of up to 64 pools and 256 pages).
+
+    ``src`` and ``dst`` are host page numbers. A page may be a source several times;
+    ``ValueError`` when one is written twice, or both read and written.
+    """
+    pools = [pages] if isinstance(pages, torch.Tensor) else list(pages)
+    return select("cache", "page_copy", pools)(pools, src, dst)
+
+
+def paged_attention(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    *,
+    pages: torch.Tensor,
+    block_table: torch.Tensor,
+    cache_lens: torch.Tensor,
+    block_boundaries: torch.Tensor | None = None,
+    softmax_scale: float | None = None,
+    causal: bool = False,
+) -> torch.Tensor:
+    """``blockwise_causal_attention`` with each sequence's cached rows in pages.
+
+    Sequence ``b`` attends to rows ``[0, cache_lens[b])`` of its pages (``block_table``
+    ``[B, W]``, ``pages`` ``[2, P, R, Hkv, D]``), then to its own ``k``/``v``, under the
+    same masks. ``k``/``v`` may be empty (keys all cached) or of another length than
+    ``q`` (no mask), and have fewer heads (grouped-query). ``block_table`` and
+    ``cache_lens`` ``[B]`` are int32 on the device, read by the kernels when they run:
+    lengths are clamped to ``[0, W * R]``, keys of an entry outside ``[0, P)`` are not
+    seen (a sequence may drop pages of its history), and a graph captured once follows
+    both. A narrower ``block_table[:, :w]`` plans the launch for fewer rows. A query
+    that sees no key gives NaN, as in ``blockwise_causal_attention``.
+    """
+    return select("attention", "paged", q, k, v)(
+        q, k, v, pages, block_table, cache_lens, block_boundaries, softmax_scale, causal)
+
+
+def shared_prefix_attention(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    *,
+    pages: torch.Tensor,
+    prefix_table: torch.Tensor,
+    prefix_len: torch.Tensor,
+    block_table: torch.Tensor | None = None,
+    cache_lens: torch.Tensor | None = None,
+    block_boundaries: torch.Tensor | None = None,
+    softmax_scale: float | None = None,
+    causal: bool = False,
+) -> torch.Tensor:
+    """``paged_attention`` for a batch that shares a prefix, computed once for all.
+
+    Every sequence attends to rows ``[0, prefix_len)`` of the pages ``prefix_table``
+    ``[Wp]`` (both int32 on the device; ``prefix_len`` one element), then to its own
+    cached rows (``block_table`` and ``cache_lens``, optional) and its ``k``/``v``. The
+    result is that of ``paged_attention`` with the prefix's pages in front of each
+    sequence's own (when the prefix fills its pages), but its keys and values are read
+    once for all queries of the batch instead of once per sequence.
+    """
+    return select("attention", "shared_prefix", q, k, v)(
+        q, k, v, pages, prefix_table, prefix_len, block_table, cache_lens, block_boundaries,
+        softmax_scale, causal)
 
 
 # Importing the implementation package is what populates the registry.

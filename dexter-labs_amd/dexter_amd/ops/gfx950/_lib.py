@@ -16,7 +16,7 @@ import torch
 
 LIB_NAME = "libdexter_gfx950.so"
 LIB_PATH = Path(__file__).resolve().parents[2] / LIB_NAME
-ABI_VERSION = 12
+ABI_VERSION = 13
 
 DX_OK, DX_EINVAL, DX_ELAUNCH, DX_EFULL, DX_EWORKSPACE = 0, 1, 2, 3, 4
 DX_BF16, DX_F16, DX_F32, DX_I32, DX_I64 = 0, 1, 2, 3, 4
@@ -158,6 +158,44 @@ _SIGNATURES: dict[str, tuple[type, list]] = {
         _p, _l, _l, _i,            # x, sb, sl, io dtype
         _p, _l, _p, _p,            # w, row stride, bias (may be null), y
         _l, _l, _l, _l, _p]),      # B, L, C, N, stream
+    "dx_kv_page_append": (_i, [
+        _p, _l, _l, _l,            # k
+        _p, _l, _l, _l,            # v
+        _p, _l, _l, _l, _l,        # pages, plane, page, row, head strides
+        _i, _l, _l,                # dtype, pages, rows per page
+        _p, _l, _l, _p, _p,        # block table, its row stride, width, starts, status
+        _l, _l, _l, _l, _p]),      # B, n, H, D, stream
+    "dx_kv_page_copy": (_i, [
+        ctypes.POINTER(_p), _l,    # pools, count
+        _l, _l, _l, _l,            # plane, page, row, head strides
+        _i, _l, _l, _l, _l,        # dtype, pages, rows per page, H, D
+        ctypes.POINTER(_l), ctypes.POINTER(_l), _l, _p]),  # src, dst, pairs, stream
+    "dx_paged_attention_workspace_bytes": (_l, [
+        _i, _l, _l, _l, _l, _l, _l,  # dtype, B, Lq, Lk, H, Hkv, D
+        _l, _l, _i, _l]),          # rows per page, table width, has prefix, prefix width
+    "dx_paged_attention": (_i, [
+        _p, _l, _l, _l,            # q
+        _p, _l, _l, _l,            # k
+        _p, _l, _l, _l,            # v
+        _p, _l, _l, _l, _l, _l, _l,  # pages, plane, page, row, head strides, pages, rows per page
+        _p, _l, _l, _p,            # block table, its row stride, width, cache lengths
+        _p, _l, _l, _l,            # out
+        _i, _l, _l, _l, _l, _l, _l,  # dtype, B, Lq, Lk, H, Hkv, D
+        _p, _i, _l,                # starts, starts dtype, n_blocks
+        _i, _f,                    # causal, scale
+        _p, _l, _p]),              # workspace, bytes, stream
+    "dx_shared_prefix_attention": (_i, [
+        _p, _l, _l, _l,
+        _p, _l, _l, _l,
+        _p, _l, _l, _l,
+        _p, _l, _l, _l, _l, _l, _l,
+        _p, _l, _p,                # prefix table, width, length
+        _p, _l, _l, _p,
+        _p, _l, _l, _l,
+        _i, _l, _l, _l, _l, _l, _l,
+        _p, _i, _l,
+        _i, _f,
+        _p, _l, _p]),
     "dx_adaln_modulate": (_i, [
         _p, _l, _l, _i,            # x, sb, sl, x dtype
         _p, _l, _l,                # scale, sb, sl

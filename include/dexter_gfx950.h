@@ -39,6 +39,12 @@
  *   dx_gated_residual        ops/gfx1151/norm/adaln.py:131-148 (kernel :51-67;
  *                            semantics ops/reference/norm.py:23-25, dispatcher
  *                            ops/__init__.py:52-54)
+ *   dx_kv_page_append, dx_kv_page_copy, dx_paged_attention,
+ *   dx_shared_prefix_attention
+ *                            a KV cache in pages that sequences can share;
+ *                            no counterpart (the reference's cache is one
+ *                            contiguous history per sequence,
+ *                            models/dreamzero/model.py:35-65)
  *
  * Conventions
  *  - Tensors are device pointers with explicit element strides; the last
@@ -79,7 +85,7 @@ const char* dx_last_error(void);
 
 /* ABI revision of this header; the Python loader checks it. */
 int dx_abi_version(void);
-#define DX_ABI_VERSION 12
+#define DX_ABI_VERSION 13
 
 /*
  * Launch-schedule overrides, for measurement and tests only: process-wide,
@@ -459,6 +465,97 @@ int dx_gated_residual(const void* x, int64_t x_sb, int64_t x_sl,
                       const void* gate, int64_t g_sb, int64_t g_sl, int gate_dtype,
                       void* out, int64_t o_sb, int64_t o_sl, int out_dtype,
                       int64_t B, int64_t L, int64_t C, void* stream);
+
+/*
+ * A KV cache in pages. A pool is [2, n_pages, page_rows, H, D] through its
+ * strides (p_plane, p_sp per page, p_sr per row, p_sh per head; plane 0 K,
+ * plane 1 V). Row r of a sequence lies in page table[r / page_rows] at row
+ * r % page_rows. block_table is int32 [B, width] with row stride t_sb; it, the
+ * start rows and the lengths are read on the device when the kernels run (no
+ * host sync, a captured graph follows them). A table entry outside
+ * [0, n_pages) holds no rows.
+ */
+
+/*
+ * Copy k and v [B, n, H, D] into the batch's pages: token t of sequence b
+ * becomes row starts[b] + t (starts: int32 [B]). Bit-exact. A row without a
+ * page (starts[b] + t negative or not below width * page_rows, or an entry that
+ * holds no rows) is not written and *status (int32, may be NULL) set to 1.
+ * dtype: DX_BF16, DX_F16 or DX_F32; D fills 16-byte chunks; any page_rows.
+ */
+int dx_kv_page_append(const void* k, int64_t k_sb, int64_t k_sl, int64_t k_sh,
+                      const void* v, int64_t v_sb, int64_t v_sl, int64_t v_sh,
+                      void* pages, int64_t p_plane, int64_t p_sp, int64_t p_sr, int64_t p_sh,
+                      int dtype, int64_t n_pages, int64_t page_rows,
+                      const void* block_table, int64_t t_sb, int64_t width,
+                      const void* starts, void* status,
+                      int64_t B, int64_t n, int64_t H, int64_t D, void* stream);
+
+/*
+ * Copy page src[i] to page dst[i] (host arrays of `pairs` page numbers) in both
+ * planes of each of n_pools pools (a host array of device pointers to plane 0;
+ * all pools have the strides given). The arrays are read before the call
+ * returns. One launch per 64 pools and 256 pages. DX_EINVAL, nothing launched,
+ * for a page outside [0, n_pages), one written twice, or one both read and
+ * written; a page may be read several times.
+ */
+int dx_kv_page_copy(const void* const* pools, int64_t n_pools,
+                    int64_t p_plane, int64_t p_sp, int64_t p_sr, int64_t p_sh,
+                    int dtype, int64_t n_pages, int64_t page_rows, int64_t H, int64_t D,
+                    const int64_t* src, const int64_t* dst, int64_t pairs, void* stream);
+
+/*
+ * dx_blockwise_causal_attention with sequence b's cached rows [0, cache_lens[b])
+ * in pages: keys = [paged rows | k/v rows 0..Lk)], the same masks and NaN rows,
+ * with cache_lens[b] (int32 [B], clamped to [0, width * page_rows]) as the cache
+ * length. Keys of an entry that holds no rows are not seen. Lk may be 0; width
+ * may be 0 (block_table and cache_lens NULL). page_rows: a multiple of 16 up to
+ * 1024. dtype: DX_BF16 or DX_F16 at D 64, 128 or 256, DX_F32 at D 64 or 128;
+ * sums and softmax in fp32, one rounding to dtype. Sequences hold fewer than
+ * 2^30 rows; the pool may exceed 4 GB. Row strides of the pool, k and v are
+ * below 2^26 bytes. workspace: dx_paged_attention_workspace_bytes(...) bytes, 16-byte
+ * aligned, no initialisation (NULL when 0); calls that share one must not
+ * overlap.
+ */
+int dx_paged_attention(
+    const void* q, int64_t q_sb, int64_t q_sl, int64_t q_sh,
+    const void* k, int64_t k_sb, int64_t k_sl, int64_t k_sh,
+    const void* v, int64_t v_sb, int64_t v_sl, int64_t v_sh,
+    const void* pages, int64_t p_plane, int64_t p_sp, int64_t p_sr, int64_t p_sh,
+    int64_t n_pages, int64_t page_rows,
+    const void* block_table, int64_t t_sb, int64_t width, const void* cache_lens,
+    void* out, int64_t o_sb, int64_t o_sl, int64_t o_sh,
+    int dtype, int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hkv, int64_t D,
+    const void* block_starts, int starts_dtype, int64_t n_blocks, int causal, float softmax_scale,
+    void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * dx_paged_attention with a prefix in front of every sequence's keys: rows
+ * [0, *prefix_len) (one int32 on the device, clamped to what the table holds) of
+ * the pages prefix_table (int32 [prefix_width]). keys = [prefix | paged rows |
+ * k/v]; the masks' cache length is *prefix_len + cache_lens[b]. The prefix's keys
+ * and values are read for all B * Lq queries at once.
+ */
+int dx_shared_prefix_attention(
+    const void* q, int64_t q_sb, int64_t q_sl, int64_t q_sh,
+    const void* k, int64_t k_sb, int64_t k_sl, int64_t k_sh,
+    const void* v, int64_t v_sb, int64_t v_sl, int64_t v_sh,
+    const void* pages, int64_t p_plane, int64_t p_sp, int64_t p_sr, int64_t p_sh,
+    int64_t n_pages, int64_t page_rows,
+    const void* prefix_table, int64_t prefix_width, const void* prefix_len,
+    const void* block_table, int64_t t_sb, int64_t width, const void* cache_lens,
+    void* out, int64_t o_sb, int64_t o_sl, int64_t o_sh,
+    int dtype, int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hkv, int64_t D,
+    const void* block_starts, int starts_dtype, int64_t n_blocks, int causal, float softmax_scale,
+    void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Workspace bytes of dx_paged_attention (has_prefix 0) or
+ * dx_shared_prefix_attention on the current device; negative DX_E* on a bad shape.
+ */
+int64_t dx_paged_attention_workspace_bytes(int dtype, int64_t B, int64_t Lq, int64_t Lk, int64_t H,
+                                           int64_t Hkv, int64_t D, int64_t page_rows,
+                                           int64_t width, int has_prefix, int64_t prefix_width);
 
 #ifdef __cplusplus
 }
