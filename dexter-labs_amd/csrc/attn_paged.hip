@@ -17,12 +17,27 @@
 // sequence (and, as everywhere here, of every query head of a K/V head): its
 // K and V are read once for 32 RW rows, whatever sequence they belong to.
 //
+// Work. The unit is a 32-key tile of a work item (32 RW rows of one K/V head, of
+// one sequence or, for the prefix, of the whole batch). There are two lines of
+// items, the own keys' and the prefix's, in one launch, and two ways to deal one:
+//  * Cut (items that share no keys: one row tile per sequence and head). All
+//    tiles of all items form one line, which is cut into equal pieces, one per
+//    workgroup, whatever the lengths are: the device cuts it, by the lengths as
+//    they are. A piece covers whole items, whose results it writes itself, and
+//    at most two broken ones, whose partials paged_merge_kernel joins.
+//  * Split (several row tiles read the same keys): every item in S equal ranges
+//    of keys, a workgroup each, those of one head next to each other on one XCD,
+//    so that they read a key tile at about the same time, through one L2. Cut
+//    instead, 16 x 83 queries over a shared 8,217-row prefix (24 heads) took 597
+//    us, every workgroup at a place of its own in the keys.
+// With a prefix every row has parts of both lines, and the merge joins them all.
+//
 // Kernel. A wave owns 32 rows (S^T = K Q^T on 32 x 32 MFMAs, the formulation of
 // attn_fwd.hip: a lane holds one row and 16 keys, P^T is the B operand of
 // O^T += V^T P^T as it is). A workgroup is RW waves of rows times KW streams,
-// which take alternate 32-key tiles; the streams' results meet in LDS at the
-// end. Tiles land by LDS DMA, 16 rows to a descriptor: pages are multiples of
-// 16 rows, so 16 rows lie in one page, the page's 64-bit address is scalar
+// which take alternate tiles; the streams' results meet in LDS at the end.
+// Tiles land by LDS DMA, 16 rows to a descriptor: pages are multiples of 16
+// rows, so 16 rows lie in one page, the page's 64-bit address is scalar
 // arithmetic, and rows past the end (or of a table entry that names no page)
 // come back as zeros from the descriptor's bound.
 #include "attn_tile.h"
@@ -31,11 +46,24 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace dx {
 namespace {
 
-constexpr int kPN = 32;  // keys per tile
+constexpr int kPN = 32;  // keys per tile of the line
+// Where an item's parts are: slot of the first, and their number (one after the
+// other). By item, or, where the line is cut and there is no prefix, by
+// workgroup: the item that it leaves broken (parts 0: none).
+struct Record { int item, slot, parts, pad; };
+
+// A line of work: its partials and records.
+struct Line {
+  float* o;     // [slot][32 RW rows][D]: unnormalised sums
+  float* ml;    // [slot][32 RW rows]: {m, l}
+  Record* rec;
+  int splits;   // key ranges per item; 0: the line is cut into pieces
+};
 
 struct PagedArgs {
   const char* q; int64_t q_sb, q_sl, q_sh;  // strides in bytes, here and below
@@ -52,13 +80,19 @@ struct PagedArgs {
   int B, H, Hkv, group, Lq, Lk, causal;
   int R;                        // rows of a (sequence, K/V head): Lq * group
   float scale_log2;             // signed
-  // Partials, by parts: of the own keys ([unit][split], a unit being 32 rows of
-  // a (K/V head, sequence)) and of the prefix (a unit being 32 of all B R rows
-  // of a K/V head). ws_o: [64 lanes] x 16 bytes per 32 x 8 block, in
-  // accumulator order; ws_ml: {m, l} per row.
-  float* own_o; float* own_ml; int own_splits, own_blocks;  // blocks: units per (head, sequence)
-  float* pre_o; float* pre_ml; int pre_splits, pre_blocks;
+  int own_n;                    // workgroups for the own line at most, where it alone is cut
+  Line own, pre;
 };
+
+// The launch arguments where they lie. reread() hides where a pointer to them
+// comes from: what is read through its result is read there, and not kept in
+// scalar registers from the kernel's start on (they hold a third of what the
+// compiler would keep, and spilled the tile loop's).
+typedef __attribute__((address_space(4))) const PagedArgs Args;
+__device__ __forceinline__ Args* reread(Args* a) {
+  asm volatile("" : "+s"(a));
+  return a;
+}
 
 template <typename T> struct Elem { static constexpr int bytes = 2; };
 template <> struct Elem<float> { static constexpr int bytes = 4; };
@@ -76,229 +110,223 @@ template <int RB, bool F32> __device__ __forceinline__ constexpr int vswz(int r)
   return 4 * (RB == 128 ? ((r >> 1) ^ (r >> 2)) & 1 : (r & 3) ^ ((r >> 2) & 1));
 }
 
+constexpr int kThreads = 512, kWaves = 8;
+
+// A workgroup's shape for RW row waves.
 template <typename T, int D, int RW> struct Shape {
   static constexpr int RB = D * Elem<T>::bytes;      // bytes of a row
-  static constexpr int KW = RB >= 512 ? 2 : RW == 4 ? 2 : 4;
-  static constexpr int NW = RW * KW;
-  static constexpr int stages = 2;
-  static constexpr int tile = kPN * RB;              // bytes of a K or V tile
-  static constexpr int stage = 2 * tile;
-  static constexpr int stream = stages * stage;
-  static constexpr int hand = (1 + D / 8) * 1024;    // bytes a wave hands over: m, l and acc
-  static constexpr int lds = KW * stream > KW / 2 * RW * hand ? KW * stream : KW / 2 * RW * hand;
+  // Keys that a stream takes at a time. One row wave: 32, streams of one wave,
+  // whose K and V are single (the next K goes out when S is done, the next V
+  // when PV is done), as many streams as fit. Else two streams with two stages
+  // of 64 keys (each of four waves then fetches 16 rows, which one page holds),
+  // or of 32 where registers and LDS hold no more.
+  static constexpr int TK = RW == 1 || RB >= 512 ? 32 : 64;
+  static constexpr int KW = RW == 1 ? (RB >= 512 ? 4 : 8) : kWaves / RW;
+  static constexpr int tile = TK * RB;               // bytes of a K or V tile
+  static constexpr int stages = RW == 1 ? 1 : 2;
+  static constexpr int stream = stages * 2 * tile;
+  // Results on their way between waves: [wave][D' / 8 vectors][64 lanes] of 16
+  // bytes, a vector's row padded by 16 (reads across vectors then hit all
+  // banks), and {m, l} of 32 rows. D' = D, or half of it where that fits.
+  static constexpr int DP = D > 128 ? 128 : D;
+  static constexpr int vec = 1040;
+  static constexpr int area = DP / 8 * vec + 256;
+  static constexpr int body = KW * stream > RW * KW * area ? KW * stream : RW * KW * area;
+  // Behind them: which 16-row groups of each stage's tile have no page.
+  static constexpr int flags = body;
+  static constexpr int lds = body + kWaves * 2 * 16;
+  static_assert(lds <= 160 * 1024, "LDS of a CU");
 };
 
-// Where a 16-row group of keys lies, and how many of its rows exist.
-struct Rows16 {
-  const char* k; const char* v;
-  int rows;
-};
+__device__ __forceinline__ int tiles_of(int rows) { return (rows + kPN - 1) / kPN; }
 
-template <typename T, int D, int RW, bool PREFIX>
-__global__ __launch_bounds__((64 * Shape<T, D, RW>::NW), 1) void paged_attn_kernel(PagedArgs a) {
-  using Sh = Shape<T, D, RW>;
-  constexpr bool F32 = Elem<T>::bytes == 4;
-  constexpr int RB = Sh::RB, KW = Sh::KW, ST = Sh::stages;
-  constexpr int KS = RB / 32, DT = D / 32, CR = RB / 16, RPP = 64 / CR;
-  constexpr int PW = kPN / RPP / RW;  // DMA pieces (of K, and of V) a wave sends per tile
-  static_assert(PW >= 1, "every wave sends whole pieces");
-  extern __shared__ __attribute__((aligned(16))) char smem[];
+// Tiles of the new keys that row tile rt sees (at least 1, so that every item
+// has a tile and a workgroup), rt differing between lanes: end_bounds' hi.
+template <int RW>
+__device__ __forceinline__ int new_tiles(Args& a, int rt) {
+  const int q_last = (min((rt + 1) * (32 * RW), a.R) - 1) / a.group;
+  int hi;
+  if (a.causal) {
+    hi = q_last + 1;
+  } else if (a.n_blocks == 0) {
+    hi = a.Lk;
+  } else {
+    bool ascending = true;
+    int prev = 0;
+    hi = 0;
+    for_each_block(a, [&](int lo, int end) __attribute__((always_inline)) {
+      ascending = ascending && lo >= prev;
+      prev = lo;
+      if (q_last >= slice_at(lo, a.Lq) && q_last < slice_at(end, a.Lq)) hi = max(hi, min(end, a.Lq));
+    });
+    if (!ascending) hi = a.Lq;
+  }
+  return max(tiles_of(hi), 1);
+}
 
-  // Work item: (sequence and K/V head, row tile, key split); late row tiles,
-  // which see the most keys under a causal mask, first. Workgroup i runs on
-  // XCD i % 8: with a multiple of 8 groups each XCD takes a run of them, so
-  // that what reads the same keys goes through one L2.
-  const int splits = PREFIX ? a.pre_splits : a.own_splits;
-  const int nrows = PREFIX ? a.B * a.R : a.R;
-  const int n_rt = (nrows + 32 * RW - 1) / (32 * RW);
-  int b, hk, rt, split;
-  {
-    const uint32_t i = blockIdx.x, G = uint32_t(PREFIX ? a.Hkv : a.B * a.Hkv);
-    uint32_t grp, rank;
-    if (G % 8 == 0) {
-      const uint32_t g8 = G / 8, slot = i / 8;
-      rank = slot / g8;
-      grp = i % 8 * g8 + (slot - rank * g8);
+__device__ __forceinline__ uint64_t scan64(uint64_t x, int lane) {  // inclusive, over a wave
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const uint64_t y = __shfl_up(x, d);
+    if (lane >= d) x += y;
+  }
+  return x;
+}
+__device__ __forceinline__ uint64_t uniform(uint64_t x) {
+  return uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(int(x)))) |
+         uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(int(x >> 32)))) << 32;
+}
+__device__ __forceinline__ int own_rows(Args& a, int b) {
+  return a.width == 0 ? 0 : min(max(a.lens[b], 0), a.width * a.page_rows);
+}
+__device__ __forceinline__ int prefix_rows(Args& a) {
+  return a.plen ? min(max(*a.plen, 0), a.pwidth * a.page_rows) : 0;
+}
+
+// n / d for uniform n; 64-bit division is long.
+__device__ __forceinline__ uint64_t udiv(uint64_t n, uint64_t d) {
+  return (n | d) >> 32 ? n / d : uint64_t(uint32_t(n) / uint32_t(d));
+}
+
+// The line of the own keys: items (sequence, K/V head, row tile), in this order.
+template <int RW>
+struct OwnLine {
+  int n_rt;
+  uint64_t fresh;  // new-key tiles of a (sequence, head): of all its row tiles
+  uint64_t total;
+  __device__ __forceinline__ void init(Args& a, int lane) {
+    n_rt = (a.R + 32 * RW - 1) / (32 * RW);
+    fresh = 0;
+    if (a.causal || a.n_blocks) {
+      for (int r0 = 0; r0 < n_rt; r0 += 64)
+        fresh += uniform(__shfl(scan64(r0 + lane < n_rt ? new_tiles<RW>(a, r0 + lane) : 0, lane), 63));
     } else {
-      rank = i / G;
-      grp = i - rank * G;
+      fresh = uint64_t(n_rt) * max(tiles_of(a.Lk), 1);
     }
-    const uint32_t t = rank / uint32_t(splits);
-    split = int(rank - t * uint32_t(splits));
-    rt = n_rt - 1 - int(t);
-    b = PREFIX ? 0 : int(grp / uint32_t(a.Hkv));
-    hk = int(grp) - b * a.Hkv;
-  }
-  const int wid = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
-  const int stream = wid / RW, wave = wid % RW, lane = int(threadIdx.x) & 63;
-  const int g = lane >> 5, n = lane & 31;
-  const int row0 = rt * 32 * RW;                   // first row of the item
-  const int row = row0 + wave * 32 + n;
-  const bool rvalid = row < nrows;
-  const bool active = row0 + wave * 32 < nrows;    // wave-uniform
-
-  // Key range: cached tiles, then tiles of the new keys; a tile never straddles.
-  const int pre_len = a.plen ? min(max(*a.plen, 0), a.pwidth * a.page_rows) : 0;
-  const int own_len = PREFIX || a.width == 0 ? 0 : min(max(a.lens[b], 0), a.width * a.page_rows);
-  const int len = __builtin_amdgcn_readfirstlane(PREFIX ? pre_len : own_len);
-  const int history = pre_len + own_len;           // what the masks call the cache
-  EndBounds eb{0, 0};
-  if (!PREFIX) eb = end_bounds(a, row0 / a.group, (min(row0 + 32 * RW, nrows) - 1) / a.group);
-  const int n_ct = (len + kPN - 1) / kPN;
-  const int n_tiles = n_ct + (eb.hi + kPN - 1) / kPN;
-  const int t_begin = int(uint32_t(split) * uint32_t(n_tiles) / uint32_t(splits));
-  const int t_end = int(uint32_t(split + 1) * uint32_t(n_tiles) / uint32_t(splits));
-  const int iters = (t_end - t_begin + KW - 1) / KW;             // barrier rounds
-  const int nt = (t_end - t_begin - stream + KW - 1) / KW;       // this stream's tiles
-
-  // This lane's row: query head h0 + gq of query qi of sequence bq.
-  int bq = b, qi = 0, hq = 0;
-  {
-    const uint32_t r = uint32_t(rvalid ? row : nrows - 1);
-    uint32_t rr = r;
-    if (PREFIX) {
-      bq = int(r / uint32_t(a.R));
-      rr = r - uint32_t(bq) * uint32_t(a.R);
+    uint64_t cached = 0;
+    if (a.B == 1) {
+      cached = tiles_of(own_rows(a, 0));
+    } else {
+      for (int b0 = 0; b0 < a.B; b0 += 64)
+        cached += uniform(__shfl(scan64(b0 + lane < a.B ? tiles_of(own_rows(a, b0 + lane)) : 0, lane), 63));
     }
-    qi = int(rr / uint32_t(a.group));
-    hq = hk * a.group + int(rr - uint32_t(qi) * uint32_t(a.group));
+    total = uint64_t(a.Hkv) * (uint64_t(n_rt) * cached + uint64_t(a.B) * fresh);
   }
-  u32x4 qr[KS];
-  {
-    const char* const qp = a.q + bq * a.q_sb + qi * a.q_sl + hq * a.q_sh + 16 * g;
-    const uint32_t flip = a.scale_log2 < 0.f ? (F32 ? 0x80000000u : 0x80008000u) : 0u;
-#pragma unroll
-    for (int s = 0; s < KS; ++s) qr[s] = *reinterpret_cast<const u32x4*>(qp + 32 * s) ^ flip;
+  // The item that holds tile `at` of the line, and the tile's number in it.
+  __device__ __forceinline__ void locate(Args& a, int lane, uint64_t at, int& b, int& hk,
+                                         int& rt, int& t) const {
+    b = 0;
+    uint64_t before = 0;  // tiles of the sequences before b, per head
+    const uint64_t want = udiv(at, a.Hkv);
+    if (a.B > 1) {
+      uint64_t cached = 0;
+      for (int b0 = 0; b0 < a.B; b0 += 64) {
+        const uint64_t own = b0 + lane < a.B ? tiles_of(own_rows(a, b0 + lane)) : 0;
+        const uint64_t upto = cached + scan64(own, lane);
+        // Tiles up to and with this lane's sequence, over all heads, against at.
+        const uint64_t end = uint64_t(n_rt) * upto + uint64_t(b0 + lane + 1) * fresh;
+        const uint64_t hit = __ballot(b0 + lane < a.B && end > want);
+        if (hit) {
+          const int j = __builtin_ctzll(hit);
+          b = b0 + j;
+          before = uniform(__shfl(uint64_t(n_rt) * (upto - own) + uint64_t(b0 + lane) * fresh, j));
+          break;
+        }
+        cached += uniform(__shfl(scan64(own, lane), 63));
+      }
+    }
+    b = __builtin_amdgcn_readfirstlane(b);
+    const uint64_t n_ct = uint64_t(__builtin_amdgcn_readfirstlane(tiles_of(own_rows(a, b))));
+    const uint64_t in_seq = at - before * uint64_t(a.Hkv);
+    const uint64_t per_head = uint64_t(n_rt) * n_ct + fresh;
+    hk = int(udiv(in_seq, per_head));
+    uint64_t r = in_seq - uint64_t(hk) * per_head;
+    rt = 0;
+    if (a.causal || a.n_blocks) {
+      uint64_t base = 0;
+      for (int r0 = 0; r0 < n_rt; r0 += 64) {
+        const uint64_t w = r0 + lane < n_rt ? n_ct + new_tiles<RW>(a, r0 + lane) : 0;
+        const uint64_t upto = base + scan64(w, lane);
+        const uint64_t hit = __ballot(r0 + lane < n_rt && upto > r);
+        if (hit) {
+          const int j = __builtin_ctzll(hit);
+          rt = r0 + j;
+          r -= uniform(__shfl(upto - w, j));
+          break;
+        }
+        base = uniform(__shfl(upto, 63));
+      }
+      t = int(r);
+    } else {
+      const uint64_t w = n_ct + max(tiles_of(a.Lk), 1);
+      rt = int(udiv(r, w));
+      t = int(r - uint64_t(rt) * w);
+    }
+    hk = __builtin_amdgcn_readfirstlane(hk);
+    rt = __builtin_amdgcn_readfirstlane(rt);
+    t = __builtin_amdgcn_readfirstlane(t);
   }
-  const int my_end = PREFIX || !rvalid ? 0 : visible_end(a, qi, history);  // new keys seen
+};
 
-  const int32_t* const table = PREFIX ? a.ptable : a.table + b * a.t_sb;
-  // Page number of the 16 cached rows from r0 (a multiple of 16 below len),
-  // and the first of them within it.
-  auto page_at = [&](int r0, int& in_page) __attribute__((always_inline)) {
-    const uint32_t x = uint32_t(r0) >> 4;
-    const uint32_t e = a.page_magic ? uint32_t((uint64_t(x) * a.page_magic) >> 32) : x;
-    in_page = r0 - int(e) * a.page_rows;
-    return ((const_i32*)reinterpret_cast<uint64_t>(table))[e];
-  };
-  const uint32_t base = lds_addr(smem) + stream * Sh::stream;
-  const int lr = lane / CR, lx = lane % CR;  // row and physical chunk within a piece
-  uint32_t gone = 0;  // two bits per stage: halves of its tile whose table entry names no page
-  // Send this wave's pieces of the stream's tile i: rows [32 / RW wave, ...).
-  auto send = [&](int i) __attribute__((always_inline)) {
-    const int t = t_begin + KW * i + stream;
-    const int st = i % ST;
-    const bool cached = t < n_ct;
-    const int first = (cached ? t : t - n_ct) * kPN;
-    const int count = (cached ? len : eb.hi) - first;  // rows of the tile that exist
-    Rows16 h[2];
-    uint32_t bad = 0;
-    if (cached) {
+// One wave's S tile (TK / 32 blocks of 32 keys), softmax step and PV product.
+template <typename T, int D, int NS>
+struct Tile {
+  static constexpr bool F32 = Elem<T>::bytes == 4;
+  static constexpr int RB = D * Elem<T>::bytes, KS = RB / 32, DT = D / 32;
+  f32x16 acc[DT];
+  float m, l;
+
+  __device__ __forceinline__ void reset() {
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        h[x] = {a.q, a.q, 0};
-        const int rows = min(count - 16 * x, 16);
-        if (rows > 0) {
-          int in_page;
-          const int page = page_at(first + 16 * x, in_page);
-          if (uint32_t(page) < uint32_t(a.n_pages)) {
-            const int64_t off = page * a.p_sp + in_page * a.p_sr + hk * a.p_sh;
-            h[x] = {a.pk + off, a.pv + off, rows};
-          } else {
-            bad |= 1u << x;
-          }
+    for (int d = 0; d < DT; ++d) acc[d] = f32x16{};
+    m = -INFINITY;
+    l = 0.f;
+  }
+  static __device__ __forceinline__ void scores(uint32_t ka, const u32x4 (&qr)[KS], f32x16 (&s)[NS]) {
+#pragma unroll
+    for (int x = 0; x < NS; ++x) s[x] = f32x16{};
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int x = 0; x < NS; ++x) {
+        const u32x4 kf = lds_read_b128_at((ka ^ (32u * k)) + 32 * RB * x);
+        if constexpr (F32) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            s[x] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(kf[e]),
+                                                        __uint_as_float(qr[k][e]), s[x], 0, 0, 0);
+        } else {
+          s[x] = Mfma<T>::run(kf, qr[k], s[x]);
         }
       }
-    } else {
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int64_t r = first + 16 * x;
-        h[x] = {a.k + b * a.k_sb + hk * a.k_sh + r * a.k_sl,
-                a.v + b * a.v_sb + hk * a.v_sh + r * a.v_sl, max(min(count - 16 * x, 16), 0)};
-      }
-    }
-    gone = (gone & ~(3u << (2 * st))) | bad << (2 * st);
-    const int sk = int(cached ? a.p_sr : a.k_sl), sv = int(cached ? a.p_sr : a.v_sl);
-    const uint32_t at = base + st * Sh::stage;
-#pragma unroll
-    for (int p = 0; p < PW; ++p) {
-      const int piece = wave * PW + p;                 // of the tile's PW * RW
-      const int x = piece * RPP / 16;                  // half it lies in
-      const Rows16 hx = x ? h[1] : h[0];
-      const int r = piece * RPP % 16 + lr;             // this lane's row of the half
-      const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
-          const_cast<char*>(hx.k), (short)0, hx.rows > 0 ? (hx.rows - 1) * sk + RB : 0, kBufWord3);
-      const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
-          const_cast<char*>(hx.v), (short)0, hx.rows > 0 ? (hx.rows - 1) * sv + RB : 0, kBufWord3);
-      const int tr = piece * RPP + lr;                 // row of the tile
-      const uint32_t past = r < hx.rows ? 0u : 0x80000000u;  // past every bound: zeros
-      dma_piece_at(rk, at + piece * 1024, (uint32_t(r * sk) + 16u * (lx ^ kswz<RB>(tr))) | past);
-      dma_piece_at(rv, at + Sh::tile + piece * 1024,
-                   (uint32_t(r * sv) + 16u * (lx ^ vswz<RB, F32>(tr))) | past);
-    }
-  };
-  for (int i = 0; i < ST - 1 && i < nt; ++i) send(i);
-
-  // c > 0: masked scores are -inf and exp2(-inf c) has to be 0 (a zero scale
-  // weighs every visible key alike: exp2(~0)).
-  const float c = fmaxf(fabsf(a.scale_log2), FLT_MIN);
-  const uint32_t ka = base + n * RB + 16 * (g ^ kswz<RB>(n));
-  uint32_t va;
-  if (F32) {
-    va = base + Sh::tile + 4 * g * RB + 4 * n + 128 * g;
-  } else {
-    const int j = lane & 15, r0 = 4 * g + (j >> 2);
-    va = base + Sh::tile + r0 * RB + 32 * ((lane >> 4) & 1) + 8 * (j & 3) + 16 * vswz<RB, F32>(r0);
   }
-
-  f32x16 acc[DT];
-#pragma unroll
-  for (int d = 0; d < DT; ++d) acc[d] = f32x16{};
-  float m = -INFINITY, l = 0.f;
-  for (int i = 0; i < iters; ++i) {
-    // This wave's pieces of tile i have landed; past the barrier the tile is
-    // whole, and reads of the stage that is sent to next have returned.
-    wait_vmcnt<0>();
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    if (i + ST - 1 < nt) send(i + ST - 1);
-    if (i >= nt || !active) continue;
-    const uint32_t st = uint32_t(i % ST) * Sh::stage;
-    f32x16 s = f32x16{};
-#pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      const u32x4 kf = lds_read_b128_at((ka + st) ^ (32u * k));
-      if constexpr (F32) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(kf[e]),
-                                                   __uint_as_float(qr[k][e]), s, 0, 0, 0);
-      } else {
-        s = Mfma<T>::run(kf, qr[k], s);
-      }
-    }
-    const int t = t_begin + KW * i + stream;
-    const bool cached = t < n_ct;
-    const int j0 = (cached ? t : t - n_ct) * kPN;
-    const uint32_t bad = gone >> (2 * (i % ST)) & 3;
-    if (cached ? j0 + kPN > len : j0 + kPN > eb.lo) {
-      int lim = (cached ? len : my_end) - j0 - 4 * g;
+  // Mask, follow the maximum, exponentials in place. lim: rows of the tile
+  // below it are seen (already less 4 g); bad: 16-row groups without a page.
+  __device__ __forceinline__ void softmax(f32x16 (&s)[NS], bool masked, int lim, uint32_t bad, float c) {
+    if (masked) {
       asm volatile("" : "+v"(lim));
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if (key_hidden(0, r, lim)) s[r] = -INFINITY;
+      for (int x = 0; x < NS; ++x)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (key_hidden(x, r, lim)) s[x][r] = -INFINITY;
     }
     if (bad) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if (bad >> (r / 8) & 1) s[r] = -INFINITY;
+      for (int x = 0; x < NS; ++x)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (bad >> (2 * x + r / 8) & 1) s[x][r] = -INFINITY;
     }
     float tm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-    for (int r = 0; r < 16; ++r) tm[r % 4] = fmaxf(tm[r % 4], s[r]);
+    for (int x = 0; x < NS; ++x)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) tm[r % 4] = fmaxf(tm[r % 4], s[x][r]);
     const float m_new = fmaxf(m, xor32_max(fmaxf(fmaxf(tm[0], tm[1]), fmaxf(tm[2], tm[3]))));
-    if (__any(m_new > m)) {
+    // The reference may lag behind the maximum by up to 2^8 (what is summed is
+    // then up to 2^8 times larger, and divided out): most tiles rescale nothing.
+    if (__any((m_new - m) * c > 8.0f)) {
       if (!__all(m == -INFINITY)) {
         const float corr = m == -INFINITY ? 0.f : fast_exp2((m - m_new) * c);
         l *= corr;
@@ -309,243 +337,749 @@ __global__ __launch_bounds__((64 * Shape<T, D, RW>::NW), 1) void paged_attn_kern
     }
     const float mb = m == -INFINITY ? 0.f : m * c;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = fast_exp2(__builtin_fmaf(s[r], c, -mb));
+    for (int x = 0; x < NS; ++x)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[x][r] = fast_exp2(__builtin_fmaf(s[x][r], c, -mb));
+  }
+  __device__ __forceinline__ void pv(uint32_t va, const f32x16 (&s)[NS]) {
     if constexpr (F32) {
       float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int r = 0; r < 16; ++r) part[r % 4] += s[r];
+      for (int x = 0; x < NS; ++x)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) part[r % 4] += s[x][r];
       l += (part[0] + part[1]) + (part[2] + part[3]);
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
+      for (int x = 0; x < NS; ++x)
 #pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          typedef __attribute__((address_space(3))) float lds_f32;
-          const float vf = *reinterpret_cast<const lds_f32*>(
-              ((va + st) ^ (128u * d)) + (8 * (r / 4) + r % 4) * RB);
-          acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf, s[r], acc[d], 0, 0, 0);
-        }
+        for (int r = 0; r < 16; ++r)
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            typedef __attribute__((address_space(3))) float lds_f32;
+            const float vf = *reinterpret_cast<const lds_f32*>(
+                (va ^ (128u * d)) + (32 * x + 8 * (r / 4) + r % 4) * RB);
+            acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf, s[x][r], acc[d], 0, 0, 0);
+          }
     } else {
-      u32x4 pk[2];
+      u32x4 pk[2 * NS];
       float part[2] = {0.f, 0.f};
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < 2 * NS; ++u)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const uint32_t p = Mfma<T>::pack(s[8 * u + 2 * e], s[8 * u + 2 * e + 1]);
+          const uint32_t p = Mfma<T>::pack(s[u / 2][8 * (u % 2) + 2 * e], s[u / 2][8 * (u % 2) + 2 * e + 1]);
           pk[u][e] = p;
           part[e & 1] = Mfma<T>::sum2(p, part[e & 1]);
         }
       l += part[0] + part[1];
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < 2 * NS; ++u)
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
-          const uint32_t vu = ((va + st) ^ (64u * d)) + 16 * u * RB;
+          const uint32_t vu = (va ^ (64u * d)) + 16 * u * RB;
           const u32x2 lo = lds_read_tr16_at(vu);
           const u32x2 hi = lds_read_tr16_at(vu + 8 * RB);
           acc[d] = Mfma<T>::run(u32x4{lo[0], lo[1], hi[0], hi[1]}, pk[u], acc[d]);
         }
     }
   }
+};
 
-  // The streams' results meet: in each round the upper half hands (m, l, acc)
-  // to the lower, lane by lane ([vector][lane], whole 1 KB rows).
-  float mref = m == -INFINITY ? -INFINITY : m * c;
-  f32x4* const x = reinterpret_cast<f32x4*>(smem);
-#pragma unroll
-  for (int half = KW / 2; half >= 1; half /= 2) {
-    __syncthreads();  // tile reads, or the last round's reads, are done
-    f32x4* const hand = x + ((stream % half) * RW + wave) * (Sh::hand / 16) + lane;
-    if (stream >= half && stream < 2 * half) {
-      hand[0] = f32x4{mref, l, 0.f, 0.f};
-#pragma unroll
-      for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-          hand[64 * (1 + 4 * d + u)] =
-              f32x4{acc[d][4 * u], acc[d][4 * u + 1], acc[d][4 * u + 2], acc[d][4 * u + 3]};
-    }
-    __syncthreads();
-    if (stream < half) {
-      const f32x4 o = hand[0];
-      const float mm = fmaxf(mref, o[0]), ref = mm == -INFINITY ? 0.f : mm;
-      const float w0 = fast_exp2(mref - ref), w1 = fast_exp2(o[0] - ref);
-      l = __builtin_fmaf(l, w0, o[1] * w1);
-      mref = mm;
-#pragma unroll
-      for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const f32x4 v = hand[64 * (1 + 4 * d + u)];
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            acc[d][4 * u + e] = __builtin_fmaf(acc[d][4 * u + e], w0, v[e] * w1);
-        }
-    }
-  }
-  if (stream != 0 || !active) return;
-  l = xor32_sum(l);
+// Where an item's keys lie, in scalar registers.
+struct Keys {
+  uint64_t pk, pv, nk, nv, table;  // pages and new keys of this head; the sequence's table
+  int64_t p_sp;
+  int p_sr, k_sl, v_sl;
+  uint32_t magic;
+  int page_rows, n_pages;
+  int len, fresh;  // cached rows, new rows that some row of the item sees
+  int n_ct;        // 32-key tiles of the cached rows; the new ones' follow
 
-  float* const part_o = PREFIX ? a.pre_o : a.own_o;
-  if (part_o == nullptr) {
-    // The only part: the result. No visible key: 0 * inf = NaN, as the
-    // reference's softmax.
-    if (!rvalid) return;
-    const float inv = 1.0f / l;
-    char* const op = a.out + bq * a.o_sb + qi * a.o_sl + hq * a.o_sh + 4 * g * Elem<T>::bytes;
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const f32x4 r = {acc[d][4 * u] * inv, acc[d][4 * u + 1] * inv, acc[d][4 * u + 2] * inv,
-                         acc[d][4 * u + 3] * inv};
-        if constexpr (F32)
-          *reinterpret_cast<f32x4*>(op + 128 * d + 32 * u) = r;
-        else
-          *reinterpret_cast<u32x2*>(op + 64 * d + 16 * u) =
-              u32x2{Mfma<T>::pack(r[0], r[1]), Mfma<T>::pack(r[2], r[3])};
-      }
-    return;
+  // The 16 rows from row r0 of the cached ones, or of the new ones: addresses,
+  // and how many exist. True where the table names no page for them.
+  __device__ __forceinline__ bool find(bool cached, int r0, uint64_t& k, uint64_t& v, int& rows) const {
+    rows = max(min((cached ? len : fresh) - r0, 16), 0);
+    bool gone = false;
+    if (cached) {
+      // Entry of these rows (the table has one for every row below len).
+      const uint32_t x16 = uint32_t(r0) >> 4;
+      uint32_t e = magic ? uint32_t((uint64_t(x16) * magic) >> 32) : x16;
+      e = rows > 0 ? e : 0;
+      const int page = rows > 0 ? ((const_i32*)table)[e] : 0;
+      gone = uint32_t(page) >= uint32_t(n_pages);
+      rows = gone ? 0 : rows;
+      const uint64_t off = uint64_t(page * p_sp) + uint64_t(uint32_t(r0) - e * uint32_t(page_rows)) * uint32_t(p_sr);
+      k = pk + off;
+      v = pv + off;
+    } else {
+      k = nk + uint64_t(uint32_t(r0)) * uint32_t(k_sl);
+      v = nv + uint64_t(uint32_t(r0)) * uint32_t(v_sl);
+    }
+    k = uniform(k);
+    v = uniform(v);
+    rows = __builtin_amdgcn_readfirstlane(rows);
+    return gone;
   }
-  const int blk = rt * RW + wave;
-  const int64_t unit = (PREFIX ? int64_t(hk) * a.pre_blocks + blk
-                               : (int64_t(hk) * a.B + b) * a.own_blocks + blk) * splits + split;
-  float* const part_ml = (PREFIX ? a.pre_ml : a.own_ml) + unit * 64;
-  if (g == 0) *reinterpret_cast<f32x2*>(part_ml + 2 * n) = f32x2{mref, l};
-  if (__all(l == 0.f)) return;  // nothing seen: the merge does not read acc where l is 0
-  f32x4* const po = reinterpret_cast<f32x4*>(part_o) + unit * (8 * D) + lane;
+};
+
+// DMA of `pieces` pieces (RPP rows each) of a 16-row group at `from`, `rows` of
+// which exist, into LDS bytes from `to`; r0: the first row within the group, tr0:
+// within the tile (multiples of RPP). K swizzle or V swizzle.
+template <int RB, bool F32, bool K>
+__device__ __forceinline__ void send_rows(uint64_t from, int rows, int step, uint32_t to, int r0, int tr0,
+                                          int pieces, int lane) {
+  constexpr int CR = RB / 16, RPP = 64 / CR;
+  const int lr = lane / CR, lx = lane % CR;  // row and physical chunk within a piece
+  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+      reinterpret_cast<char*>(from), (short)0, rows > 0 ? (rows - 1) * step + RB : 0, kBufWord3);
 #pragma unroll
-  for (int d = 0; d < DT; ++d)
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-      po[64 * (4 * d + u)] =
-          f32x4{acc[d][4 * u], acc[d][4 * u + 1], acc[d][4 * u + 2], acc[d][4 * u + 3]};
+  for (int p = 0; p < pieces; ++p) {
+    const int r = r0 + p * RPP + lr, tr = tr0 + p * RPP + lr;
+    const uint32_t past = r < rows ? 0u : 0x80000000u;  // past every bound: zeros
+    const int swz = K ? kswz<RB>(tr) : vswz<RB, F32>(tr);
+    dma_piece_at(rs, to + p * 1024, (uint32_t(r * step) + 16u * (lx ^ swz)) | past);
+  }
 }
 
-// Join the parts of 32 rows of one (K/V head, sequence), 32 of their D values
-// per workgroup (blockIdx.y): thread (u, lane) holds 4 values of row lane % 32.
-// Prefix parts are numbered over all sequences' rows, so a unit's rows may
-// begin in the middle of one. A part that saw nothing has l = 0 and is not read.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
-  const int lane = int(threadIdx.x) & 63, u = int(threadIdx.x) >> 6, d = int(blockIdx.y);
-  const int g = lane >> 5, n = lane & 31;
-  uint32_t i = blockIdx.x;
-  const int blk = int(i % uint32_t(a.own_blocks));
-  i /= uint32_t(a.own_blocks);
-  const int b = int(i % uint32_t(a.B)), hk = int(i / uint32_t(a.B));
-  const int row = blk * 32 + n;
-  if (row >= a.R) return;
-  const int64_t own = ((int64_t(hk) * a.B + b) * a.own_blocks + blk) * a.own_splits;
-  const uint32_t pr = uint32_t(b) * uint32_t(a.R) + uint32_t(row);
-  const int64_t pre = (int64_t(hk) * a.pre_blocks + (pr >> 5)) * a.pre_splits;
-  const int pn = int(pr & 31);
-  const f32x2* const own_ml = reinterpret_cast<const f32x2*>(a.own_ml) + own * 32 + n;
-  const f32x2* const pre_ml = reinterpret_cast<const f32x2*>(a.pre_ml) + pre * 32 + pn;
-  float m = -INFINITY;
-  for (int s = 0; s < a.own_splits; ++s) m = fmaxf(m, own_ml[32 * s][0]);
-  for (int s = 0; s < a.pre_splits; ++s) m = fmaxf(m, pre_ml[32 * s][0]);
-  const f32x4* const own_o = reinterpret_cast<const f32x4*>(a.own_o) + own * (8 * D) +
-                             64 * (4 * d + u) + lane;
-  const f32x4* const pre_o = reinterpret_cast<const f32x4*>(a.pre_o) + pre * (8 * D) +
-                             64 * (4 * d + u) + 32 * g + pn;
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  float l = 0.f;
-  auto join = [&](const f32x2 ml, const f32x4* o) __attribute__((always_inline)) {
-    if (ml[1] == 0.f) return;
-    const float w = fast_exp2(ml[0] - m);
-    l = __builtin_fmaf(ml[1], w, l);
-    const f32x4 v = *o;
+// One workgroup's share of a line: workgroup w of n.
+template <typename T, int D, int RW, bool PREFIX, bool SHARED>
+__device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uint32_t n,
+                                         uint64_t total, int line_rt, uint64_t line_fresh) {
+  using Sh = Shape<T, D, RW>;
+  constexpr int RB = Sh::RB, KW = Sh::KW, TK = Sh::TK, CR = RB / 16, RPP = 64 / CR;
+  using Ti = Tile<T, D, TK / 32>;
+  constexpr bool F32 = Ti::F32;
+  constexpr int KS = Ti::KS;
+  constexpr int UT = TK / kPN;  // 32-key tiles that a stream takes at a time
+  const int wid = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
+  const int stream = wid / RW, wave = wid % RW, lane = int(threadIdx.x) & 63;
+  const int g = lane >> 5, nl = lane & 31;
+
+  // Cut: tiles [w T / n, (w + 1) T / n) of the line, from tile t0 of an item on.
+  // Split: range t0 (for now) of an item.
+  uint64_t at = 0;
+  int todo = 1;  // tiles left to do (the host limits a workgroup's share to 31 bits)
+  int b = 0, hk = 0, rt = 0, t0 = 0;
+  int n_rt, splits;
+  {
+    Args& a = *reread(args);
+    const int nrows = PREFIX ? a.B * a.R : a.R;
+    n_rt = __builtin_amdgcn_readfirstlane((nrows + 32 * RW - 1) / (32 * RW));
+    splits = __builtin_amdgcn_readfirstlane(PREFIX ? a.pre.splits : a.own.splits);
+    if (splits == 0) {
+      at = uniform(udiv(uint64_t(w) * total, n));
+      todo = __builtin_amdgcn_readfirstlane(int(udiv(uint64_t(w + 1) * total, n) - at));
+      if (todo > 0) {
+        if (PREFIX) {
+          const uint64_t pre_w = uint64_t(max(tiles_of(prefix_rows(a)), 1));
+          const uint64_t item = udiv(at, pre_w);
+          t0 = int(at - item * pre_w);
+          hk = int(uint32_t(item) / uint32_t(n_rt));
+          rt = int(uint32_t(item) - uint32_t(hk) * uint32_t(n_rt));
+        } else {
+          const OwnLine<RW> line{line_rt, line_fresh, total};
+          line.locate(a, lane, at, b, hk, rt, t0);
+        }
+      }
+    } else {
+      // Groups (sequence and head) to XCDs in runs; there, range by range of the
+      // keys, group by group, late row tiles (most keys under a causal mask) first.
+      const uint32_t G = uint32_t(PREFIX ? a.Hkv : a.B * a.Hkv);
+      uint32_t grp0 = 0, groups = G, i = w;
+      if (G % 8 == 0) {
+        groups = G / 8;
+        grp0 = w % 8 * groups;
+        i = w / 8;
+      }
+      const uint32_t range = i / (groups * uint32_t(n_rt));
+      i -= range * (groups * uint32_t(n_rt));
+      const uint32_t grp = i / uint32_t(n_rt);
+      rt = n_rt - 1 - int(i - grp * uint32_t(n_rt));
+      t0 = int(range);
+      b = int((grp0 + grp) / uint32_t(a.Hkv));
+      hk = int(grp0 + grp) - b * a.Hkv;
+      if (PREFIX) b = 0;
+    }
+  }
+  Record left{0, 0, 0, 0};
+
+  while (todo > 0) {
+    // The item and this share's tiles [t0, t1) of it, in scalar registers.
+    b = __builtin_amdgcn_readfirstlane(b);
+    hk = __builtin_amdgcn_readfirstlane(hk);
+    rt = __builtin_amdgcn_readfirstlane(rt);
+    t0 = __builtin_amdgcn_readfirstlane(t0);
+    const int row0 = rt * 32 * RW;
+    Keys keys;
+    u32x4 qr[KS];
+    float c;
+    int my_end = 0, full_end, t1, weight, nt, iters, item;
+    uint32_t slot;
+    const bool first = t0 == 0;  // this share holds the item's first tile: it leaves the record
+    bool active;
+    {
+      Args& a = *reread(args);
+      const int nrows = PREFIX ? a.B * a.R : a.R;
+      const int pre_len = __builtin_amdgcn_readfirstlane(prefix_rows(a));
+      const int own_len = PREFIX ? 0 : __builtin_amdgcn_readfirstlane(own_rows(a, b));
+      const int history = pre_len + own_len;  // what the masks call the cache
+      EndBounds eb{0, 0};
+      if (!PREFIX) eb = end_bounds(a, row0 / a.group, (min(row0 + 32 * RW, nrows) - 1) / a.group);
+      full_end = eb.lo;
+      keys.len = PREFIX ? pre_len : own_len;
+      keys.fresh = __builtin_amdgcn_readfirstlane(eb.hi);
+      keys.n_ct = tiles_of(keys.len);
+      weight = max(keys.n_ct, 1);
+      if (!PREFIX) weight = keys.n_ct + max(tiles_of(keys.fresh), 1);
+      item = PREFIX ? hk * n_rt + rt : (b * a.Hkv + hk) * n_rt + rt;
+      if (splits == 0) {
+        t1 = __builtin_amdgcn_readfirstlane(min(weight - t0, todo) + t0);
+        // Without a prefix a workgroup breaks two items at most; with one, every
+        // item has parts, and (workgroup, item) grow together.
+        slot = SHARED ? w + uint32_t(item) : 2 * w + uint32_t(first);
+      } else {
+        slot = uint32_t(item) * uint32_t(splits) + uint32_t(t0);
+        t1 = int(uint64_t(weight) * uint32_t(t0 + 1) / uint32_t(splits));
+        t0 = __builtin_amdgcn_readfirstlane(int(uint64_t(weight) * uint32_t(t0) / uint32_t(splits)));
+        t1 = __builtin_amdgcn_readfirstlane(t1);
+      }
+      const int count = __builtin_amdgcn_readfirstlane(
+          max(min(t1, keys.n_ct + tiles_of(keys.fresh)) - t0, 0));  // tiles that exist
+      iters = (count + KW * UT - 1) / (KW * UT);  // barrier rounds
+      // How many tiles this stream takes (the last may be past t1: it is masked).
+      nt = stream < KW && count > stream * UT ? (count - stream * UT + KW * UT - 1) / (KW * UT) : 0;
+      keys.pk = reinterpret_cast<uint64_t>(a.pk) + uint64_t(hk * a.p_sh);
+      keys.pv = reinterpret_cast<uint64_t>(a.pv) + uint64_t(hk * a.p_sh);
+      keys.nk = reinterpret_cast<uint64_t>(a.k) + uint64_t(b * a.k_sb + hk * a.k_sh);
+      keys.nv = reinterpret_cast<uint64_t>(a.v) + uint64_t(b * a.v_sb + hk * a.v_sh);
+      keys.table = reinterpret_cast<uint64_t>(PREFIX ? a.ptable : a.table + b * a.t_sb);
+      keys.p_sp = a.p_sp;
+      keys.p_sr = int(a.p_sr);
+      keys.k_sl = int(a.k_sl);
+      keys.v_sl = int(a.v_sl);
+      keys.magic = a.page_magic;
+      keys.page_rows = a.page_rows;
+      keys.n_pages = a.n_pages;
+      c = fmaxf(fabsf(a.scale_log2), FLT_MIN);
+
+      // This lane's row: query head hq of query qi of sequence bq.
+      const int row = row0 + wave * 32 + nl;
+      const bool rvalid = row < nrows;
+      active = row0 + wave * 32 < nrows && stream < KW;  // wave-uniform
+      int bq = b;
+      const uint32_t r = uint32_t(rvalid ? row : nrows - 1);
+      uint32_t rr = r;
+      if (PREFIX) {
+        bq = int(r / uint32_t(a.R));
+        rr = r - uint32_t(bq) * uint32_t(a.R);
+      }
+      const int qi = int(rr / uint32_t(a.group));
+      const int hq = hk * a.group + int(rr - uint32_t(qi) * uint32_t(a.group));
+      const char* const qp = a.q + bq * a.q_sb + qi * a.q_sl + hq * a.q_sh + 16 * g;
+      const uint32_t flip = a.scale_log2 < 0.f ? (F32 ? 0x80000000u : 0x80008000u) : 0u;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(v[e], w, acc[e]);
+      for (int s = 0; s < KS; ++s) qr[s] = *reinterpret_cast<const u32x4*>(qp + 32 * s) ^ flip;
+      if (!PREFIX && rvalid) my_end = visible_end(a, qi, history);  // new keys seen
+    }
+
+    const uint32_t base = lds_addr(smem) + stream * Sh::stream;
+    const uint32_t ka = base + nl * RB + 16 * (g ^ kswz<RB>(nl));
+    uint32_t va;
+    if (F32) {
+      va = base + Sh::tile + 4 * g * RB + 4 * nl + 128 * g;
+    } else {
+      const int j = lane & 15, r0 = 4 * g + (j >> 2);
+      va = base + Sh::tile + r0 * RB + 32 * ((lane >> 4) & 1) + 8 * (j & 3) + 16 * vswz<RB, F32>(r0);
+    }
+    // A stream's i-th 32-key tile. A 64-key one may begin with the last cached
+    // tile and end with the first new one: its halves are found one by one.
+    auto tile_at = [&](int i) __attribute__((always_inline)) { return t0 + (KW * i + stream) * UT; };
+    Ti ti;
+    ti.reset();
+    // Mask of tile i: rows of it that are seen, less 4 g, per 32-key block; all
+    // of it where `masked` comes back false.
+    auto limits = [&](int t, bool& masked) __attribute__((always_inline)) {
+      const bool cached = t < keys.n_ct;
+      const int j0 = (cached ? t : t - keys.n_ct) * kPN;
+      masked = t >= t1 || (cached ? j0 + kPN > keys.len : j0 + kPN > full_end);
+      return t >= t1 ? -64 : (cached ? keys.len : my_end) - j0 - 4 * g;
+    };
+    if constexpr (RW == 1) {
+      // Streams of one wave: no barriers, each wave waits for its own pieces.
+      constexpr int HP = 16 / RPP;  // pieces of a 16-row group
+      uint64_t k0, v0, k1, v1;
+      int rows0, rows1, sv = 0;
+      uint32_t gone = 0;
+      auto find = [&](int t) __attribute__((always_inline)) {
+        const bool cached = t < keys.n_ct;
+        const int r0 = (cached ? t : t - keys.n_ct) * kPN;
+        gone = keys.find(cached, r0, k0, v0, rows0) ? 1 : 0;
+        gone |= keys.find(cached, r0 + 16, k1, v1, rows1) ? 2 : 0;
+        const int sk = __builtin_amdgcn_readfirstlane(cached ? keys.p_sr : keys.k_sl);
+        sv = __builtin_amdgcn_readfirstlane(cached ? keys.p_sr : keys.v_sl);
+        send_rows<RB, F32, true>(k0, rows0, sk, base, 0, 0, HP, lane);
+        send_rows<RB, F32, true>(k1, rows1, sk, base + 16 * RB, 0, 16, HP, lane);
+      };
+      auto send_v = [&]() __attribute__((always_inline)) {
+        send_rows<RB, F32, false>(v0, rows0, sv, base + Sh::tile, 0, 0, HP, lane);
+        send_rows<RB, F32, false>(v1, rows1, sv, base + Sh::tile + 16 * RB, 0, 16, HP, lane);
+      };
+      if (nt > 0) {
+        find(tile_at(0));
+        send_v();
+      }
+      for (int i = 0; i < nt; ++i) {
+        const bool more = i + 1 < nt;
+        const uint32_t bad = gone;
+        wait_vmcnt<2 * HP>();  // K of tile i (its V was sent last)
+        f32x16 s[1];
+        Ti::scores(ka, qr, s);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K is read: its place is free
+        if (more) find(tile_at(i + 1));
+        bool masked;
+        const int lim = limits(tile_at(i), masked);
+        ti.softmax(s, masked, lim, bad, c);
+        if (more) wait_vmcnt<2 * HP>();  // V of tile i (the next K was sent last)
+        else wait_vmcnt<0>();
+        ti.pv(va, s);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (more) send_v();
+      }
+    } else {
+      // Each wave of a stream fetches TK / RW rows of a tile, all in one page.
+      constexpr int WR = TK / RW;
+      static_assert(16 % WR == 0 && WR % RPP == 0, "a wave's rows lie in one 16-row group");
+      uint32_t* const flags = reinterpret_cast<uint32_t*>(smem + Sh::flags) + stream * 2 * 4;
+      auto send_tile = [&](int i) __attribute__((always_inline)) {
+        const int st = i & 1;
+        const int tr = wave * WR;                 // this wave's first row of the tile
+        const int t = tile_at(i) + tr / kPN;      // 32-key tile it lies in
+        const bool cached = t < keys.n_ct;
+        const int r0 = (cached ? t : t - keys.n_ct) * kPN + tr % kPN / 16 * 16;
+        uint64_t k, v;
+        int rows;
+        const bool gone = keys.find(cached, r0, k, v, rows);
+        if (lane == 0) flags[4 * st + wave] = gone ? 1u : 0u;
+        const int sk = __builtin_amdgcn_readfirstlane(cached ? keys.p_sr : keys.k_sl);
+        const int sv = __builtin_amdgcn_readfirstlane(cached ? keys.p_sr : keys.v_sl);
+        const uint32_t to = base + st * 2 * Sh::tile + tr * RB;
+        send_rows<RB, F32, true>(k, rows, sk, to, tr % 16, tr, WR / RPP, lane);
+        send_rows<RB, F32, false>(v, rows, sv, to + Sh::tile, tr % 16, tr, WR / RPP, lane);
+      };
+      if (nt > 0) send_tile(0);
+      for (int i = 0; i < iters; ++i) {
+        // This wave's pieces of tile i have landed; past the barrier the tile
+        // is whole, and reads of the stage that is sent to next have returned.
+        wait_vmcnt<0>();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (i + 1 < nt) send_tile(i + 1);
+        if (i >= nt || !active) continue;
+        const uint32_t st = uint32_t(i & 1) * 2 * Sh::tile;
+        const u32x4 fl = *reinterpret_cast<const u32x4*>(flags + 4 * (i & 1));
+        f32x16 s[UT];
+        Ti::scores(ka + st, qr, s);
+        const int t = tile_at(i);
+        bool masked, masked1 = false;
+        int lim = limits(t, masked);
+        if constexpr (UT == 2) {
+          // The second block counts its rows from 32 on.
+          const int lim1 = limits(t + 1, masked1) + kPN;
+          if (masked || masked1) {
+            if (!masked) lim = kPN;
+            // Blocks of one source: one limit does. Else mask each by its own.
+            asm volatile("" : "+v"(lim));
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              if (key_hidden(0, r, lim)) s[0][r] = -INFINITY;
+              if (masked1 && key_hidden(1, r, lim1)) s[1][r] = -INFINITY;
+            }
+          }
+          masked = false;
+        }
+        uint32_t bad = 0;
+        if (__builtin_amdgcn_readfirstlane(int(fl[0] | fl[1] | fl[2] | fl[3]))) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) bad |= fl[x] << (x * WR / 16);
+          bad = uint32_t(__builtin_amdgcn_readfirstlane(int(bad)));
+        }
+        ti.softmax(s, masked, lim, bad, c);
+        ti.pv(va + st, s);
+      }
+    }
+
+    // The streams' results meet in LDS. Thread j of a row takes 8 of its
+    // values: it reads them from every stream and weighs them by its maximum.
+    const bool whole = first && t1 == weight && splits <= 1;
+    const float mref = ti.m == -INFINITY ? -INFINITY : ti.m * c;
+    const float lsum = xor32_sum(ti.l);
+    Args& a = *reread(args);
+    const int nrows = PREFIX ? a.B * a.R : a.R;
+#pragma unroll
+    for (int pass = 0; pass < D / Sh::DP; ++pass) {
+      __syncthreads();  // tile reads, or the last pass's reads, are done
+      if (stream < KW) {
+        char* const area = smem + wid * Sh::area;
+#pragma unroll
+        for (int d = 0; d < Sh::DP / 32; ++d)
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const f32x16& v = ti.acc[pass * (Sh::DP / 32) + d];
+            *reinterpret_cast<f32x4*>(area + (4 * d + u) * Sh::vec + 16 * lane) =
+                f32x4{v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]};
+          }
+        if (g == 0)
+          *reinterpret_cast<f32x2*>(area + Sh::DP / 8 * Sh::vec + 8 * nl) = f32x2{mref, lsum};
+      }
+      __syncthreads();
+      constexpr int CD = Sh::DP / 8;  // 8-value chunks of a row in this pass
+#pragma unroll 1
+      for (int e = 0; e < (RW * 32 * CD + kThreads - 1) / kThreads; ++e) {
+        const int u = e * kThreads + int(threadIdx.x);
+        const int r = u / CD, ch = u % CD;  // row of the item, chunk
+        if (r < 32 * RW && row0 + r < nrows) {
+          const char* const area = smem + (r / 32) * Sh::area;
+          f32x2 ml[KW];
+          float mm = -INFINITY;
+#pragma unroll
+          for (int s = 0; s < KW; ++s) {
+            ml[s] = *reinterpret_cast<const f32x2*>(area + s * RW * Sh::area + CD * Sh::vec + 8 * (r % 32));
+            mm = fmaxf(mm, ml[s][0]);
+          }
+          const float ref = mm == -INFINITY ? 0.f : mm;
+          float l = 0.f;
+          f32x4 o[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+          for (int s = 0; s < KW; ++s) {
+            const float wt = fast_exp2(ml[s][0] - ref);
+            l = __builtin_fmaf(ml[s][1], wt, l);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const f32x4 v = *reinterpret_cast<const f32x4*>(area + s * RW * Sh::area + ch * Sh::vec +
+                                                              16 * (r % 32 + 32 * x));
+#pragma unroll
+              for (int y = 0; y < 4; ++y) o[x][y] = __builtin_fmaf(v[y], wt, o[x][y]);
+            }
+          }
+          const int col = pass * Sh::DP + 8 * ch;
+          if (!SHARED && whole) {
+            // The result. No visible key: 0 * inf = NaN, as the reference's softmax.
+            const float inv = 1.0f / l;
+            const uint32_t rr = uint32_t(row0 + r);
+            const int qo = int(rr / uint32_t(a.group));
+            const int ho = hk * a.group + int(rr - uint32_t(qo) * uint32_t(a.group));
+            char* const op = a.out + b * a.o_sb + qo * a.o_sl + ho * a.o_sh + col * Elem<T>::bytes;
+            if constexpr (F32) {
+              reinterpret_cast<f32x4*>(op)[0] = o[0] * inv;
+              reinterpret_cast<f32x4*>(op)[1] = o[1] * inv;
+            } else {
+              *reinterpret_cast<u32x4*>(op) =
+                  u32x4{Mfma<T>::pack(o[0][0] * inv, o[0][1] * inv), Mfma<T>::pack(o[0][2] * inv, o[0][3] * inv),
+                        Mfma<T>::pack(o[1][0] * inv, o[1][1] * inv), Mfma<T>::pack(o[1][2] * inv, o[1][3] * inv)};
+            }
+          } else {
+            const int64_t at_row = int64_t(slot) * (32 * RW) + r;
+            f32x4* const po = reinterpret_cast<f32x4*>((PREFIX ? a.pre.o : a.own.o) + at_row * D + col);
+            po[0] = o[0];
+            po[1] = o[1];
+            if (col == 0)
+              *reinterpret_cast<f32x2*>((PREFIX ? a.pre.ml : a.own.ml) + at_row * 2) = f32x2{mm, l};
+          }
+        }
+      }
+    }
+    if (first && (SHARED || !whole)) {
+      left = Record{item, int(slot), splits, 0};
+      if (splits == 0) {
+        // Up to the workgroup that holds the item's last tile.
+        const uint64_t last = udiv((at + uint64_t(weight)) * n - 1, total);
+        left.parts = int(last) - int(w) + 1;
+      }
+      if ((SHARED || splits) && threadIdx.x == 0) (PREFIX ? a.pre.rec : a.own.rec)[item] = left;
+    }
+    if (splits) return;
+    __syncthreads();  // the results are read: tiles may land again
+    at = uniform(at + uint64_t(t1 - t0));
+    todo = __builtin_amdgcn_readfirstlane(todo - (t1 - t0));
+    t0 = 0;
+    if (++rt == n_rt) {
+      rt = 0;
+      if (++hk == a.Hkv) {
+        hk = 0;
+        ++b;
+      }
+    }
+  }
+  if (!SHARED && splits == 0 && threadIdx.x == 0) args->own.rec[w] = left;
+}
+
+// Tiles that a workgroup should have before more of them are put to work.
+template <typename T, int D, int RW> constexpr int kMinTiles = Shape<T, D, RW>::KW * Shape<T, D, RW>::TK / kPN * 2;
+
+template <typename T, int D, int RWP, int RWO>
+__global__ __launch_bounds__(kThreads, 1) void paged_attn_kernel(PagedArgs) {
+  Args* const args = (Args*)(uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
+  Args& a = *reread(args);
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int lane = int(threadIdx.x) & 63;
+  OwnLine<RWO> own{};
+  const uint32_t grid = gridDim.x;
+  if (a.own.splits == 0) own.init(a, lane);
+  auto wanted = [&](uint64_t tiles, int least, uint32_t most) __attribute__((always_inline)) {
+    const uint64_t x = (tiles + least - 1) / least;
+    return x < most ? uint32_t(x) : most;
   };
-  for (int s = 0; s < a.pre_splits; ++s) join(pre_ml[32 * s], pre_o + int64_t(s) * (8 * D));
-  for (int s = 0; s < a.own_splits; ++s) join(own_ml[32 * s], own_o + int64_t(s) * (8 * D));
+  // Workgroups of each line, the prefix's first.
+  uint32_t n_own, n_pre = 0;
+  uint64_t pre_total = 0;
+  if constexpr (RWP > 0) {
+    const uint32_t pre_items = uint32_t(a.Hkv) * uint32_t((a.B * a.R + 32 * RWP - 1) / (32 * RWP));
+    pre_total = uint64_t(pre_items) * max(tiles_of(prefix_rows(a)), 1);
+    if (a.pre.splits) n_pre = pre_items * uint32_t(a.pre.splits);
+    else n_pre = wanted(pre_total, kMinTiles<T, D, RWP>, grid);
+  }
+  if (a.own.splits) {
+    n_own = uint32_t(a.B * a.Hkv) * uint32_t((a.R + 32 * RWO - 1) / (32 * RWO)) * uint32_t(a.own.splits);
+  } else {
+    n_own = wanted(own.total, kMinTiles<T, D, RWO>, uint32_t(a.own_n));
+    if (RWP > 0 && a.pre.splits == 0 && n_pre + n_own > grid) {
+      // Both are cut: in proportion to their tiles.
+      const float part = float(pre_total) / float(pre_total + own.total);
+      n_pre = uint32_t(part * float(grid) + 0.5f);
+      n_pre = min(max(n_pre, 1u), grid - 1);
+      n_own = grid - n_pre;
+    }
+  }
+  n_pre = uint32_t(__builtin_amdgcn_readfirstlane(int(n_pre)));
+  n_own = uint32_t(__builtin_amdgcn_readfirstlane(int(n_own)));
+  uint32_t w = blockIdx.x;
+  if (w >= n_pre + n_own) {
+    if (RWP == 0 && threadIdx.x == 0) a.own.rec[w] = Record{0, 0, 0, 0};
+    return;
+  }
+  // Workgroup i runs on XCD i % 8: consecutive pieces of a cut line, which may
+  // share keys, go to one XCD's L2.
+  auto in_runs = [](uint32_t i, uint32_t n) __attribute__((always_inline)) {
+    const uint32_t n8 = n & ~7u;
+    return i < n8 ? i % 8 * (n8 / 8) + i / 8 : i;
+  };
+  if constexpr (RWP > 0) {
+    if (w < n_pre) {
+      if (a.pre.splits == 0) w = in_runs(w, n_pre);
+      run_line<T, D, RWP, true, true>(args, smem, w, n_pre, pre_total, 0, 0);
+      return;
+    }
+  }
+  w -= n_pre;
+  if (a.own.splits == 0) w = in_runs(w, n_own);
+  run_line<T, D, RWO, false, (RWP > 0)>(args, smem, w, n_own, own.total, own.n_rt, own.fresh);
+}
+
+// Join the parts of 32 rows of an item, D / gridDim.z of their values: a thread
+// holds 8 values of a row. blockIdx.x is a record. Prefix items are over all
+// sequences' rows, so the rows here may be those of two. A part that saw nothing
+// has l = 0.
+template <typename T, int D, int RWP, int RWO>
+__global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
+  const Record rec = a.own.rec[blockIdx.x];
+  if (rec.parts == 0) return;
+  const int n_rt = (a.R + 32 * RWO - 1) / (32 * RWO);
+  constexpr int CD = 8;  // 8-value chunks of a row here: 64 values
+  const int r = int(threadIdx.x) / CD, ch = int(blockIdx.z) * CD + int(threadIdx.x) % CD;
+  const int in_item = int(blockIdx.y) * 32 + r;
+  const int rt = rec.item % n_rt, bh = rec.item / n_rt;
+  const int b = bh / a.Hkv, hk = bh % a.Hkv;
+  const int row = rt * 32 * RWO + in_item;
+  if (row >= a.R) return;
+  // Rows of the parts in each line: part p of the own keys, and of the prefix.
+  auto own_row = [&](int p) __attribute__((always_inline)) {
+    // Of a cut line without a prefix, a broken item's first part is its
+    // workgroup's odd slot, the others are the next workgroups' even ones.
+    const int64_t slot = RWP == 0 && a.own.splits == 0
+                             ? int64_t(rec.slot) + (p ? 2 * p - 1 : 0) : int64_t(rec.slot) + p;
+    return slot * (32 * RWO) + in_item;
+  };
+  int pre_parts = 0;
+  int64_t pre_row = 0;
+  if constexpr (RWP > 0) {
+    const int pr = b * a.R + row;
+    const int pre_rt = (a.B * a.R + 32 * RWP - 1) / (32 * RWP);
+    const Record p = a.pre.rec[hk * pre_rt + pr / (32 * RWP)];
+    pre_parts = p.parts;
+    pre_row = int64_t(p.slot) * (32 * RWP) + pr % (32 * RWP);
+  }
+  float m = -INFINITY, l = 0.f;
+  f32x4 o[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+  // Four parts at a time: their loads do not wait for one another.
+  auto join = [&](const Line& line, int parts, auto row_of) __attribute__((always_inline)) {
+    for (int p0 = 0; p0 < parts; p0 += 4) {
+      f32x2 ml[4];
+      f32x4 v[4][2];
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        const int64_t at = row_of(min(p0 + p, parts - 1));
+        ml[p] = *reinterpret_cast<const f32x2*>(line.ml + at * 2);
+        const f32x4* const x = reinterpret_cast<const f32x4*>(line.o + at * D + 8 * ch);
+        v[p][0] = x[0];
+        v[p][1] = x[1];
+        if (p0 + p >= parts) ml[p] = f32x2{-INFINITY, 0.f};
+      }
+      float mm = m;
+#pragma unroll
+      for (int p = 0; p < 4; ++p) mm = fmaxf(mm, ml[p][0]);
+      const float ref = mm == -INFINITY ? 0.f : mm;
+      const float keep = fast_exp2(m - ref);
+      l *= keep;
+      o[0] *= keep;
+      o[1] *= keep;
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        const float wt = fast_exp2(ml[p][0] - ref);
+        if (p0 + p < parts) {
+          l = __builtin_fmaf(ml[p][1], wt, l);
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            o[0][y] = __builtin_fmaf(v[p][0][y], wt, o[0][y]);
+            o[1][y] = __builtin_fmaf(v[p][1][y], wt, o[1][y]);
+          }
+        }
+      }
+      m = mm;
+    }
+  };
+  if constexpr (RWP > 0)
+    join(a.pre, pre_parts, [&](int p) { return pre_row + int64_t(p) * (32 * RWP); });
+  join(a.own, rec.parts, own_row);
   const float inv = 1.0f / l;  // no visible key: 0 * inf = NaN
   const int qi = row / a.group, hq = hk * a.group + row % a.group;
-  char* const op = a.out + b * a.o_sb + qi * a.o_sl + hq * a.o_sh +
-                   (32 * d + 8 * u + 4 * g) * Elem<T>::bytes;
-  const f32x4 r = {acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv};
-  if constexpr (Elem<T>::bytes == 4)
-    *reinterpret_cast<f32x4*>(op) = r;
-  else
-    *reinterpret_cast<u32x2*>(op) = u32x2{Mfma<T>::pack(r[0], r[1]), Mfma<T>::pack(r[2], r[3])};
+  char* const op = a.out + b * a.o_sb + qi * a.o_sl + hq * a.o_sh + 8 * ch * Elem<T>::bytes;
+  if constexpr (Elem<T>::bytes == 4) {
+    reinterpret_cast<f32x4*>(op)[0] = o[0] * inv;
+    reinterpret_cast<f32x4*>(op)[1] = o[1] * inv;
+  } else {
+    *reinterpret_cast<u32x4*>(op) =
+        u32x4{Mfma<T>::pack(o[0][0] * inv, o[0][1] * inv), Mfma<T>::pack(o[0][2] * inv, o[0][3] * inv),
+              Mfma<T>::pack(o[1][0] * inv, o[1][1] * inv), Mfma<T>::pack(o[1][2] * inv, o[1][3] * inv)};
+  }
 }
 
 // ---------------------------------------------------------------------------
 // Host side: the plan and the launches.
 // ---------------------------------------------------------------------------
 struct PagedPlan {
-  int rw_own, rw_pre;        // row waves of a workgroup
-  int own_splits, pre_splits;  // pre_splits 0: no prefix
-  int64_t own_blocks, pre_blocks;
-  int64_t own_units, pre_units;  // 32-row partials (0: the kernel writes the result)
+  int rw_own, rw_pre;            // row waves of a workgroup; rw_pre 0: no prefix
+  int own_splits, pre_splits;    // 0: the line is cut
+  int64_t own_items, pre_items;
+  int64_t work;                  // tiles of both lines, at the largest lengths
+  int64_t own_n, grid;           // workgroups
+  int64_t own_slots, pre_slots;  // partials of 32 rw rows
+  int64_t own_recs, pre_recs;
+  bool merge;
 };
 
-int row_waves(int64_t rows) { return rows <= 32 ? 1 : rows <= 64 ? 2 : 4; }
+int row_waves(int64_t rows) { return rows <= 32 ? 1 : 4; }
 
-constexpr int kPagedMaxSplits = 64;
-
-int split_count(int64_t items, int64_t tiles, int cus) {
-  const int64_t want = (cus + items - 1) / std::max<int64_t>(items, 1);
-  return int(std::max<int64_t>(1, std::min({want, tiles / 8, int64_t(kPagedMaxSplits)})));
+// LDS of a workgroup (Shape::lds), by what the plan knows.
+int lds_bytes(int64_t D, int64_t es, int rw) {
+  const int64_t rb = D * es, kw = rw == 1 ? (rb >= 512 ? 4 : 8) : kWaves / rw;
+  const int64_t stages = kw * (rw == 1 ? 1 : 2) * 2 * (rw == 1 || rb >= 512 ? 32 : 64) * rb;
+  const int64_t areas = rw * kw * (std::min<int64_t>(D, 128) / 8 * 1040 + 256);
+  return int(std::max(stages, areas) + kWaves * 2 * 16);
 }
 
-PagedPlan plan_paged(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hkv, int64_t own_rows,
-                     int64_t pre_rows, bool prefix, int cus) {
+// Key ranges per item of a split line: `tiles` per item, rounds of `slots`
+// workgroups, each with the cost of some tiles for its start and end. The
+// smallest of the counts that are within 2% of the best.
+int range_count(int64_t items, int64_t tiles, int64_t slots) {
+  auto cost = [&](int64_t s) {
+    const int64_t rounds = (items * s + slots - 1) / slots;
+    return double(rounds) * (double((tiles + s - 1) / s) + 8) + (s > 1 ? 8 : 0);
+  };
+  double best = cost(1);
+  const int64_t most = std::min<int64_t>(16, std::max<int64_t>(1, tiles / 8));
+  for (int64_t s = 2; s <= most; ++s) best = std::min(best, cost(s));
+  int s = 1;
+  while (cost(s) > 1.02 * best) ++s;
+  return s;
+}
+
+PagedPlan plan_paged(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hkv, int64_t D, int64_t es,
+                     int64_t own_rows, int64_t pre_rows, bool prefix, int cus) {
   PagedPlan p{};
   const int64_t R = Lq * (H / Hkv);
-  auto tiles = [](int64_t rows) { return (rows + kPN - 1) / kPN; };
   auto row_tiles = [](int64_t rows, int rw) { return (rows + 32 * rw - 1) / (32 * rw); };
+  auto tiles = [](int64_t rows) { return (rows + kPN - 1) / kPN; };
   p.rw_own = row_waves(R);
-  p.own_blocks = (R + 31) / 32;
-  p.own_splits = split_count(B * Hkv * row_tiles(R, p.rw_own), tiles(own_rows) + tiles(Lk), cus);
+  p.own_items = B * Hkv * row_tiles(R, p.rw_own);
+  const int64_t own_tiles = tiles(own_rows) + std::max<int64_t>(tiles(Lk), 1);
+  int lds = lds_bytes(D, es, p.rw_own);
+  p.work = p.own_items * own_tiles;
+  int64_t pre_tiles = 0;
   if (prefix) {
     p.rw_pre = row_waves(B * R);
-    p.pre_blocks = (B * R + 31) / 32;
-    p.pre_splits = split_count(Hkv * row_tiles(B * R, p.rw_pre), tiles(pre_rows), cus);
-    p.pre_units = Hkv * p.pre_blocks * p.pre_splits;
+    p.pre_items = Hkv * row_tiles(B * R, p.rw_pre);
+    pre_tiles = std::max<int64_t>(tiles(pre_rows), 1);
+    lds = std::max(lds, lds_bytes(D, es, p.rw_pre));
+    p.work += p.pre_items * pre_tiles;
   }
-  if (prefix || p.own_splits > 1) p.own_units = Hkv * B * p.own_blocks * p.own_splits;
+  // Workgroups that run at once.
+  const int64_t slots = int64_t(cus) * (2 * lds <= 160 * 1024 ? 2 : 1);
+  if (prefix && row_tiles(B * R, p.rw_pre) > 1) p.pre_splits = range_count(p.pre_items, pre_tiles, slots);
+  if (row_tiles(R, p.rw_own) > 1) p.own_splits = range_count(p.own_items, own_tiles, slots);
+  // A cut line: no more of them than its tiles at the largest lengths.
+  p.own_n = p.own_splits ? p.own_items * p.own_splits : std::min(slots, p.own_items * own_tiles);
+  const int64_t pre_n = p.pre_splits ? p.pre_items * p.pre_splits
+                                     : std::min(slots, p.pre_items * pre_tiles);
+  p.grid = p.own_n;
+  if (prefix) {
+    p.grid = p.own_splits || p.pre_splits ? p.own_n + pre_n
+                                          : std::max<int64_t>(2, std::min(slots, p.own_n + pre_n));
+    p.own_slots = p.own_splits ? p.own_n : p.own_items + p.grid;
+    p.pre_slots = p.pre_splits ? pre_n : p.pre_items + p.grid;
+    p.own_recs = p.own_items;
+    p.pre_recs = p.pre_items;
+    p.merge = true;
+  } else if (p.own_splits) {
+    p.merge = p.own_splits > 1;
+    p.own_slots = p.merge ? p.own_n : 0;
+    p.own_recs = p.merge ? p.own_items : 0;
+  } else {
+    p.merge = true;
+    p.own_slots = 2 * p.grid + 1;
+    p.own_recs = p.grid;
+  }
   return p;
 }
 
-int64_t unit_bytes(int64_t D) { return 32 * D * 4 + 32 * 8; }
-
-template <typename T, int D, int RW, bool PREFIX>
-hipError_t launch_part(const PagedArgs& a, int64_t items, hipStream_t st) {
-  using Sh = Shape<T, D, RW>;
-  const void* fn = reinterpret_cast<const void*>(&paged_attn_kernel<T, D, RW, PREFIX>);
-  const hipError_t e = opt_in_lds(fn, Sh::lds);
-  if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((paged_attn_kernel<T, D, RW, PREFIX>), dim3(unsigned(items)),
-                     dim3(64 * Sh::NW), Sh::lds, st, a);
-  return hipGetLastError();
+int64_t slot_bytes(int rw, int64_t D) { return 32 * int64_t(rw) * (D * 4 + 8); }
+int64_t plan_bytes(const PagedPlan& p, int64_t D) {
+  return p.own_slots * slot_bytes(p.rw_own, D) + p.pre_slots * slot_bytes(p.rw_pre, D) +
+         (p.own_recs + p.pre_recs) * int64_t(sizeof(Record));
 }
 
-template <typename T, int D, bool PREFIX>
-hipError_t launch_rows(const PagedArgs& a, int rw, int64_t items, hipStream_t st) {
-  switch (rw) {
-    case 1: return launch_part<T, D, 1, PREFIX>(a, items, st);
-    case 2: return launch_part<T, D, 2, PREFIX>(a, items, st);
-    default: return launch_part<T, D, 4, PREFIX>(a, items, st);
-  }
+template <typename T, int D, int RWP, int RWO>
+hipError_t launch_form(const PagedArgs& a, const PagedPlan& p, hipStream_t st) {
+  constexpr int lds_own = Shape<T, D, RWO>::lds, lds_pre = RWP ? Shape<T, D, RWP ? RWP : 1>::lds : 0;
+  constexpr int lds = lds_own > lds_pre ? lds_own : lds_pre;
+  const void* fn = reinterpret_cast<const void*>(&paged_attn_kernel<T, D, RWP, RWO>);
+  hipError_t e = opt_in_lds(fn, lds);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((paged_attn_kernel<T, D, RWP, RWO>), dim3(unsigned(p.grid)), dim3(kThreads), lds,
+                     st, a);
+  e = hipGetLastError();
+  if (e != hipSuccess || !p.merge) return e;
+  hipLaunchKernelGGL((paged_merge_kernel<T, D, RWP, RWO>), dim3(unsigned(p.own_recs), RWO, D / 64),
+                     dim3(256), 0, st, a);
+  return hipGetLastError();
 }
 
 template <typename T, int D>
 hipError_t launch_paged(const PagedArgs& a, const PagedPlan& p, hipStream_t st) {
-  auto row_tiles = [](int64_t rows, int rw) { return (rows + 32 * rw - 1) / (32 * rw); };
-  if (p.pre_splits) {
-    const hipError_t e = launch_rows<T, D, true>(
-        a, p.rw_pre, int64_t(a.Hkv) * row_tiles(int64_t(a.B) * a.R, p.rw_pre) * p.pre_splits, st);
-    if (e != hipSuccess) return e;
-  }
-  const hipError_t e = launch_rows<T, D, false>(
-      a, p.rw_own, int64_t(a.B) * a.Hkv * row_tiles(a.R, p.rw_own) * p.own_splits, st);
-  if (e != hipSuccess || p.own_units == 0) return e;
-  hipLaunchKernelGGL((paged_merge_kernel<T, D>), dim3(unsigned(a.Hkv * a.B * p.own_blocks), D / 32),
-                     dim3(256), 0, st, a);
-  return hipGetLastError();
+  if (p.rw_pre == 0)
+    return p.rw_own == 1 ? launch_form<T, D, 0, 1>(a, p, st) : launch_form<T, D, 0, 4>(a, p, st);
+  if (p.rw_pre == 1) return launch_form<T, D, 1, 1>(a, p, st);
+  return p.rw_own == 1 ? launch_form<T, D, 4, 1>(a, p, st) : launch_form<T, D, 4, 4>(a, p, st);
 }
 
 struct PagedCall {
@@ -619,18 +1153,20 @@ int paged_entry(const char* what, const PagedCall& c, bool prefix, void* stream)
     DX_CHECK_ARG(s >= 0 && s * es < (int64_t(1) << 26), "%s: row stride %lld out of range", what,
                  (long long)s);
 
-  const PagedPlan p = plan_paged(c.B, c.Lq, c.Lk, c.H, c.Hkv, c.width * c.page_rows,
+  const PagedPlan p = plan_paged(c.B, c.Lq, c.Lk, c.H, c.Hkv, c.D, es, c.width * c.page_rows,
                                  c.prefix_width * c.page_rows, prefix, device_cus());
-  const int64_t need = (p.own_units + p.pre_units) * unit_bytes(c.D);
+  const int64_t need = plan_bytes(p, c.D);
   if (need > c.ws_bytes || (need > 0 && !c.ws)) {
-    set_error("%s: workspace of %lld bytes, %lld needed", what, (long long)c.ws_bytes,
+    set_error("%s: workspace of %lld bytes, %lld needed", what, (long long)(c.ws ? c.ws_bytes : 0),
               (long long)need);
     return DX_EWORKSPACE;
   }
   DX_CHECK_ARG(al(c.ws), "%s: workspace must be 16-byte aligned", what);
   const int64_t group = c.H / c.Hkv, R = c.Lq * group;
-  DX_CHECK_ARG(grid_fits(c.B * c.Hkv * p.own_blocks * p.own_splits, 512) &&
-                   grid_fits(c.Hkv * p.pre_blocks * std::max(p.pre_splits, 1), 512),
+  // Item numbers and slots are 32-bit; the merge takes a workgroup per item.
+  DX_CHECK_ARG(p.work / p.grid < (int64_t(1) << 30), "%s: too many keys for one launch", what);
+  DX_CHECK_ARG(grid_fits(p.own_recs, 256) && grid_fits(p.grid, kThreads) && p.own_items < (int64_t(1) << 30) &&
+                   p.pre_items < (int64_t(1) << 30),
                "%s: the call exceeds one launch", what);
   PagedArgs a{};
   a.q = static_cast<const char*>(c.q); a.q_sb = c.q_sb * es; a.q_sl = c.q_sl * es; a.q_sh = c.q_sh * es;
@@ -652,14 +1188,21 @@ int paged_entry(const char* what, const PagedCall& c, bool prefix, void* stream)
   a.Lq = int(c.Lq); a.Lk = int(c.Lk); a.causal = c.causal != 0;
   a.R = int(R);
   a.scale_log2 = c.scale * 1.4426950408889634f;
-  a.own_splits = p.own_splits; a.own_blocks = int(p.own_blocks);
-  a.pre_splits = p.pre_splits; a.pre_blocks = int(p.pre_blocks);
-  if (p.own_units) {
-    a.own_o = static_cast<float*>(c.ws);
-    a.pre_o = a.own_o + p.own_units * 32 * c.D;
-    a.own_ml = a.pre_o + p.pre_units * 32 * c.D;
-    a.pre_ml = a.own_ml + p.own_units * 64;
-  }
+  a.own.splits = p.own_splits;
+  a.pre.splits = p.pre_splits;
+  a.own_n = int(p.own_n);
+  char* ws = static_cast<char*>(c.ws);
+  auto take = [&](int64_t bytes) {
+    char* const at = ws;
+    ws += bytes;
+    return at;
+  };
+  a.own.o = reinterpret_cast<float*>(take(p.own_slots * 32 * p.rw_own * c.D * 4));
+  a.pre.o = reinterpret_cast<float*>(take(p.pre_slots * 32 * p.rw_pre * c.D * 4));
+  a.own.ml = reinterpret_cast<float*>(take(p.own_slots * 32 * p.rw_own * 8));
+  a.pre.ml = reinterpret_cast<float*>(take(p.pre_slots * 32 * p.rw_pre * 8));
+  a.own.rec = reinterpret_cast<Record*>(take(p.own_recs * int64_t(sizeof(Record))));
+  a.pre.rec = reinterpret_cast<Record*>(take(p.pre_recs * int64_t(sizeof(Record))));
   const hipStream_t st = static_cast<hipStream_t>(stream);
   hipError_t e;
   if (c.dtype == DX_F32)
@@ -692,9 +1235,9 @@ extern "C" int64_t dx_paged_attention_workspace_bytes(int dtype, int64_t B, int6
                               prefix_width);
   if (bad) return -bad;
   if (B == 0 || Lq == 0) return 0;
-  const PagedPlan p = plan_paged(B, Lq, Lk, H, Hkv, width * page_rows, prefix_width * page_rows,
-                                 has_prefix != 0, device_cus());
-  return (p.own_units + p.pre_units) * unit_bytes(D);
+  const PagedPlan p = plan_paged(B, Lq, Lk, H, Hkv, D, dtype == DX_F32 ? 4 : 2, width * page_rows,
+                                 prefix_width * page_rows, has_prefix != 0, device_cus());
+  return plan_bytes(p, D);
 }
 
 extern "C" int dx_paged_attention(
