@@ -110,18 +110,22 @@ template <int RB, bool F32> __device__ __forceinline__ constexpr int vswz(int r)
   return 4 * (RB == 128 ? ((r >> 1) ^ (r >> 2)) & 1 : (r & 3) ^ ((r >> 2) & 1));
 }
 
-constexpr int kThreads = 512, kWaves = 8;
+constexpr int kThreads = 256, kWaves = 4;
 
 // A workgroup's shape for RW row waves.
 template <typename T, int D, int RW> struct Shape {
   static constexpr int RB = D * Elem<T>::bytes;      // bytes of a row
-  // Keys that a stream takes at a time. One row wave: 32, streams of one wave,
-  // whose K and V are single (the next K goes out when S is done, the next V
-  // when PV is done), as many streams as fit. Else two streams with two stages
-  // of 64 keys (each of four waves then fetches 16 rows, which one page holds),
-  // or of 32 where registers and LDS hold no more.
+  // Four waves and half of a CU's LDS, so that two workgroups share a CU and one
+  // starts, ends or waits while the other computes. One row wave: streams of one
+  // wave, as many as fit, 32 keys at a time, whose K and V are single (the next
+  // K goes out when S is done, the next V when PV is done). Four: one stream,
+  // two stages of 64 keys (each wave then fetches 16 rows, which one page
+  // holds), or of 32 where registers and LDS hold no more.
+  // Head dim 256 (queries and sums of a wave alone take 192 registers) has a CU
+  // to itself: registers for one wave per SIMD, 32 of them spilled otherwise.
+  static constexpr int per_cu = D == 256 ? 1 : 2;
   static constexpr int TK = RW == 1 || RB >= 512 ? 32 : 64;
-  static constexpr int KW = RW == 1 ? (RB >= 512 ? 4 : 8) : kWaves / RW;
+  static constexpr int KW = RW == 1 ? (RB * per_cu >= 1024 ? 2 : 4) : kWaves / RW;
   static constexpr int tile = TK * RB;               // bytes of a K or V tile
   static constexpr int stages = RW == 1 ? 1 : 2;
   static constexpr int stream = stages * 2 * tile;
@@ -135,7 +139,7 @@ template <typename T, int D, int RW> struct Shape {
   // Behind them: which 16-row groups of each stage's tile have no page.
   static constexpr int flags = body;
   static constexpr int lds = body + kWaves * 2 * 16;
-  static_assert(lds <= 160 * 1024, "LDS of a CU");
+  static_assert(lds * per_cu <= 160 * 1024, "the LDS of a CU");
 };
 
 __device__ __forceinline__ int tiles_of(int rows) { return (rows + kPN - 1) / kPN; }
@@ -164,17 +168,23 @@ __device__ __forceinline__ int new_tiles(Args& a, int rt) {
   return max(tiles_of(hi), 1);
 }
 
-__device__ __forceinline__ uint64_t scan64(uint64_t x, int lane) {  // inclusive, over a wave
+__device__ __forceinline__ uint32_t scan(uint32_t x, int lane) {  // inclusive, over a wave
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
-    const uint64_t y = __shfl_up(x, d);
+    const uint32_t y = __shfl_up(x, d);
     if (lane >= d) x += y;
   }
   return x;
 }
+__device__ __forceinline__ uint32_t lane_of(uint32_t x, int lane) {
+  return uint32_t(__builtin_amdgcn_readlane(int(x), lane));
+}
 __device__ __forceinline__ uint64_t uniform(uint64_t x) {
   return uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(int(x)))) |
          uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(int(x >> 32)))) << 32;
+}
+__device__ __forceinline__ uint32_t uniform(uint32_t x) {
+  return uint32_t(__builtin_amdgcn_readfirstlane(int(x)));
 }
 __device__ __forceinline__ int own_rows(Args& a, int b) {
   return a.width == 0 ? 0 : min(max(a.lens[b], 0), a.width * a.page_rows);
@@ -183,88 +193,100 @@ __device__ __forceinline__ int prefix_rows(Args& a) {
   return a.plen ? min(max(*a.plen, 0), a.pwidth * a.page_rows) : 0;
 }
 
-// n / d for uniform n; 64-bit division is long.
-__device__ __forceinline__ uint64_t udiv(uint64_t n, uint64_t d) {
-  return (n | d) >> 32 ? n / d : uint64_t(uint32_t(n) / uint32_t(d));
-}
+// Work on a line is counted in tiles; an item adds `kItemCost` to its tiles, for
+// its queries and its result (what a piece of so many tiles costs). A cut that
+// falls among those is taken as one behind the item.
+template <typename T, int D, int RW>
+constexpr uint32_t kItemCost = Shape<T, D, RW>::KW * Shape<T, D, RW>::TK / kPN * 2;
+
+// A line of `total` cut into n pieces, the first `longer` of them q + 1 long.
+struct Cut {
+  uint32_t q, longer;
+  __device__ __forceinline__ Cut(uint32_t total, uint32_t n) : q(total / n), longer(total - q * n) {}
+  __device__ __forceinline__ uint32_t start(uint32_t w) const { return w * q + min(w, longer); }
+  // The piece that holds position x.
+  __device__ __forceinline__ uint32_t piece(uint32_t x) const {
+    const uint32_t y = longer * (q + 1);
+    return x < y ? x / (q + 1) : longer + (x - y) / q;
+  }
+};
 
 // The line of the own keys: items (sequence, K/V head, row tile), in this order.
+// The host holds its length below 2^31.
 template <int RW>
 struct OwnLine {
-  int n_rt;
-  uint64_t fresh;  // new-key tiles of a (sequence, head): of all its row tiles
-  uint64_t total;
-  __device__ __forceinline__ void init(Args& a, int lane) {
-    n_rt = (a.R + 32 * RW - 1) / (32 * RW);
-    fresh = 0;
+  uint32_t n_rt;
+  uint32_t fresh;  // new-key tiles and costs of a (sequence, head): of all its row tiles
+  uint32_t total;
+  __device__ __forceinline__ void init(Args& a, int lane, uint32_t cost) {
+    n_rt = uniform(uint32_t(a.R + 32 * RW - 1) / (32 * RW));
+    uint32_t tiles = 0;
     if (a.causal || a.n_blocks) {
-      for (int r0 = 0; r0 < n_rt; r0 += 64)
-        fresh += uniform(__shfl(scan64(r0 + lane < n_rt ? new_tiles<RW>(a, r0 + lane) : 0, lane), 63));
+      for (uint32_t r0 = 0; r0 < n_rt; r0 += 64)
+        tiles += lane_of(scan(r0 + lane < n_rt ? new_tiles<RW>(a, int(r0) + lane) : 0, lane), 63);
     } else {
-      fresh = uint64_t(n_rt) * max(tiles_of(a.Lk), 1);
+      tiles = n_rt * uint32_t(max(tiles_of(a.Lk), 1));
     }
-    uint64_t cached = 0;
+    fresh = uniform(tiles + n_rt * cost);
+    uint32_t cached = 0;
     if (a.B == 1) {
-      cached = tiles_of(own_rows(a, 0));
+      cached = uint32_t(tiles_of(own_rows(a, 0)));
     } else {
       for (int b0 = 0; b0 < a.B; b0 += 64)
-        cached += uniform(__shfl(scan64(b0 + lane < a.B ? tiles_of(own_rows(a, b0 + lane)) : 0, lane), 63));
+        cached += lane_of(scan(b0 + lane < a.B ? tiles_of(own_rows(a, b0 + lane)) : 0, lane), 63);
     }
-    total = uint64_t(a.Hkv) * (uint64_t(n_rt) * cached + uint64_t(a.B) * fresh);
+    total = uniform(uint32_t(a.Hkv) * (n_rt * cached + uint32_t(a.B) * fresh));
   }
-  // The item that holds tile `at` of the line, and the tile's number in it.
-  __device__ __forceinline__ void locate(Args& a, int lane, uint64_t at, int& b, int& hk,
+  // The item that holds position `at` of the line, and the place in it.
+  __device__ __forceinline__ void locate(Args& a, int lane, uint32_t cost, uint32_t at, int& b, int& hk,
                                          int& rt, int& t) const {
     b = 0;
-    uint64_t before = 0;  // tiles of the sequences before b, per head
-    const uint64_t want = udiv(at, a.Hkv);
+    uint32_t before = 0;  // what the sequences before b have, per head
     if (a.B > 1) {
-      uint64_t cached = 0;
+      const uint32_t want = at / uint32_t(a.Hkv);
+      uint32_t cached = 0;
       for (int b0 = 0; b0 < a.B; b0 += 64) {
-        const uint64_t own = b0 + lane < a.B ? tiles_of(own_rows(a, b0 + lane)) : 0;
-        const uint64_t upto = cached + scan64(own, lane);
-        // Tiles up to and with this lane's sequence, over all heads, against at.
-        const uint64_t end = uint64_t(n_rt) * upto + uint64_t(b0 + lane + 1) * fresh;
+        const uint32_t own = b0 + lane < a.B ? tiles_of(own_rows(a, b0 + lane)) : 0;
+        const uint32_t upto = cached + scan(own, lane);
+        // Up to and with this lane's sequence.
+        const uint32_t end = n_rt * upto + uint32_t(b0 + lane + 1) * fresh;
         const uint64_t hit = __ballot(b0 + lane < a.B && end > want);
         if (hit) {
           const int j = __builtin_ctzll(hit);
           b = b0 + j;
-          before = uniform(__shfl(uint64_t(n_rt) * (upto - own) + uint64_t(b0 + lane) * fresh, j));
+          before = lane_of(end, j) - n_rt * lane_of(own, j) - fresh;
           break;
         }
-        cached += uniform(__shfl(scan64(own, lane), 63));
+        cached = lane_of(upto, 63);
       }
     }
     b = __builtin_amdgcn_readfirstlane(b);
-    const uint64_t n_ct = uint64_t(__builtin_amdgcn_readfirstlane(tiles_of(own_rows(a, b))));
-    const uint64_t in_seq = at - before * uint64_t(a.Hkv);
-    const uint64_t per_head = uint64_t(n_rt) * n_ct + fresh;
-    hk = int(udiv(in_seq, per_head));
-    uint64_t r = in_seq - uint64_t(hk) * per_head;
+    const uint32_t n_ct = uniform(uint32_t(tiles_of(own_rows(a, b))));
+    const uint32_t in_seq = at - before * uint32_t(a.Hkv);
+    const uint32_t per_head = n_rt * n_ct + fresh;
+    hk = int(in_seq / per_head);
+    uint32_t r = in_seq - uint32_t(hk) * per_head;
     rt = 0;
     if (a.causal || a.n_blocks) {
-      uint64_t base = 0;
-      for (int r0 = 0; r0 < n_rt; r0 += 64) {
-        const uint64_t w = r0 + lane < n_rt ? n_ct + new_tiles<RW>(a, r0 + lane) : 0;
-        const uint64_t upto = base + scan64(w, lane);
+      uint32_t base = 0;
+      for (uint32_t r0 = 0; r0 < n_rt; r0 += 64) {
+        const uint32_t w = r0 + lane < n_rt ? n_ct + new_tiles<RW>(a, int(r0) + lane) + cost : 0;
+        const uint32_t upto = base + scan(w, lane);
         const uint64_t hit = __ballot(r0 + lane < n_rt && upto > r);
         if (hit) {
           const int j = __builtin_ctzll(hit);
-          rt = r0 + j;
-          r -= uniform(__shfl(upto - w, j));
+          rt = int(r0) + j;
+          r -= lane_of(upto, j) - lane_of(w, j);
           break;
         }
-        base = uniform(__shfl(upto, 63));
+        base = lane_of(upto, 63);
       }
-      t = int(r);
     } else {
-      const uint64_t w = n_ct + max(tiles_of(a.Lk), 1);
-      rt = int(udiv(r, w));
-      t = int(r - uint64_t(rt) * w);
+      const uint32_t w = n_ct + uint32_t(max(tiles_of(a.Lk), 1)) + cost;
+      rt = int(r / w);
+      r -= uint32_t(rt) * w;
     }
-    hk = __builtin_amdgcn_readfirstlane(hk);
-    rt = __builtin_amdgcn_readfirstlane(rt);
-    t = __builtin_amdgcn_readfirstlane(t);
+    t = int(r);
   }
 };
 
@@ -444,7 +466,7 @@ __device__ __forceinline__ void send_rows(uint64_t from, int rows, int step, uin
 // One workgroup's share of a line: workgroup w of n.
 template <typename T, int D, int RW, bool PREFIX, bool SHARED>
 __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uint32_t n,
-                                         uint64_t total, int line_rt, uint64_t line_fresh) {
+                                         uint32_t total, uint32_t line_fresh) {
   using Sh = Shape<T, D, RW>;
   constexpr int RB = Sh::RB, KW = Sh::KW, TK = Sh::TK, CR = RB / 16, RPP = 64 / CR;
   using Ti = Tile<T, D, TK / 32>;
@@ -455,10 +477,12 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
   const int stream = wid / RW, wave = wid % RW, lane = int(threadIdx.x) & 63;
   const int g = lane >> 5, nl = lane & 31;
 
-  // Cut: tiles [w T / n, (w + 1) T / n) of the line, from tile t0 of an item on.
-  // Split: range t0 (for now) of an item.
-  uint64_t at = 0;
-  int todo = 1;  // tiles left to do (the host limits a workgroup's share to 31 bits)
+  // Cut: piece w of the line, from tile t0 of an item on. Split: range t0 (for
+  // now) of an item.
+  const Cut cut(total, n);
+  constexpr uint32_t kCost = kItemCost<T, D, RW>;
+  uint32_t at = 0;
+  int todo = 1;  // what is left of the piece
   int b = 0, hk = 0, rt = 0, t0 = 0;
   int n_rt, splits;
   {
@@ -467,18 +491,18 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
     n_rt = __builtin_amdgcn_readfirstlane((nrows + 32 * RW - 1) / (32 * RW));
     splits = __builtin_amdgcn_readfirstlane(PREFIX ? a.pre.splits : a.own.splits);
     if (splits == 0) {
-      at = uniform(udiv(uint64_t(w) * total, n));
-      todo = __builtin_amdgcn_readfirstlane(int(udiv(uint64_t(w + 1) * total, n) - at));
+      at = uniform(cut.start(w));
+      todo = __builtin_amdgcn_readfirstlane(int(cut.start(w + 1) - at));
       if (todo > 0) {
         if (PREFIX) {
-          const uint64_t pre_w = uint64_t(max(tiles_of(prefix_rows(a)), 1));
-          const uint64_t item = udiv(at, pre_w);
-          t0 = int(at - item * pre_w);
-          hk = int(uint32_t(item) / uint32_t(n_rt));
-          rt = int(uint32_t(item) - uint32_t(hk) * uint32_t(n_rt));
+          const uint32_t weight = uint32_t(max(tiles_of(prefix_rows(a)), 1)) + kCost;
+          const uint32_t item = at / weight;
+          t0 = int(at - item * weight);
+          hk = int(item / uint32_t(n_rt));
+          rt = int(item - uint32_t(hk) * uint32_t(n_rt));
         } else {
-          const OwnLine<RW> line{line_rt, line_fresh, total};
-          line.locate(a, lane, at, b, hk, rt, t0);
+          const OwnLine<RW> line{uint32_t(n_rt), line_fresh, total};
+          line.locate(a, lane, kCost, at, b, hk, rt, t0);
         }
       }
     } else {
@@ -516,7 +540,7 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
     int my_end = 0, full_end, t1, weight, nt, iters, item;
     uint32_t slot;
     const bool first = t0 == 0;  // this share holds the item's first tile: it leaves the record
-    bool active;
+    bool active, behind = false;
     {
       Args& a = *reread(args);
       const int nrows = PREFIX ? a.B * a.R : a.R;
@@ -533,7 +557,8 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
       if (!PREFIX) weight = keys.n_ct + max(tiles_of(keys.fresh), 1);
       item = PREFIX ? hk * n_rt + rt : (b * a.Hkv + hk) * n_rt + rt;
       if (splits == 0) {
-        t1 = __builtin_amdgcn_readfirstlane(min(weight - t0, todo) + t0);
+        behind = t0 >= weight;  // the piece begins behind the item's tiles
+        t1 = __builtin_amdgcn_readfirstlane(max(min(weight - t0, todo), 0) + t0);
         // Without a prefix a workgroup breaks two items at most; with one, every
         // item has parts, and (workgroup, item) grow together.
         slot = SHARED ? w + uint32_t(item) : 2 * w + uint32_t(first);
@@ -709,6 +734,7 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
       }
     }
 
+    if (!behind) {
     // The streams' results meet in LDS. Thread j of a row takes 8 of its
     // values: it reads them from every stream and weighs them by its maximum.
     const bool whole = first && t1 == weight && splits <= 1;
@@ -793,19 +819,20 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
       left = Record{item, int(slot), splits, 0};
       if (splits == 0) {
         // Up to the workgroup that holds the item's last tile.
-        const uint64_t last = udiv((at + uint64_t(weight)) * n - 1, total);
-        left.parts = int(last) - int(w) + 1;
+        left.parts = int(cut.piece(at + uint32_t(weight) - 1)) - int(w) + 1;
       }
       if ((SHARED || splits) && threadIdx.x == 0) (PREFIX ? a.pre.rec : a.own.rec)[item] = left;
     }
     if (splits) return;
     __syncthreads();  // the results are read: tiles may land again
-    at = uniform(at + uint64_t(t1 - t0));
-    todo = __builtin_amdgcn_readfirstlane(todo - (t1 - t0));
+    }
+    const int used = weight + int(kCost) - t0;  // to the next item
+    at += uint32_t(used);
+    todo = __builtin_amdgcn_readfirstlane(todo - used);
     t0 = 0;
     if (++rt == n_rt) {
       rt = 0;
-      if (++hk == a.Hkv) {
+      if (++hk == reread(args)->Hkv) {
         hk = 0;
         ++b;
       }
@@ -814,145 +841,179 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
   if (!SHARED && splits == 0 && threadIdx.x == 0) args->own.rec[w] = left;
 }
 
-// Tiles that a workgroup should have before more of them are put to work.
-template <typename T, int D, int RW> constexpr int kMinTiles = Shape<T, D, RW>::KW * Shape<T, D, RW>::TK / kPN * 2;
-
 template <typename T, int D, int RWP, int RWO>
-__global__ __launch_bounds__(kThreads, 1) void paged_attn_kernel(PagedArgs) {
+__global__ __launch_bounds__(kThreads, (Shape<T, D, RWO>::per_cu)) void paged_attn_kernel(PagedArgs) {
   Args* const args = (Args*)(uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
+  // Touch every line of the arguments up front: one wait instead of one for
+  // each line at its first use.
+  {
+    const uint32_t* const x = (const uint32_t*)(uint64_t)args;
+    static_assert(sizeof(PagedArgs) > 5 * 64 && sizeof(PagedArgs) <= 7 * 64, "lines of the arguments");
+    typedef __attribute__((address_space(4))) const uint32_t const_u32;
+    const_u32* const l = (const_u32*)(uint64_t)x;
+    const uint32_t l0 = l[0], l1 = l[16], l2 = l[32], l3 = l[48], l4 = l[64], l5 = l[80],
+                   l6 = l[sizeof(PagedArgs) / 4 - 1];
+    asm volatile("" ::"s"(l0), "s"(l1), "s"(l2), "s"(l3), "s"(l4), "s"(l5), "s"(l6));
+  }
   Args& a = *reread(args);
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = int(threadIdx.x) & 63;
-  OwnLine<RWO> own{};
+  constexpr uint32_t kCostO = kItemCost<T, D, RWO>, kCostP = kItemCost<T, D, RWP ? RWP : 1>;
   const uint32_t grid = gridDim.x;
-  if (a.own.splits == 0) own.init(a, lane);
-  auto wanted = [&](uint64_t tiles, int least, uint32_t most) __attribute__((always_inline)) {
-    const uint64_t x = (tiles + least - 1) / least;
-    return x < most ? uint32_t(x) : most;
+  // Workgroups of a cut line: one for what an item costs besides its tiles.
+  auto wanted = [&](uint32_t total, uint32_t least, uint32_t most) __attribute__((always_inline)) {
+    return min((total + least - 1) / least, most);
   };
-  // Workgroups of each line, the prefix's first.
-  uint32_t n_own, n_pre = 0;
-  uint64_t pre_total = 0;
-  if constexpr (RWP > 0) {
-    const uint32_t pre_items = uint32_t(a.Hkv) * uint32_t((a.B * a.R + 32 * RWP - 1) / (32 * RWP));
-    pre_total = uint64_t(pre_items) * max(tiles_of(prefix_rows(a)), 1);
-    if (a.pre.splits) n_pre = pre_items * uint32_t(a.pre.splits);
-    else n_pre = wanted(pre_total, kMinTiles<T, D, RWP>, grid);
-  }
-  if (a.own.splits) {
-    n_own = uint32_t(a.B * a.Hkv) * uint32_t((a.R + 32 * RWO - 1) / (32 * RWO)) * uint32_t(a.own.splits);
-  } else {
-    n_own = wanted(own.total, kMinTiles<T, D, RWO>, uint32_t(a.own_n));
-    if (RWP > 0 && a.pre.splits == 0 && n_pre + n_own > grid) {
-      // Both are cut: in proportion to their tiles.
-      const float part = float(pre_total) / float(pre_total + own.total);
-      n_pre = uint32_t(part * float(grid) + 0.5f);
-      n_pre = min(max(n_pre, 1u), grid - 1);
-      n_own = grid - n_pre;
-    }
-  }
-  n_pre = uint32_t(__builtin_amdgcn_readfirstlane(int(n_pre)));
-  n_own = uint32_t(__builtin_amdgcn_readfirstlane(int(n_own)));
-  uint32_t w = blockIdx.x;
-  if (w >= n_pre + n_own) {
-    if (RWP == 0 && threadIdx.x == 0) a.own.rec[w] = Record{0, 0, 0, 0};
-    return;
-  }
   // Workgroup i runs on XCD i % 8: consecutive pieces of a cut line, which may
   // share keys, go to one XCD's L2.
   auto in_runs = [](uint32_t i, uint32_t n) __attribute__((always_inline)) {
     const uint32_t n8 = n & ~7u;
     return i < n8 ? i % 8 * (n8 / 8) + i / 8 : i;
   };
+  // The prefix's workgroups come first.
+  uint32_t w = blockIdx.x, n_pre = 0, pre_total = 0;
   if constexpr (RWP > 0) {
-    if (w < n_pre) {
-      if (a.pre.splits == 0) w = in_runs(w, n_pre);
-      run_line<T, D, RWP, true, true>(args, smem, w, n_pre, pre_total, 0, 0);
-      return;
+    const uint32_t pre_items = uint32_t(a.Hkv) * (uint32_t(a.B * a.R + 32 * RWP - 1) / (32 * RWP));
+    pre_total = uniform(pre_items * (uint32_t(max(tiles_of(prefix_rows(a)), 1)) + kCostP));
+    if (a.pre.splits) {
+      n_pre = pre_items * uint32_t(a.pre.splits);
+      if (w < n_pre) {
+        run_line<T, D, RWP, true, true>(args, smem, w, n_pre, pre_total, 0);
+        return;
+      }
     }
   }
+  OwnLine<RWO> own{};
+  uint32_t n_own;
+  if (a.own.splits) {
+    n_own = uint32_t(a.B * a.Hkv) * (uint32_t(a.R + 32 * RWO - 1) / (32 * RWO)) * uint32_t(a.own.splits);
+  } else {
+    own.init(a, lane, kCostO);
+    n_own = wanted(own.total, kCostO, uint32_t(a.own_n));
+  }
+  if constexpr (RWP > 0) {
+    if (a.pre.splits == 0) {
+      n_pre = wanted(pre_total, kCostP, grid);
+      if (a.own.splits == 0 && n_pre + n_own > grid) {
+        // Both are cut: in proportion to their length.
+        const float part = float(pre_total) / (float(pre_total) + float(own.total));
+        n_pre = uint32_t(part * float(grid) + 0.5f);
+        n_pre = min(max(n_pre, 1u), grid - 1);
+        n_own = grid - n_pre;
+      }
+      n_pre = uniform(n_pre);
+      if (w < n_pre) {
+        run_line<T, D, RWP, true, true>(args, smem, in_runs(w, n_pre), n_pre, pre_total, 0);
+        return;
+      }
+    }
+  }
+  n_own = uniform(n_own);
   w -= n_pre;
+  if (w >= n_own) {
+    if (RWP == 0 && threadIdx.x == 0) a.own.rec[w] = Record{0, 0, 0, 0};
+    return;
+  }
   if (a.own.splits == 0) w = in_runs(w, n_own);
-  run_line<T, D, RWO, false, (RWP > 0)>(args, smem, w, n_own, own.total, own.n_rt, own.fresh);
+  run_line<T, D, RWO, false, (RWP > 0)>(args, smem, w, n_own, own.total, own.fresh);
 }
 
-// Join the parts of 32 rows of an item, D / gridDim.z of their values: a thread
-// holds 8 values of a row. blockIdx.x is a record. Prefix items are over all
-// sequences' rows, so the rows here may be those of two. A part that saw nothing
-// has l = 0.
+// Join the parts of 8 rows of an item, 64 of their values (blockIdx.z): a lane
+// holds 8 values of a row, and the four waves take every fourth part each, so
+// that a long list of parts is no long chain of loads; their sums meet in LDS.
+// blockIdx.x is a record. Prefix items are over all sequences' rows, so the rows
+// here may be those of two. A part that saw nothing has l = 0.
 template <typename T, int D, int RWP, int RWO>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
+  __shared__ f32x4 sums[3][64][2];
+  __shared__ f32x2 stats[3][64];
   const Record rec = a.own.rec[blockIdx.x];
   if (rec.parts == 0) return;
-  const int n_rt = (a.R + 32 * RWO - 1) / (32 * RWO);
+  const uint32_t n_rt = uint32_t(a.R + 32 * RWO - 1) / (32 * RWO);
   constexpr int CD = 8;  // 8-value chunks of a row here: 64 values
-  const int r = int(threadIdx.x) / CD, ch = int(blockIdx.z) * CD + int(threadIdx.x) % CD;
-  const int in_item = int(blockIdx.y) * 32 + r;
-  const int rt = rec.item % n_rt, bh = rec.item / n_rt;
-  const int b = bh / a.Hkv, hk = bh % a.Hkv;
-  const int row = rt * 32 * RWO + in_item;
-  if (row >= a.R) return;
-  // Rows of the parts in each line: part p of the own keys, and of the prefix.
-  auto own_row = [&](int p) __attribute__((always_inline)) {
-    // Of a cut line without a prefix, a broken item's first part is its
-    // workgroup's odd slot, the others are the next workgroups' even ones.
-    const int64_t slot = RWP == 0 && a.own.splits == 0
-                             ? int64_t(rec.slot) + (p ? 2 * p - 1 : 0) : int64_t(rec.slot) + p;
-    return slot * (32 * RWO) + in_item;
-  };
-  int pre_parts = 0;
-  int64_t pre_row = 0;
-  if constexpr (RWP > 0) {
-    const int pr = b * a.R + row;
-    const int pre_rt = (a.B * a.R + 32 * RWP - 1) / (32 * RWP);
-    const Record p = a.pre.rec[hk * pre_rt + pr / (32 * RWP)];
-    pre_parts = p.parts;
-    pre_row = int64_t(p.slot) * (32 * RWP) + pr % (32 * RWP);
-  }
+  const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6), lane = int(threadIdx.x) & 63;
+  const int ch = int(blockIdx.z) * CD + lane % CD;
+  const int in_item = int(blockIdx.y) * 8 + lane / CD;
+  const uint32_t bh = uint32_t(rec.item) / n_rt, rt = uint32_t(rec.item) - bh * n_rt;
+  const int b = int(bh / uint32_t(a.Hkv)), hk = int(bh) - b * a.Hkv;
+  const int row = int(rt) * 32 * RWO + in_item;
+  if (int(rt) * 32 * RWO + int(blockIdx.y) * 8 >= a.R) return;  // no row of this workgroup exists
+  const bool valid = row < a.R;
   float m = -INFINITY, l = 0.f;
   f32x4 o[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-  // Four parts at a time: their loads do not wait for one another.
+  auto add = [&](const f32x2 ml, const f32x4 (&v)[2], float ref) __attribute__((always_inline)) {
+    const float wt = fast_exp2(ml[0] - ref);
+    l = __builtin_fmaf(ml[1], wt, l);
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int y = 0; y < 4; ++y) o[x][y] = __builtin_fmaf(v[x][y], wt, o[x][y]);
+  };
+  auto rescale = [&](float mm) __attribute__((always_inline)) {
+    const float ref = mm == -INFINITY ? 0.f : mm, keep = fast_exp2(m - ref);
+    l *= keep;
+    o[0] *= keep;
+    o[1] *= keep;
+    m = mm;
+    return ref;
+  };
+  // This wave's parts, four at a time: their loads do not wait for one another.
   auto join = [&](const Line& line, int parts, auto row_of) __attribute__((always_inline)) {
-    for (int p0 = 0; p0 < parts; p0 += 4) {
+    for (int p0 = wave; p0 < parts; p0 += 16) {
       f32x2 ml[4];
       f32x4 v[4][2];
 #pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        const int64_t at = row_of(min(p0 + p, parts - 1));
-        ml[p] = *reinterpret_cast<const f32x2*>(line.ml + at * 2);
-        const f32x4* const x = reinterpret_cast<const f32x4*>(line.o + at * D + 8 * ch);
-        v[p][0] = x[0];
-        v[p][1] = x[1];
-        if (p0 + p >= parts) ml[p] = f32x2{-INFINITY, 0.f};
+      for (int x = 0; x < 4; ++x) {
+        const int p = p0 + 4 * x;
+        ml[x] = f32x2{-INFINITY, 0.f};
+        v[x][0] = v[x][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (p < parts) {
+          const int64_t at = row_of(p);
+          ml[x] = *reinterpret_cast<const f32x2*>(line.ml + at * 2);
+          const f32x4* const from = reinterpret_cast<const f32x4*>(line.o + at * D + 8 * ch);
+          v[x][0] = from[0];
+          v[x][1] = from[1];
+        }
       }
       float mm = m;
 #pragma unroll
-      for (int p = 0; p < 4; ++p) mm = fmaxf(mm, ml[p][0]);
-      const float ref = mm == -INFINITY ? 0.f : mm;
-      const float keep = fast_exp2(m - ref);
-      l *= keep;
-      o[0] *= keep;
-      o[1] *= keep;
+      for (int x = 0; x < 4; ++x) mm = fmaxf(mm, ml[x][0]);
+      const float ref = rescale(mm);
 #pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        const float wt = fast_exp2(ml[p][0] - ref);
-        if (p0 + p < parts) {
-          l = __builtin_fmaf(ml[p][1], wt, l);
-#pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            o[0][y] = __builtin_fmaf(v[p][0][y], wt, o[0][y]);
-            o[1][y] = __builtin_fmaf(v[p][1][y], wt, o[1][y]);
-          }
-        }
-      }
-      m = mm;
+      for (int x = 0; x < 4; ++x) add(ml[x], v[x], ref);
     }
   };
-  if constexpr (RWP > 0)
-    join(a.pre, pre_parts, [&](int p) { return pre_row + int64_t(p) * (32 * RWP); });
-  join(a.own, rec.parts, own_row);
+  if (valid) {
+    if constexpr (RWP > 0) {
+      const uint32_t pr = uint32_t(b) * uint32_t(a.R) + uint32_t(row);
+      const uint32_t pre_rt = uint32_t(a.B * a.R + 32 * RWP - 1) / (32 * RWP);
+      const Record p = a.pre.rec[uint32_t(hk) * pre_rt + pr / (32 * RWP)];
+      const int64_t first = int64_t(p.slot) * (32 * RWP) + pr % (32 * RWP);
+      join(a.pre, p.parts, [&](int x) { return first + int64_t(x) * (32 * RWP); });
+    }
+    // Of a cut line without a prefix, a broken item's first part is its
+    // workgroup's odd slot, the others are the next workgroups' even ones.
+    const bool broken = RWP == 0 && a.own.splits == 0;
+    join(a.own, rec.parts, [&](int x) {
+      const int64_t slot = int64_t(rec.slot) + (broken ? (x ? 2 * x - 1 : 0) : x);
+      return slot * (32 * RWO) + in_item;
+    });
+  }
+  if (wave > 0) {
+    stats[wave - 1][lane] = f32x2{m, l};
+    sums[wave - 1][lane][0] = o[0];
+    sums[wave - 1][lane][1] = o[1];
+  }
+  __syncthreads();
+  if (wave > 0 || !valid) return;
+  float mm = m;
+#pragma unroll
+  for (int x = 0; x < 3; ++x) mm = fmaxf(mm, stats[x][lane][0]);
+  const float ref = rescale(mm);
+#pragma unroll
+  for (int x = 0; x < 3; ++x) add(stats[x][lane], sums[x][lane], ref);
   const float inv = 1.0f / l;  // no visible key: 0 * inf = NaN
-  const int qi = row / a.group, hq = hk * a.group + row % a.group;
+  const int qi = int(uint32_t(row) / uint32_t(a.group)), hq = hk * a.group + row - qi * a.group;
   char* const op = a.out + b * a.o_sb + qi * a.o_sl + hq * a.o_sh + 8 * ch * Elem<T>::bytes;
   if constexpr (Elem<T>::bytes == 4) {
     reinterpret_cast<f32x4*>(op)[0] = o[0] * inv;
@@ -967,11 +1028,13 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
 // ---------------------------------------------------------------------------
 // Host side: the plan and the launches.
 // ---------------------------------------------------------------------------
+constexpr int64_t kMaxItemCost = 16;  // kItemCost at most
+
 struct PagedPlan {
   int rw_own, rw_pre;            // row waves of a workgroup; rw_pre 0: no prefix
   int own_splits, pre_splits;    // 0: the line is cut
   int64_t own_items, pre_items;
-  int64_t work;                  // tiles of both lines, at the largest lengths
+  int64_t own_work, pre_work;    // lengths of the lines at most, at the largest row counts
   int64_t own_n, grid;           // workgroups
   int64_t own_slots, pre_slots;  // partials of 32 rw rows
   int64_t own_recs, pre_recs;
@@ -979,14 +1042,6 @@ struct PagedPlan {
 };
 
 int row_waves(int64_t rows) { return rows <= 32 ? 1 : 4; }
-
-// LDS of a workgroup (Shape::lds), by what the plan knows.
-int lds_bytes(int64_t D, int64_t es, int rw) {
-  const int64_t rb = D * es, kw = rw == 1 ? (rb >= 512 ? 4 : 8) : kWaves / rw;
-  const int64_t stages = kw * (rw == 1 ? 1 : 2) * 2 * (rw == 1 || rb >= 512 ? 32 : 64) * rb;
-  const int64_t areas = rw * kw * (std::min<int64_t>(D, 128) / 8 * 1040 + 256);
-  return int(std::max(stages, areas) + kWaves * 2 * 16);
-}
 
 // Key ranges per item of a split line: `tiles` per item, rounds of `slots`
 // workgroups, each with the cost of some tiles for its start and end. The
@@ -1004,7 +1059,7 @@ int range_count(int64_t items, int64_t tiles, int64_t slots) {
   return s;
 }
 
-PagedPlan plan_paged(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hkv, int64_t D, int64_t es,
+PagedPlan plan_paged(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hkv, int64_t D,
                      int64_t own_rows, int64_t pre_rows, bool prefix, int cus) {
   PagedPlan p{};
   const int64_t R = Lq * (H / Hkv);
@@ -1013,24 +1068,22 @@ PagedPlan plan_paged(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hkv, 
   p.rw_own = row_waves(R);
   p.own_items = B * Hkv * row_tiles(R, p.rw_own);
   const int64_t own_tiles = tiles(own_rows) + std::max<int64_t>(tiles(Lk), 1);
-  int lds = lds_bytes(D, es, p.rw_own);
-  p.work = p.own_items * own_tiles;
+  p.own_work = p.own_items * (own_tiles + kMaxItemCost);
   int64_t pre_tiles = 0;
   if (prefix) {
     p.rw_pre = row_waves(B * R);
     p.pre_items = Hkv * row_tiles(B * R, p.rw_pre);
     pre_tiles = std::max<int64_t>(tiles(pre_rows), 1);
-    lds = std::max(lds, lds_bytes(D, es, p.rw_pre));
-    p.work += p.pre_items * pre_tiles;
+    p.pre_work = p.pre_items * (pre_tiles + kMaxItemCost);
   }
   // Workgroups that run at once.
-  const int64_t slots = int64_t(cus) * (2 * lds <= 160 * 1024 ? 2 : 1);
+  const int64_t slots = (D == 256 ? 1 : 2) * int64_t(cus);
   if (prefix && row_tiles(B * R, p.rw_pre) > 1) p.pre_splits = range_count(p.pre_items, pre_tiles, slots);
   if (row_tiles(R, p.rw_own) > 1) p.own_splits = range_count(p.own_items, own_tiles, slots);
-  // A cut line: no more of them than its tiles at the largest lengths.
-  p.own_n = p.own_splits ? p.own_items * p.own_splits : std::min(slots, p.own_items * own_tiles);
+  // A cut line: no more of them than it has tiles and items.
+  p.own_n = p.own_splits ? p.own_items * p.own_splits : std::min(slots, p.own_items * (own_tiles + 1));
   const int64_t pre_n = p.pre_splits ? p.pre_items * p.pre_splits
-                                     : std::min(slots, p.pre_items * pre_tiles);
+                                     : std::min(slots, p.pre_items * (pre_tiles + 1));
   p.grid = p.own_n;
   if (prefix) {
     p.grid = p.own_splits || p.pre_splits ? p.own_n + pre_n
@@ -1069,7 +1122,7 @@ hipError_t launch_form(const PagedArgs& a, const PagedPlan& p, hipStream_t st) {
                      st, a);
   e = hipGetLastError();
   if (e != hipSuccess || !p.merge) return e;
-  hipLaunchKernelGGL((paged_merge_kernel<T, D, RWP, RWO>), dim3(unsigned(p.own_recs), RWO, D / 64),
+  hipLaunchKernelGGL((paged_merge_kernel<T, D, RWP, RWO>), dim3(unsigned(p.own_recs), 4 * RWO, D / 64),
                      dim3(256), 0, st, a);
   return hipGetLastError();
 }
@@ -1153,7 +1206,7 @@ int paged_entry(const char* what, const PagedCall& c, bool prefix, void* stream)
     DX_CHECK_ARG(s >= 0 && s * es < (int64_t(1) << 26), "%s: row stride %lld out of range", what,
                  (long long)s);
 
-  const PagedPlan p = plan_paged(c.B, c.Lq, c.Lk, c.H, c.Hkv, c.D, es, c.width * c.page_rows,
+  const PagedPlan p = plan_paged(c.B, c.Lq, c.Lk, c.H, c.Hkv, c.D, c.width * c.page_rows,
                                  c.prefix_width * c.page_rows, prefix, device_cus());
   const int64_t need = plan_bytes(p, c.D);
   if (need > c.ws_bytes || (need > 0 && !c.ws)) {
@@ -1164,7 +1217,9 @@ int paged_entry(const char* what, const PagedCall& c, bool prefix, void* stream)
   DX_CHECK_ARG(al(c.ws), "%s: workspace must be 16-byte aligned", what);
   const int64_t group = c.H / c.Hkv, R = c.Lq * group;
   // Item numbers and slots are 32-bit; the merge takes a workgroup per item.
-  DX_CHECK_ARG(p.work / p.grid < (int64_t(1) << 30), "%s: too many keys for one launch", what);
+  // Lines are counted in 32 bits.
+  DX_CHECK_ARG(p.own_work < (int64_t(1) << 31) && p.pre_work < (int64_t(1) << 31),
+               "%s: too many queries and keys for one launch", what);
   DX_CHECK_ARG(grid_fits(p.own_recs, 256) && grid_fits(p.grid, kThreads) && p.own_items < (int64_t(1) << 30) &&
                    p.pre_items < (int64_t(1) << 30),
                "%s: the call exceeds one launch", what);
@@ -1235,7 +1290,7 @@ extern "C" int64_t dx_paged_attention_workspace_bytes(int dtype, int64_t B, int6
                               prefix_width);
   if (bad) return -bad;
   if (B == 0 || Lq == 0) return 0;
-  const PagedPlan p = plan_paged(B, Lq, Lk, H, Hkv, D, dtype == DX_F32 ? 4 : 2, width * page_rows,
+  const PagedPlan p = plan_paged(B, Lq, Lk, H, Hkv, D, width * page_rows,
                                  prefix_width * page_rows, has_prefix != 0, device_cus());
   return plan_bytes(p, D);
 }
