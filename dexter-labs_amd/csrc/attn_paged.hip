@@ -53,8 +53,8 @@ namespace {
 
 constexpr int kPN = 32;  // keys per tile of the line
 // Where an item's parts are: slot of the first, and their number (one after the
-// other). By item, or, where the line is cut and there is no prefix, by
-// workgroup: the item that it leaves broken (parts 0: none).
+// other; 0: none, its result is written). By item; or, where a cut line without
+// a prefix has more items than workgroups, by workgroup: the item it leaves broken.
 struct Record { int item, slot, parts, pad; };
 
 // A line of work: its partials and records.
@@ -63,6 +63,7 @@ struct Line {
   float* ml;    // [slot][32 RW rows]: {m, l}
   Record* rec;
   int splits;   // key ranges per item; 0: the line is cut into pieces
+  int by_item;  // the records are, and there are some
 };
 
 struct PagedArgs {
@@ -304,23 +305,41 @@ struct Tile {
     m = -INFINITY;
     l = 0.f;
   }
+  // S^T = K Q^T of the tile, K fragments read W ahead of the products that use
+  // them: left alone the compiler reads each right before its product, which
+  // then waits out the LDS latency.
   static __device__ __forceinline__ void scores(uint32_t ka, const u32x4 (&qr)[KS], f32x16 (&s)[NS]) {
+    constexpr int N = KS * NS, W = F32 ? 2 : 4;
+    auto frag = [&](int i) __attribute__((always_inline)) {
+      return lds_read_b128_at((ka ^ (32u * (i / NS))) + 32 * RB * (i % NS));
+    };
+    __builtin_amdgcn_sched_barrier(0);
+    u32x4 kf[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) kf[i] = frag(i);
 #pragma unroll
     for (int x = 0; x < NS; ++x) s[x] = f32x16{};
 #pragma unroll
-    for (int k = 0; k < KS; ++k)
+    for (int i = 0; i < N; ++i) {
+      f32x16& sx = s[i % NS];
+      if constexpr (F32) {
 #pragma unroll
-      for (int x = 0; x < NS; ++x) {
-        const u32x4 kf = lds_read_b128_at((ka ^ (32u * k)) + 32 * RB * x);
-        if constexpr (F32) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            s[x] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(kf[e]),
-                                                        __uint_as_float(qr[k][e]), s[x], 0, 0, 0);
-        } else {
-          s[x] = Mfma<T>::run(kf, qr[k], s[x]);
-        }
+        for (int e = 0; e < 4; ++e)
+          sx = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(kf[i % W][e]),
+                                                    __uint_as_float(qr[i / NS][e]), sx, 0, 0, 0);
+      } else {
+        sx = Mfma<T>::run(kf[i % W], qr[i / NS], sx);
       }
+      if (i + W < N) kf[i % W] = frag(i + W);
+    }
+    constexpr int kMfma = 0x008, kDsRead = 0x100;
+    __builtin_amdgcn_sched_group_barrier(kDsRead, W, 0);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      __builtin_amdgcn_sched_group_barrier(kMfma, F32 ? 4 : 1, 0);
+      if (i + W < N) __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
   }
   // Mask, follow the maximum, exponentials in place. lim: rows of the tile
   // below it are seen (already less 4 g); bad: 16-row groups without a page.
@@ -702,9 +721,9 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
         if (i + 1 < nt) send_tile(i + 1);
         if (i >= nt || !active) continue;
         const uint32_t st = uint32_t(i & 1) * 2 * Sh::tile;
-        const u32x4 fl = *reinterpret_cast<const u32x4*>(flags + 4 * (i & 1));
         f32x16 s[UT];
         Ti::scores(ka + st, qr, s);
+        const u32x4 fl = *reinterpret_cast<const u32x4*>(flags + 4 * (i & 1));
         const int t = tile_at(i);
         bool masked, masked1 = false;
         int lim = limits(t, masked);
@@ -815,13 +834,12 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
         }
       }
     }
-    if (first && (SHARED || !whole)) {
-      left = Record{item, int(slot), splits, 0};
-      if (splits == 0) {
-        // Up to the workgroup that holds the item's last tile.
-        left.parts = int(cut.piece(at + uint32_t(weight) - 1)) - int(w) + 1;
-      }
-      if ((SHARED || splits) && threadIdx.x == 0) (PREFIX ? a.pre.rec : a.own.rec)[item] = left;
+    if (first) {
+      // Parts up to the workgroup that holds the item's last tile.
+      const int parts = splits ? splits : int(cut.piece(at + uint32_t(weight) - 1)) - int(w) + 1;
+      left = Record{item, int(slot), !SHARED && whole ? 0 : parts, 0};
+      if ((PREFIX ? a.pre.by_item : a.own.by_item) && threadIdx.x == 0)
+        (PREFIX ? a.pre.rec : a.own.rec)[item] = left;
     }
     if (splits) return;
     __syncthreads();  // the results are read: tiles may land again
@@ -838,7 +856,7 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
       }
     }
   }
-  if (!SHARED && splits == 0 && threadIdx.x == 0) args->own.rec[w] = left;
+  if (!SHARED && splits == 0 && !args->own.by_item && threadIdx.x == 0) args->own.rec[w] = left;
 }
 
 template <typename T, int D, int RWP, int RWO>
@@ -911,7 +929,7 @@ __global__ __launch_bounds__(kThreads, (Shape<T, D, RWO>::per_cu)) void paged_at
   n_own = uniform(n_own);
   w -= n_pre;
   if (w >= n_own) {
-    if (RWP == 0 && threadIdx.x == 0) a.own.rec[w] = Record{0, 0, 0, 0};
+    if (RWP == 0 && !a.own.by_item && threadIdx.x == 0) a.own.rec[w] = Record{0, 0, 0, 0};
     return;
   }
   if (a.own.splits == 0) w = in_runs(w, n_own);
@@ -1099,8 +1117,8 @@ PagedPlan plan_paged(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hkv, 
     p.own_recs = p.merge ? p.own_items : 0;
   } else {
     p.merge = true;
-    p.own_slots = 2 * p.grid + 1;
-    p.own_recs = p.grid;
+    p.own_slots = 2 * p.grid;
+    p.own_recs = std::min(p.grid, p.own_items);
   }
   return p;
 }
@@ -1244,6 +1262,8 @@ int paged_entry(const char* what, const PagedCall& c, bool prefix, void* stream)
   a.R = int(R);
   a.scale_log2 = c.scale * 1.4426950408889634f;
   a.own.splits = p.own_splits;
+  a.own.by_item = p.own_recs == p.own_items;  // no records: nothing is left to join
+  a.pre.by_item = p.pre_recs > 0;
   a.pre.splits = p.pre_splits;
   a.own_n = int(p.own_n);
   char* ws = static_cast<char*>(c.ws);
