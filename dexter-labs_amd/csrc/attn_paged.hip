@@ -390,17 +390,31 @@ struct Tile {
 #pragma unroll
         for (int r = 0; r < 16; ++r) part[r % 4] += s[x][r];
       l += (part[0] + part[1]) + (part[2] + part[3]);
+      // V read W ahead of the products, as K is in scores().
+      constexpr int N = 16 * NS * DT, W = 8;
+      auto frag = [&](int i) __attribute__((always_inline)) {
+        typedef __attribute__((address_space(3))) float lds_f32;
+        const int x = i / DT / 16, r = i / DT % 16;
+        return *reinterpret_cast<const lds_f32*>((va ^ (128u * (i % DT))) +
+                                                 (32 * x + 8 * (r / 4) + r % 4) * RB);
+      };
+      __builtin_amdgcn_sched_barrier(0);
+      float vf[W];
 #pragma unroll
-      for (int x = 0; x < NS; ++x)
+      for (int i = 0; i < W; ++i) vf[i] = frag(i);
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
+      for (int i = 0; i < N; ++i) {
+        acc[i % DT] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf[i % W], s[i / DT / 16][i / DT % 16],
+                                                           acc[i % DT], 0, 0, 0);
+        if (i + W < N) vf[i % W] = frag(i + W);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x100, W, 0);
 #pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            typedef __attribute__((address_space(3))) float lds_f32;
-            const float vf = *reinterpret_cast<const lds_f32*>(
-                (va ^ (128u * d)) + (32 * x + 8 * (r / 4) + r % 4) * RB);
-            acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf, s[x][r], acc[d], 0, 0, 0);
-          }
+      for (int i = 0; i < N; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if (i + W < N) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     } else {
       u32x4 pk[2 * NS];
       float part[2] = {0.f, 0.f};
@@ -560,12 +574,13 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
     uint32_t slot;
     const bool first = t0 == 0;  // this share holds the item's first tile: it leaves the record
     bool active, behind = false;
+    int history;  // what the masks call the cache
     {
       Args& a = *reread(args);
       const int nrows = PREFIX ? a.B * a.R : a.R;
       const int pre_len = __builtin_amdgcn_readfirstlane(prefix_rows(a));
       const int own_len = PREFIX ? 0 : __builtin_amdgcn_readfirstlane(own_rows(a, b));
-      const int history = pre_len + own_len;  // what the masks call the cache
+      history = pre_len + own_len;
       EndBounds eb{0, 0};
       if (!PREFIX) eb = end_bounds(a, row0 / a.group, (min(row0 + 32 * RW, nrows) - 1) / a.group);
       full_end = eb.lo;
@@ -606,10 +621,16 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
       keys.n_pages = a.n_pages;
       c = fmaxf(fabsf(a.scale_log2), FLT_MIN);
 
-      // This lane's row: query head hq of query qi of sequence bq.
+      active = row0 + wave * 32 < nrows && stream < KW;  // wave-uniform
+    }
+    // This lane's row: query head hq of query qi of sequence bq; its queries, and
+    // how many of the new keys it sees. Called once the first tiles are on their
+    // way: one wait is both's.
+    auto load_queries = [&]() __attribute__((always_inline)) {
+      Args& a = *reread(args);
+      const int nrows = PREFIX ? a.B * a.R : a.R;
       const int row = row0 + wave * 32 + nl;
       const bool rvalid = row < nrows;
-      active = row0 + wave * 32 < nrows && stream < KW;  // wave-uniform
       int bq = b;
       const uint32_t r = uint32_t(rvalid ? row : nrows - 1);
       uint32_t rr = r;
@@ -624,7 +645,7 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
 #pragma unroll
       for (int s = 0; s < KS; ++s) qr[s] = *reinterpret_cast<const u32x4*>(qp + 32 * s) ^ flip;
       if (!PREFIX && rvalid) my_end = visible_end(a, qi, history);  // new keys seen
-    }
+    };
 
     const uint32_t base = lds_addr(smem) + stream * Sh::stream;
     const uint32_t ka = base + nl * RB + 16 * (g ^ kswz<RB>(nl));
@@ -672,6 +693,7 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
         find(tile_at(0));
         send_v();
       }
+      load_queries();
       for (int i = 0; i < nt; ++i) {
         const bool more = i + 1 < nt;
         const uint32_t bad = gone;
@@ -711,6 +733,7 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
         send_rows<RB, F32, false>(v, rows, sv, to + Sh::tile, tr % 16, tr, WR / RPP, lane);
       };
       if (nt > 0) send_tile(0);
+      load_queries();
       for (int i = 0; i < iters; ++i) {
         // This wave's pieces of tile i have landed; past the barrier the tile
         // is whole, and reads of the stage that is sent to next have returned.
@@ -1153,26 +1176,13 @@ hipError_t launch_paged(const PagedArgs& a, const PagedPlan& p, hipStream_t st) 
   return p.rw_own == 1 ? launch_form<T, D, 4, 1>(a, p, st) : launch_form<T, D, 4, 4>(a, p, st);
 }
 
-struct PagedCall {
-  const void* q; int64_t q_sb, q_sl, q_sh;
-  const void* k; int64_t k_sb, k_sl, k_sh;
-  const void* v; int64_t v_sb, v_sl, v_sh;
-  const void* pages; int64_t p_plane, p_sp, p_sr, p_sh, n_pages, page_rows;
-  const void* prefix_table; int64_t prefix_width; const void* prefix_len;
-  const void* table; int64_t t_sb, width; const void* lens;
-  void* out; int64_t o_sb, o_sl, o_sh;
-  int dtype; int64_t B, Lq, Lk, H, Hkv, D;
-  const void* starts; int starts_dtype; int64_t n_blocks; int causal; float scale;
-  void* ws; int64_t ws_bytes;
-};
-
 constexpr int64_t kMaxRows = int64_t(1) << 30;  // rows of a sequence or prefix, and keys
 
 // Sizes that the kernels' 32-bit arithmetic and one launch hold.
 int check_sizes(const char* what, int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hkv,
-                int64_t D, int dtype, int64_t page_rows, int64_t width, int64_t prefix_width) {
+                int64_t D, int64_t dtype, int64_t page_rows, int64_t width, int64_t prefix_width) {
   DX_CHECK_ARG(dtype == DX_BF16 || dtype == DX_F16 || dtype == DX_F32,
-               "%s: dtype code %d unsupported", what, dtype);
+               "%s: dtype code %lld unsupported", what, (long long)dtype);
   DX_CHECK_ARG(D == 64 || D == 128 || (D == 256 && dtype != DX_F32),
                "%s: head_dim %lld (supported: 64, 128, and 256 in 16 bits)", what, (long long)D);
   DX_CHECK_ARG(B >= 0 && Lq >= 0 && Lk >= 0 && H > 0 && Hkv > 0 && width >= 0 && prefix_width >= 0,
@@ -1192,7 +1202,13 @@ int check_sizes(const char* what, int64_t B, int64_t Lq, int64_t Lk, int64_t H, 
   return DX_OK;
 }
 
-int paged_entry(const char* what, const PagedCall& c, bool prefix, void* stream) {
+int paged_entry(const char* what, const dx_paged_call* call, bool prefix) {
+  DX_CHECK_ARG(call, "%s: null call", what);
+  dx_paged_call c = *call;
+  if (!prefix) {
+    c.prefix_table = c.prefix_len = nullptr;
+    c.prefix_width = 0;
+  }
   const int bad = check_sizes(what, c.B, c.Lq, c.Lk, c.H, c.Hkv, c.D, c.dtype, c.page_rows, c.width,
                               c.prefix_width);
   if (bad) return bad;
@@ -1200,17 +1216,17 @@ int paged_entry(const char* what, const PagedCall& c, bool prefix, void* stream)
   DX_CHECK_ARG(c.n_blocks >= 0 && c.n_blocks < kMaxRows &&
                    (c.starts_dtype == DX_I32 || c.starts_dtype == DX_I64),
                "%s: bad block starts", what);
-  DX_CHECK_ARG(c.n_blocks == 0 || c.starts, "%s: null block starts", what);
+  DX_CHECK_ARG(c.n_blocks == 0 || c.block_starts, "%s: null block starts", what);
   DX_CHECK_ARG(c.Lk == c.Lq || (!c.causal && c.n_blocks == 0),
                "%s: k/v length %lld must equal q length %lld with block starts or causal", what,
                (long long)c.Lk, (long long)c.Lq);
-  DX_CHECK_ARG(std::isfinite(c.scale), "%s: softmax scale must be finite", what);
+  DX_CHECK_ARG(std::isfinite(float(c.softmax_scale)), "%s: softmax scale must be finite", what);
   if (c.B == 0 || c.Lq == 0) return DX_OK;
   const int64_t es = c.dtype == DX_F32 ? 4 : 2, per16 = 16 / es;
   auto al = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
   DX_CHECK_ARG(c.q && c.out, "%s: null pointer", what);
   DX_CHECK_ARG(c.Lk == 0 || (c.k && c.v), "%s: null k or v", what);
-  DX_CHECK_ARG(c.width == 0 || (c.table && c.lens), "%s: null block table or lengths", what);
+  DX_CHECK_ARG(c.width == 0 || (c.block_table && c.cache_lens), "%s: null block table or lengths", what);
   DX_CHECK_ARG(!prefix || c.prefix_len, "%s: null prefix length", what);
   DX_CHECK_ARG(c.prefix_width == 0 || c.prefix_table, "%s: null prefix table", what);
   DX_CHECK_ARG(c.n_pages == 0 || c.pages, "%s: null pages", what);
@@ -1227,12 +1243,12 @@ int paged_entry(const char* what, const PagedCall& c, bool prefix, void* stream)
   const PagedPlan p = plan_paged(c.B, c.Lq, c.Lk, c.H, c.Hkv, c.D, c.width * c.page_rows,
                                  c.prefix_width * c.page_rows, prefix, device_cus());
   const int64_t need = plan_bytes(p, c.D);
-  if (need > c.ws_bytes || (need > 0 && !c.ws)) {
-    set_error("%s: workspace of %lld bytes, %lld needed", what, (long long)(c.ws ? c.ws_bytes : 0),
+  if (need > c.workspace_bytes || (need > 0 && !c.workspace)) {
+    set_error("%s: workspace of %lld bytes, %lld needed", what, (long long)(c.workspace ? c.workspace_bytes : 0),
               (long long)need);
     return DX_EWORKSPACE;
   }
-  DX_CHECK_ARG(al(c.ws), "%s: workspace must be 16-byte aligned", what);
+  DX_CHECK_ARG(al(c.workspace), "%s: workspace must be 16-byte aligned", what);
   const int64_t group = c.H / c.Hkv, R = c.Lq * group;
   // Item numbers and slots are 32-bit; the merge takes a workgroup per item.
   // Lines are counted in 32 bits.
@@ -1248,25 +1264,25 @@ int paged_entry(const char* what, const PagedCall& c, bool prefix, void* stream)
   a.pk = static_cast<const char*>(c.pages); a.pv = a.pk + c.p_plane * es;
   a.p_sp = c.p_sp * es; a.p_sr = c.p_sr * es; a.p_sh = c.p_sh * es;
   a.out = static_cast<char*>(c.out); a.o_sb = c.o_sb * es; a.o_sl = c.o_sl * es; a.o_sh = c.o_sh * es;
-  a.table = static_cast<const int32_t*>(c.table); a.t_sb = c.t_sb;
-  a.lens = static_cast<const int32_t*>(c.lens);
+  a.table = static_cast<const int32_t*>(c.block_table); a.t_sb = c.t_sb;
+  a.lens = static_cast<const int32_t*>(c.cache_lens);
   a.ptable = static_cast<const int32_t*>(c.prefix_table);
   a.plen = prefix ? static_cast<const int32_t*>(c.prefix_len) : nullptr;
   a.width = int(c.width); a.pwidth = int(c.prefix_width);
   a.n_pages = int(c.n_pages); a.page_rows = int(c.page_rows);
   const uint64_t per = uint64_t(c.page_rows / 16);
   a.page_magic = per == 1 ? 0u : uint32_t(((uint64_t(1) << 32) + per - 1) / per);
-  a.starts = c.starts; a.starts_i64 = c.starts_dtype == DX_I64; a.n_blocks = int(c.n_blocks);
+  a.starts = c.block_starts; a.starts_i64 = c.starts_dtype == DX_I64; a.n_blocks = int(c.n_blocks);
   a.B = int(c.B); a.H = int(c.H); a.Hkv = int(c.Hkv); a.group = int(group);
   a.Lq = int(c.Lq); a.Lk = int(c.Lk); a.causal = c.causal != 0;
   a.R = int(R);
-  a.scale_log2 = c.scale * 1.4426950408889634f;
+  a.scale_log2 = float(c.softmax_scale * 1.4426950408889634);
   a.own.splits = p.own_splits;
   a.own.by_item = p.own_recs == p.own_items;  // no records: nothing is left to join
   a.pre.by_item = p.pre_recs > 0;
   a.pre.splits = p.pre_splits;
   a.own_n = int(p.own_n);
-  char* ws = static_cast<char*>(c.ws);
+  char* ws = static_cast<char*>(c.workspace);
   auto take = [&](int64_t bytes) {
     char* const at = ws;
     ws += bytes;
@@ -1278,7 +1294,7 @@ int paged_entry(const char* what, const PagedCall& c, bool prefix, void* stream)
   a.pre.ml = reinterpret_cast<float*>(take(p.pre_slots * 32 * p.rw_pre * 8));
   a.own.rec = reinterpret_cast<Record*>(take(p.own_recs * int64_t(sizeof(Record))));
   a.pre.rec = reinterpret_cast<Record*>(take(p.pre_recs * int64_t(sizeof(Record))));
-  const hipStream_t st = static_cast<hipStream_t>(stream);
+  const hipStream_t st = static_cast<hipStream_t>(c.stream);
   hipError_t e;
   if (c.dtype == DX_F32)
     e = c.D == 64 ? launch_paged<float, 64>(a, p, st) : launch_paged<float, 128>(a, p, st);
@@ -1315,42 +1331,10 @@ extern "C" int64_t dx_paged_attention_workspace_bytes(int dtype, int64_t B, int6
   return plan_bytes(p, D);
 }
 
-extern "C" int dx_paged_attention(
-    const void* q, int64_t q_sb, int64_t q_sl, int64_t q_sh,
-    const void* k, int64_t k_sb, int64_t k_sl, int64_t k_sh,
-    const void* v, int64_t v_sb, int64_t v_sl, int64_t v_sh,
-    const void* pages, int64_t p_plane, int64_t p_sp, int64_t p_sr, int64_t p_sh,
-    int64_t n_pages, int64_t page_rows,
-    const void* block_table, int64_t t_sb, int64_t width, const void* cache_lens,
-    void* out, int64_t o_sb, int64_t o_sl, int64_t o_sh,
-    int dtype, int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hkv, int64_t D,
-    const void* block_starts, int starts_dtype, int64_t n_blocks, int causal, float softmax_scale,
-    void* workspace, int64_t workspace_bytes, void* stream) {
-  const PagedCall c{q, q_sb, q_sl, q_sh, k, k_sb, k_sl, k_sh, v, v_sb, v_sl, v_sh,
-                    pages, p_plane, p_sp, p_sr, p_sh, n_pages, page_rows, nullptr, 0, nullptr,
-                    block_table, t_sb, width, cache_lens, out, o_sb, o_sl, o_sh,
-                    dtype, B, Lq, Lk, H, Hkv, D, block_starts, starts_dtype, n_blocks, causal,
-                    softmax_scale, workspace, workspace_bytes};
-  return paged_entry("paged_attention", c, false, stream);
+extern "C" int dx_paged_attention(const dx_paged_call* call) {
+  return paged_entry("paged_attention", call, false);
 }
 
-extern "C" int dx_shared_prefix_attention(
-    const void* q, int64_t q_sb, int64_t q_sl, int64_t q_sh,
-    const void* k, int64_t k_sb, int64_t k_sl, int64_t k_sh,
-    const void* v, int64_t v_sb, int64_t v_sl, int64_t v_sh,
-    const void* pages, int64_t p_plane, int64_t p_sp, int64_t p_sr, int64_t p_sh,
-    int64_t n_pages, int64_t page_rows,
-    const void* prefix_table, int64_t prefix_width, const void* prefix_len,
-    const void* block_table, int64_t t_sb, int64_t width, const void* cache_lens,
-    void* out, int64_t o_sb, int64_t o_sl, int64_t o_sh,
-    int dtype, int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hkv, int64_t D,
-    const void* block_starts, int starts_dtype, int64_t n_blocks, int causal, float softmax_scale,
-    void* workspace, int64_t workspace_bytes, void* stream) {
-  const PagedCall c{q, q_sb, q_sl, q_sh, k, k_sb, k_sl, k_sh, v, v_sb, v_sl, v_sh,
-                    pages, p_plane, p_sp, p_sr, p_sh, n_pages, page_rows,
-                    prefix_table, prefix_width, prefix_len,
-                    block_table, t_sb, width, cache_lens, out, o_sb, o_sl, o_sh,
-                    dtype, B, Lq, Lk, H, Hkv, D, block_starts, starts_dtype, n_blocks, causal,
-                    softmax_scale, workspace, workspace_bytes};
-  return paged_entry("shared_prefix_attention", c, true, stream);
+extern "C" int dx_shared_prefix_attention(const dx_paged_call* call) {
+  return paged_entry("shared_prefix_attention", call, true);
 }

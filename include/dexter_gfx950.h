@@ -505,49 +505,51 @@ int dx_kv_page_copy(const void* const* pools, int64_t n_pools,
                     const int64_t* src, const int64_t* dst, int64_t pairs, void* stream);
 
 /*
+ * A call of dx_paged_attention or dx_shared_prefix_attention. Every field is 8
+ * bytes wide (a binding packs them in this order); strides are in elements.
+ * Unused pointers are NULL.
+ */
+typedef struct dx_paged_call {
+  const void* q; int64_t q_sb, q_sl, q_sh;          /* [B, Lq, H, D] */
+  const void* k; int64_t k_sb, k_sl, k_sh;          /* [B, Lk, Hkv, D] */
+  const void* v; int64_t v_sb, v_sl, v_sh;
+  void* out; int64_t o_sb, o_sl, o_sh;              /* [B, Lq, H, D] */
+  const void* pages; int64_t p_plane, p_sp, p_sr, p_sh, n_pages, page_rows;
+  const void* block_table; int64_t t_sb, width;     /* int32 [B, width], row stride t_sb */
+  const void* cache_lens;                           /* int32 [B] */
+  const void* prefix_table; int64_t prefix_width;   /* int32 [prefix_width] */
+  const void* prefix_len;                           /* int32 [1] */
+  int64_t dtype, B, Lq, Lk, H, Hkv, D;
+  const void* block_starts; int64_t starts_dtype, n_blocks;
+  int64_t causal;
+  double softmax_scale;
+  void* workspace; int64_t workspace_bytes;
+  void* stream;
+} dx_paged_call;
+
+/*
  * dx_blockwise_causal_attention with sequence b's cached rows [0, cache_lens[b])
  * in pages: keys = [paged rows | k/v rows 0..Lk)], the same masks and NaN rows,
- * with cache_lens[b] (int32 [B], clamped to [0, width * page_rows]) as the cache
- * length. Keys of an entry that holds no rows are not seen. Lk may be 0; width
- * may be 0 (block_table and cache_lens NULL). page_rows: a multiple of 16 up to
- * 1024. dtype: DX_BF16 or DX_F16 at D 64, 128 or 256, DX_F32 at D 64 or 128;
- * sums and softmax in fp32, one rounding to dtype. Sequences hold fewer than
- * 2^30 rows; the pool may exceed 4 GB. Row strides of the pool, k and v are
- * below 2^26 bytes. workspace: dx_paged_attention_workspace_bytes(...) bytes, 16-byte
+ * with cache_lens[b] (clamped to [0, width * page_rows]) as the cache length.
+ * Keys of a table entry that holds no rows are not seen. Lk may be 0; width may
+ * be 0 (block_table and cache_lens NULL). page_rows: a multiple of 16 up to 1024.
+ * dtype: DX_BF16 or DX_F16 at D 64, 128 or 256, DX_F32 at D 64 or 128; sums and
+ * softmax in fp32, one rounding to dtype. Sequences hold fewer than 2^30 rows;
+ * the pool may exceed 4 GB. Row strides of the pool, k and v are below 2^26
+ * bytes. workspace: dx_paged_attention_workspace_bytes(...) bytes, 16-byte
  * aligned, no initialisation (NULL when 0); calls that share one must not
- * overlap.
+ * overlap. The prefix fields are not read.
  */
-int dx_paged_attention(
-    const void* q, int64_t q_sb, int64_t q_sl, int64_t q_sh,
-    const void* k, int64_t k_sb, int64_t k_sl, int64_t k_sh,
-    const void* v, int64_t v_sb, int64_t v_sl, int64_t v_sh,
-    const void* pages, int64_t p_plane, int64_t p_sp, int64_t p_sr, int64_t p_sh,
-    int64_t n_pages, int64_t page_rows,
-    const void* block_table, int64_t t_sb, int64_t width, const void* cache_lens,
-    void* out, int64_t o_sb, int64_t o_sl, int64_t o_sh,
-    int dtype, int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hkv, int64_t D,
-    const void* block_starts, int starts_dtype, int64_t n_blocks, int causal, float softmax_scale,
-    void* workspace, int64_t workspace_bytes, void* stream);
+int dx_paged_attention(const dx_paged_call* call);
 
 /*
  * dx_paged_attention with a prefix in front of every sequence's keys: rows
  * [0, *prefix_len) (one int32 on the device, clamped to what the table holds) of
- * the pages prefix_table (int32 [prefix_width]). keys = [prefix | paged rows |
- * k/v]; the masks' cache length is *prefix_len + cache_lens[b]. The prefix's keys
- * and values are read for all B * Lq queries at once.
+ * the pages prefix_table. keys = [prefix | paged rows | k/v]; the masks' cache
+ * length is *prefix_len + cache_lens[b]. The prefix's keys and values are read
+ * for all B * Lq queries at once.
  */
-int dx_shared_prefix_attention(
-    const void* q, int64_t q_sb, int64_t q_sl, int64_t q_sh,
-    const void* k, int64_t k_sb, int64_t k_sl, int64_t k_sh,
-    const void* v, int64_t v_sb, int64_t v_sl, int64_t v_sh,
-    const void* pages, int64_t p_plane, int64_t p_sp, int64_t p_sr, int64_t p_sh,
-    int64_t n_pages, int64_t page_rows,
-    const void* prefix_table, int64_t prefix_width, const void* prefix_len,
-    const void* block_table, int64_t t_sb, int64_t width, const void* cache_lens,
-    void* out, int64_t o_sb, int64_t o_sl, int64_t o_sh,
-    int dtype, int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hkv, int64_t D,
-    const void* block_starts, int starts_dtype, int64_t n_blocks, int causal, float softmax_scale,
-    void* workspace, int64_t workspace_bytes, void* stream);
+int dx_shared_prefix_attention(const dx_paged_call* call);
 
 /*
  * Workspace bytes of dx_paged_attention (has_prefix 0) or

@@ -270,6 +270,23 @@ def test_strided_inputs(device, built_lib):
         _case(device, dtype, dim, lens=[40, 90], lq=20, prefix_len=50, strided=True, what="strided")
 
 
+def test_misaligned_inputs_are_copied(device, built_lib):
+    """Contiguous q, k, v that begin off a 16-byte boundary."""
+    lens, lq, heads, dim, rows = [20], 5, 2, 64, 16
+    count, tables, _ = _tables(lens, rows, 1)
+    pages = _rand((2, count, rows, heads, dim), torch.bfloat16, 2).to(device)
+    q, k, v = (_rand((1, lq, heads, dim), torch.bfloat16, s).to(device) for s in (3, 4, 5))
+    odd = [torch.cat((torch.zeros_like(t.flatten()[:1]), t.flatten()))[1:].view(t.shape)
+           for t in (q, k, v)]
+    assert all(t.data_ptr() % 16 and t.is_contiguous() for t in odd)
+    args = dict(pages=pages, block_table=_i32(tables, device), cache_lens=_i32(lens, device))
+    assert torch.equal(ops.paged_attention(*odd, **args), ops.paged_attention(q, k, v, **args))
+    other = pages.clone()
+    ops.kv_page_append(pages, k, v, args["block_table"], _i32([3], device))
+    ops.kv_page_append(other, *odd[1:], args["block_table"], _i32([3], device))
+    assert torch.equal(pages, other)
+
+
 def test_entries_without_a_page_hide_their_keys(device, built_lib):
     """Dropped pages (-1), numbers past the pool: their keys are not seen, whichever half of a
     tile they fall in; lengths past the table, and negative ones, are clamped."""

@@ -3,12 +3,15 @@
 from __future__ import annotations
 
 import ctypes
+import re
+from pathlib import Path
 
 import pytest
 import torch
 
 from dexter_amd.ops.gfx950 import _lib, paged
 
+HEADER = Path(__file__).resolve().parents[1] / "include" / "dexter_gfx950.h"
 BF, F32, I32 = _lib.DX_BF16, _lib.DX_F32, _lib.DX_I32
 
 
@@ -66,17 +69,18 @@ def test_copy_refusals(built_lib):
 def _attend(lib, prefix=False, *, q=16, out=16, pages=16, dtype=BF, b=2, lq=4, lk=4, h=4, hkv=2,
             d=128, rows=16, width=3, table=16, lens=16, n_blocks=0, starts=None, causal=0, scale=1.0,
             ws=None, ws_bytes=0, p_sr=256, q_sl=512, p_width=2, p_table=16, p_len=16):
-    args = [q, 2048, q_sl, 128, 16, 1024, 256, 128, 16, 1024, 256, 128, pages, 1 << 20, 4096, p_sr,
-            128, 8, rows]
-    if prefix:
-        args += [p_table, p_width, p_len]
-    args += [table, width, width, lens, out, 2048, 512, 128, dtype, b, lq, lk, h, hkv, d, starts, I32,
-             n_blocks, causal, scale, ws, ws_bytes, None]
-    return (lib.dx_shared_prefix_attention if prefix else lib.dx_paged_attention)(*args)
+    z = lambda x: 0 if x is None else x  # noqa: E731
+    call = _lib.PAGED_CALL.pack(
+        z(q), 2048, q_sl, 128, 16, 1024, 256, 128, 16, 1024, 256, 128, z(out), 2048, 512, 128,
+        z(pages), 1 << 20, 4096, p_sr, 128, 8, rows, z(table), width, width, z(lens),
+        z(p_table), p_width, z(p_len), dtype, b, lq, lk, h, hkv, d, z(starts), I32, n_blocks,
+        causal, scale, z(ws), ws_bytes, 0)
+    return (lib.dx_shared_prefix_attention if prefix else lib.dx_paged_attention)(call)
 
 
 def test_attention_refusals(built_lib):
     lib = _lib.load()
+    assert "null call" in _message(lib, lib.dx_paged_attention(None))
     for prefix in (False, True):
         def bad(**kw):
             return _message(lib, _attend(lib, prefix, **kw))
@@ -182,6 +186,31 @@ def test_append_argument_checks():
             (dict(pages=t["pages"][:1]), "pages must be")]:
         with pytest.raises(ValueError, match=message):
             call(**change)
+
+
+def test_tensors_off_the_gpu_are_refused():
+    """A pinned implementation is called without its predicate: it checks the device itself."""
+    t = _tensors()
+    with pytest.raises(ValueError, match="GPU"):
+        _call(t)
+    with pytest.raises(ValueError, match="GPU"):
+        paged.kv_page_append(t["pages"], t["k"], t["v"], t["table"], t["lens"])
+    with pytest.raises(ValueError, match="GPU"):
+        paged.kv_page_copy([t["pages"]], [0], [1])
+
+
+def test_packed_call_matches_the_header():
+    """PAGED_CALL has a field for each of struct dx_paged_call's, in its order."""
+    text = HEADER.read_text()
+    body = text[text.index("typedef struct dx_paged_call {"):text.index("} dx_paged_call;")]
+    body = re.sub(r"/\*.*?\*/", "", body, flags=re.S).split("{", 1)[1]
+    kinds = []
+    for part in body.split(";"):
+        words = part.replace("*", " ").split()
+        if words:
+            kinds += ["d" if "double" in words else "q"] * (part.count(",") + 1)
+    fmt = "".join(c * int(n or 1) for n, c in re.findall(r"(\d*)([qd])", _lib.PAGED_CALL.format))
+    assert fmt == "".join(kinds) and _lib.PAGED_CALL.size == 8 * len(kinds)
 
 
 def test_copy_argument_checks():
