@@ -15,6 +15,10 @@ the projections, the prologue and the cache write in two kernels, and up to
 chunks use ``torch.nn.functional.linear`` (hipBLASLt) for the projections and,
 with a host cache length, ``ops.qk_norm_rope_attention`` for the prologue,
 append and attention in one call.
+
+With a ``PagedKVCache`` the same steps run over pages: the projections and the
+prologue as above, then ``PagedKVCache.append`` and ``PagedKVCache.attend``
+(``ops.paged_attention``, or ``ops.shared_prefix_attention`` when it holds a prefix).
 """
 
 from __future__ import annotations
@@ -29,6 +33,7 @@ from torch.utils._device import DeviceContext
 from .. import ops
 from ..registry import NoKernelError, select
 from .kv_cache import KVCache
+from .paged_kv_cache import PagedKVCache
 
 
 def _computes_only(*params) -> bool:
@@ -63,11 +68,13 @@ class SelfAttention(nn.Module):
 
     @torch.no_grad()
     def forward(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
-                kv_cache: KVCache | None, layer: int,
+                kv_cache: KVCache | PagedKVCache | None, layer: int,
                 block_boundaries: torch.Tensor | None = None, write: bool = False,
                 fused_append: bool = True, fused_qkv: bool = True) -> torch.Tensor:
         b, seq, dim = x.shape
         shape = (b, seq, self.heads, self.head_dim)
+        if isinstance(kv_cache, PagedKVCache):
+            return self._paged(x, cos, sin, kv_cache, layer, block_boundaries, write, fused_qkv)
         # Read before appending; with a device cursor this is the cursor itself,
         # which the commit after all layers advances.
         cache_len = kv_cache.cache_len if kv_cache is not None else 0
@@ -104,6 +111,24 @@ class SelfAttention(nn.Module):
             if append:
                 kv_cache.append(layer, k, v)
         return self._attend(q, k, v, kv_cache, layer, cache_len, block_boundaries)
+
+    def _paged(self, x, cos, sin, kv_cache, layer, block_boundaries, write, fused_qkv):
+        b, seq, dim = x.shape
+        if write:
+            kv_cache.reserve(seq)  # "KV cache full" before anything is written
+        if fused_qkv and b * seq <= 128 and dim % 512 == 0 and self.head_dim % 16 == 0:
+            q, k, v = ops.qkv_norm_rope(
+                x, self.q.weight, self.q.bias, self.k.weight, self.k.bias, self.v.weight,
+                self.v.bias, self.q_norm, self.k_norm, cos, sin, self.heads, self.eps)
+        else:
+            shape = (b, seq, self.heads, self.head_dim)
+            q = F.linear(x, self.q.weight, self.q.bias).view(shape)
+            k = F.linear(x, self.k.weight, self.k.bias).view(shape)
+            v = F.linear(x, self.v.weight, self.v.bias).view(shape)
+            q, k = ops.qk_norm_rope(q, k, self.q_norm, self.k_norm, cos, sin, self.eps)
+        if write:
+            kv_cache.append(layer, k, v)
+        return self._project_out(kv_cache.attend(layer, q, k, v, block_boundaries))
 
     def _attend(self, q, k, v, kv_cache, layer, cache_len, block_boundaries):
         out = ops.blockwise_causal_attention(

@@ -30,6 +30,7 @@ from typing import Callable, Sequence
 import torch
 
 from ..models.kv_cache import KVCache
+from ..models.paged_kv_cache import PagedKVCache
 
 
 class GraphRunner:
@@ -105,29 +106,32 @@ def capture(fn: Callable[..., object], sample_inputs: Sequence[torch.Tensor],
 
 
 class CachedStepGraph:
-    """A captured step that appends ``rows`` rows to device-cursor KV caches and commits them.
+    """A captured step that appends ``rows`` rows to device-cursor KV caches (or to paged
+    ones, whose lengths are on the device always) and commits them.
 
     ``fn(*inputs)`` runs one step: its layers append at each cache's cursor
     (``KVCache.append`` / ``append_fused``) and read ``cache_len`` from it, and it
     calls ``commit(rows)`` on every cache in ``caches`` once, at its end. The
     eager warm-up and the capture leave the caches' cursors, host lengths and
     statuses as they found them; rows the warm-up wrote past the cursor are
-    rewritten by the first replay.
+    rewritten by the first replay. A paged cache's pages for the next rows are
+    reserved before each replay, outside the graph, which reads the table that
+    changed in place; whether it has a prefix is fixed by the capture.
     """
 
     def __init__(self, fn: Callable[..., object], sample_inputs: Sequence[torch.Tensor],
-                 caches: Sequence[KVCache], rows: int, warmup: int = 2) -> None:
+                 caches: Sequence[KVCache | PagedKVCache], rows: int, warmup: int = 2) -> None:
         if not caches or any(c.cursor is None for c in caches):
             raise ValueError("CachedStepGraph needs KVCache(device_cursor=True) caches")
         self.caches = list(caches)
         self.rows = int(rows)
         for c in self.caches:
             c._check_room(self.rows)
-        saved = [(c.length, c.cursor.clone(), c.status.clone()) for c in self.caches]
+        saved = [(c._host_state(), c.cursor.clone(), c.status.clone()) for c in self.caches]
 
         def restore():
-            for c, (length, cursor, status) in zip(self.caches, saved):
-                c.length = length
+            for c, (host, cursor, status) in zip(self.caches, saved):
+                c._restore_host(host)
                 c.cursor.copy_(cursor)
                 c.status.copy_(status)
 
@@ -135,13 +139,13 @@ class CachedStepGraph:
                               after_each_warmup=restore)
         # Recording ran fn's host code once (its commits moved the host lengths)
         # but no kernel: restore the host side only.
-        for c, (length, _, _) in zip(self.caches, saved):
-            c.length = length
+        for c, (host, _, _) in zip(self.caches, saved):
+            c._restore_host(host)
 
     def __call__(self, *args: torch.Tensor) -> tuple[torch.Tensor, ...]:
         for c in self.caches:
             c._check_room(self.rows)
         out = self.runner(*args)
         for c in self.caches:
-            c.length += self.rows
+            c._advance(self.rows)
         return out
