@@ -311,6 +311,68 @@ def test_all_pages_dropped(device, built_lib):
     assert torch.isnan(out.float()).all()
 
 
+@pytest.mark.parametrize("dtype,dim", TYPES, ids=IDS)
+@pytest.mark.parametrize("lq,prefix_len", [(9, 0), (45, 0), (200, 0), (45, 70)])
+@pytest.mark.parametrize("mask", ["causal", "blocks"])
+def test_nothing_unseen_is_taken(device, built_lib, dtype, dim, lq, prefix_len, mask):
+    """Infinities and NaN in keys and values that a query does not see, in the same tile as
+    some that it does: its result is bit for bit what it was. Queries that see them get a
+    result that is not finite in the columns that are not, and the others' bits elsewhere."""
+    b, heads, rows, lens = 2, 2, 16, [21, 40]
+    count, tables, prefix = _tables(lens, rows, 1, prefix_rows=prefix_len)
+    pages = _rand((2, count, rows, heads, dim), dtype, 2).to(device)
+    q, k, v = (_rand((b, lq, heads, dim), dtype, s).to(device) for s in (3, 4, 5))
+    args = dict(pages=pages, block_table=_i32(tables, device), cache_lens=_i32(lens, device))
+    if mask == "causal":
+        args["causal"] = True
+        end = torch.arange(lq)
+    else:
+        args["block_boundaries"] = torch.arange(0, lq, 7).to(device)
+        end = (torch.arange(lq) // 7 + 1) * 7 - 1
+
+    def run():
+        if prefix_len:
+            return ops.shared_prefix_attention(q, k, v, prefix_table=_i32(prefix, device),
+                                               prefix_len=_i32([prefix_len], device), **args)
+        return ops.paged_attention(q, k, v, **args)
+    want = run()
+    for at, col, bad in ((5, 3, math.inf), (5, 30, math.nan), (lq - 2, 50, -math.inf), (7, 63, math.nan)):
+        v[1, at, 1, col] = bad
+    got = run()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1, :, 0], want[1, :, 0])
+    for at, cols in ((5, [3, 30]), (lq - 2, [50]), (7, [63])):
+        sees = (end >= at).to(device)
+        hit = got[1, :, 1][:, cols]
+        assert torch.equal(hit[~sees], want[1, :, 1][:, cols][~sees])
+        assert not torch.isfinite(hit[sees].float()).any()
+    clean = [c for c in range(dim) if c not in (3, 30, 50, 63)]
+    assert torch.equal(got[1, :, 1][:, clean], want[1, :, 1][:, clean])
+    assert torch.equal(got[1, end >= 5, 1, 3].float().isinf().cpu(), torch.ones(int((end >= 5).sum()), dtype=torch.bool))
+    # A key that is not finite: whole rows, of those that see it.
+    k[0, 6, 0, 1] = math.nan
+    got = run()
+    sees = (end >= 6).to(device)
+    assert torch.equal(got[0, ~sees, 0], want[0, ~sees, 0])
+    assert torch.isnan(got[0, sees, 0].float()).all()
+    assert torch.equal(got[0, :, 1], want[0, :, 1])
+
+
+def test_one_query_does_not_spoil_another(device, built_lib):
+    """NaN in a query: its own row alone."""
+    for dtype, dim in ((torch.bfloat16, 128), (torch.float32, 64)):
+        lens, rows, heads, lq = [40, 9], 16, 2, 40
+        count, tables, _ = _tables(lens, rows, 1)
+        pages = _rand((2, count, rows, heads, dim), dtype, 2).to(device)
+        q, k, v = (_rand((2, lq, heads, dim), dtype, s).to(device) for s in (3, 4, 5))
+        args = dict(pages=pages, block_table=_i32(tables, device), cache_lens=_i32(lens, device))
+        want = ops.paged_attention(q, k, v, **args)
+        q[1, 7, 1, 5] = math.nan
+        got = ops.paged_attention(q, k, v, **args)
+        assert torch.isnan(got[1, 7, 1].float()).all()
+        got[1, 7, 1] = want[1, 7, 1]
+        assert torch.equal(got, want)
+
+
 # ---------------------------------------------------------------------------
 # Shared prefix
 # ---------------------------------------------------------------------------
