@@ -46,6 +46,7 @@
 #include "attn_tile.h"
 
 #include <float.h>
+#include <limits.h>
 
 #include <type_traits>
 
@@ -105,9 +106,11 @@ template <typename T, int D, int RW> struct Shape {
   static constexpr int vec = 1040;
   static constexpr int area = DP / 8 * vec + 256;
   static constexpr int body = KW * stream > RW * KW * area ? KW * stream : RW * KW * area;
-  // Behind them: which 16-row groups of each stage's tile have no page.
+  // Behind them: which 16-row groups of each stage's tile have no page, and
+  // whether a wave's sums hold what is no number.
   static constexpr int flags = body;
-  static constexpr int lds = body + kWaves * 2 * 16;
+  static constexpr int votes = flags + kWaves * 2 * 16;
+  static constexpr int lds = votes + 16;
   static_assert(lds * per_cu <= 160 * 1024, "the LDS of a CU");
 };
 
@@ -410,11 +413,14 @@ struct Tile {
   }
 
   // An infinity or NaN in V that some rows do not see. Their weight for it is 0, and
-  // 0 times that is NaN in the product, so a tile that some rows do not see to its
-  // end is looked through (poisoned); if there is any, the rows that see it take it
-  // key by key on the vector units (take_poison), it is cleared in LDS (clear_poison),
-  // and the product goes on without it. Slow, rolled and in place: rare tiles, and
-  // another product beside pv() would cost the loop its registers.
+  // 0 times that is NaN in the product. Sums with such a value in them (wild_sums) of an
+  // item whose rows do not all see the same keys send its workgroup through the item once
+  // more, carefully: it looks through the tiles that some rows do not see to their end
+  // (poisoned), the rows that see what is no number take it key by key on the vector
+  // units (take_poison), it is cleared in LDS (clear_poison), and the product goes on
+  // without it. Slow, rolled and in place: rare, and another product beside pv() would
+  // cost the loop its registers. Looking through those tiles always cost 5 us of 76 (2 x
+  // 1,500 causal queries over 400 to 1,000 cached rows, 16 heads).
   static __device__ __forceinline__ bool poisoned(uint32_t v0, int lane) {
     // Any order does; not unrolled further, to keep its registers few.
     typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
@@ -437,6 +443,14 @@ struct Tile {
   }
   static __device__ __forceinline__ bool wild(float x) {
     return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u;
+  }
+  __device__ __forceinline__ bool wild_sums() const {
+    uint32_t top = 0;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = max(top, __float_as_uint(acc[d][r]) & 0x7f800000u);
+    return top == 0x7f800000u;
   }
   // seen[x]: rows of 32-key block x below it are seen (the same in both lanes of a row).
   __device__ __forceinline__ void take_poison(uint32_t v0, const f32x16 (&s)[NS], const int (&seen)[NS],
@@ -720,7 +734,6 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
     // tile and end with the first new one: its halves are found one by one.
     auto tile_at = [&](int i) __attribute__((always_inline)) { return t0 + (KW * i + stream) * UT; };
     Ti ti;
-    ti.reset();
     // Mask of tile i: rows of it that are seen, less 4 g, per 32-key block; all
     // of it where `masked` comes back false.
     auto limits = [&](int t, bool& masked) __attribute__((always_inline)) {
@@ -729,6 +742,11 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
       masked = t >= t1 || (cached ? j0 + kPN > keys.len : j0 + kPN > full_end);
       return t >= t1 ? -64 : (cached ? keys.len : my_end) - j0 - 4 * g;
     };
+    // Carefully the second time, if there is one: some sum is no number, and may come
+    // from a key that its row does not see.
+    const bool partly = !PREFIX && full_end < keys.fresh;
+    for (bool careful = false;; careful = true) {
+    ti.reset();
     if constexpr (RW == 1) {
       // Streams of one wave: no barriers, each wave waits for its own pieces.
       constexpr int HP = 16 / RPP;  // pieces of a 16-row group
@@ -753,7 +771,7 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
         find(tile_at(0));
         send_v();
       }
-      load_queries();
+      if (!careful) load_queries();
       for (int i = 0; i < nt; ++i) {
         const bool more = i + 1 < nt;
         const uint32_t bad = gone;
@@ -767,7 +785,7 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
         ti.softmax(s, masked, lim, bad, c);
         if (more) wait_vmcnt<2 * HP>();  // V of tile i (the next K was sent last)
         else wait_vmcnt<0>();
-        if (!PREFIX && masked && tile_at(i) >= keys.n_ct && Ti::poisoned(base + Sh::tile, lane)) {
+        if (!PREFIX && careful && masked && tile_at(i) >= keys.n_ct && Ti::poisoned(base + Sh::tile, lane)) {
           ti.take_poison(base + Sh::tile, s, {lim + 4 * g}, lane);
           Ti::clear_poison(base + Sh::tile, 0, Sh::tile, lane);
           asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -785,8 +803,10 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
         const int st = i & 1;
         const int tr = wave * WR;                 // this wave's first row of the tile
         const int t = tile_at(i) + tr / kPN;      // 32-key tile it lies in
-        const bool cached = t < keys.n_ct;
-        const int r0 = (cached ? t : t - keys.n_ct) * kPN + tr % kPN / 16 * 16;
+        // Past t1: rows that do not exist (seen rows of the next part may hold
+        // infinities, which have no weight of 0 here).
+        const bool cached = t < min(keys.n_ct, t1);
+        const int r0 = t < t1 ? (cached ? t : t - keys.n_ct) * kPN + tr % kPN / 16 * 16 : INT_MAX;
         uint64_t k, v;
         int rows;
         const bool gone = keys.find(cached, r0, k, v, rows);
@@ -798,7 +818,7 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
         send_rows<RB, F32, false>(v, rows, sv, to + Sh::tile, tr % 16, tr, WR / RPP, lane);
       };
       if (nt > 0) send_tile(0);
-      load_queries();
+      if (!careful) load_queries();
       for (int i = 0; i < iters; ++i) {
         // This wave's pieces of tile i have landed; past the barrier the tile
         // is whole, and reads of the stage that is sent to next have returned.
@@ -814,9 +834,10 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
         int lim = limits(t, masked), lim1 = 0;
         if (UT == 2) lim1 = limits(t + 1, masked1);
         const uint32_t v0 = base + st + Sh::tile;
-        // Some row does not see all of the tile's new keys: the whole workgroup
-        // looks through its V.
-        const bool poison = !PREFIX && (masked || masked1) && t + UT > keys.n_ct && Ti::poisoned(v0, lane);
+        // Some row does not see all of the tile's new keys: the whole workgroup looks
+        // through its V.
+        const bool poison =
+            !PREFIX && careful && (masked || masked1) && t + UT > keys.n_ct && Ti::poisoned(v0, lane);
         auto clear = [&]() __attribute__((always_inline)) {
           // Every wave has looked and taken its rows' share, then each clears its
           // part, then all go on.
@@ -865,6 +886,13 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
         }
         ti.pv(va + st, s);
       }
+    }
+    if (!partly || careful) break;
+    const uint32_t vote = __any(ti.wild_sums()) ? 1u : 0u;
+    if (lane == 0) reinterpret_cast<uint32_t*>(smem + Sh::votes)[wid] = vote;
+    __syncthreads();
+    const u32x4 all = *reinterpret_cast<const u32x4*>(smem + Sh::votes);
+    if (__builtin_amdgcn_readfirstlane(int(all[0] | all[1] | all[2] | all[3])) == 0) break;
     }
 
     if (!behind) {

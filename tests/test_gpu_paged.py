@@ -357,6 +357,31 @@ def test_nothing_unseen_is_taken(device, built_lib, dtype, dim, lq, prefix_len, 
     assert torch.equal(got[0, :, 1], want[0, :, 1])
 
 
+@pytest.mark.parametrize("dtype,dim", TYPES, ids=IDS)
+@pytest.mark.parametrize("lq,lens,prefix_len", [(3, [2080], 0), (130, [2080], 0), (70, [2000], 0),
+                                                (50, [16, 21, 40], 2080), (2, [16, 21, 40], 2080)])
+def test_infinities_that_every_query_sees(device, built_lib, dtype, dim, lq, lens, prefix_len):
+    """Key j of the long run of keys has an infinite value in column j % dim, and all keys
+    weigh the same: every result is that infinity, wherever the work is split."""
+    heads, rows = 2, 16
+    count, tables, prefix = _tables(lens, rows, 1, prefix_rows=prefix_len)
+    pages = _rand((2, count, rows, heads, dim), dtype, 2)
+    pages[0] = 0
+    n = prefix_len or lens[0]
+    j = torch.arange(n)
+    held = torch.tensor(prefix or tables[0])
+    pages[1, held[j // rows], j % rows, :, j % dim] = math.inf
+    q, k, v = (_rand((len(lens), lq, heads, dim), dtype, s).to(device) for s in (3, 4, 5))
+    k.zero_()
+    args = dict(pages=pages.to(device), block_table=_i32(tables, device), cache_lens=_i32(lens, device))
+    if prefix_len:
+        got = ops.shared_prefix_attention(q, k, v, prefix_table=_i32(prefix, device),
+                                          prefix_len=_i32([prefix_len], device), **args)
+    else:
+        got = ops.paged_attention(q, k, v, causal=True, **args)
+    assert bool((got == math.inf).all())
+
+
 def test_one_query_does_not_spoil_another(device, built_lib):
     """NaN in a query: its own row alone."""
     for dtype, dim in ((torch.bfloat16, 128), (torch.float32, 64)):
