@@ -1117,20 +1117,37 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
     m = mm;
     return ref;
   };
-  // This wave's parts, four at a time: their loads do not wait for one another.
-  auto join = [&](const Line& line, int parts, auto row_of) __attribute__((always_inline)) {
+  if (valid) {
+    // The row's parts of the prefix, then those of its own keys.
+    int pre_parts = 0;
+    int64_t pre_row = 0;
+    if constexpr (RWP > 0) {
+      const uint32_t pr = uint32_t(b) * uint32_t(a.R) + uint32_t(row);
+      const uint32_t pre_rt = uint32_t(a.B * a.R + 32 * RWP - 1) / (32 * RWP);
+      const Record p = a.pre.rec[uint32_t(hk) * pre_rt + pr / (32 * RWP)];
+      pre_parts = p.parts;
+      pre_row = int64_t(p.slot) * (32 * RWP) + pr % (32 * RWP);
+    }
+    // Of a cut line without a prefix, a broken item's first part is its
+    // workgroup's odd slot, the others are the next workgroups' even ones.
+    const bool broken = RWP == 0 && a.own.splits == 0;
+    const int64_t own_row = int64_t(rec.slot) * (32 * RWO) + in_item;
+    const int parts = pre_parts + rec.parts;
+    // This wave's parts, four at a time: their loads do not wait for one another.
     for (int p0 = wave; p0 < parts; p0 += 16) {
       f32x2 ml[4];
       f32x4 v[4][2];
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        const int p = p0 + 4 * x;
+        const int p = p0 + 4 * x, q = p - pre_parts;
         ml[x] = f32x2{-INFINITY, 0.f};
         v[x][0] = v[x][1] = f32x4{0.f, 0.f, 0.f, 0.f};
         if (p < parts) {
-          const int64_t at = row_of(p);
-          ml[x] = *reinterpret_cast<const f32x2*>(line.ml + at * 2);
-          const f32x4* const from = reinterpret_cast<const f32x4*>(line.o + at * D + 8 * ch);
+          const bool pre = RWP > 0 && q < 0;
+          const int64_t at = pre ? pre_row + int64_t(p) * (32 * RWP)
+                                 : own_row + int64_t(broken ? (q ? 2 * q - 1 : 0) : q) * (32 * RWO);
+          ml[x] = *reinterpret_cast<const f32x2*>((pre ? a.pre.ml : a.own.ml) + at * 2);
+          const f32x4* const from = reinterpret_cast<const f32x4*>((pre ? a.pre.o : a.own.o) + at * D + 8 * ch);
           v[x][0] = from[0];
           v[x][1] = from[1];
         }
@@ -1142,22 +1159,6 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
 #pragma unroll
       for (int x = 0; x < 4; ++x) add(ml[x], v[x], ref);
     }
-  };
-  if (valid) {
-    if constexpr (RWP > 0) {
-      const uint32_t pr = uint32_t(b) * uint32_t(a.R) + uint32_t(row);
-      const uint32_t pre_rt = uint32_t(a.B * a.R + 32 * RWP - 1) / (32 * RWP);
-      const Record p = a.pre.rec[uint32_t(hk) * pre_rt + pr / (32 * RWP)];
-      const int64_t first = int64_t(p.slot) * (32 * RWP) + pr % (32 * RWP);
-      join(a.pre, p.parts, [&](int x) { return first + int64_t(x) * (32 * RWP); });
-    }
-    // Of a cut line without a prefix, a broken item's first part is its
-    // workgroup's odd slot, the others are the next workgroups' even ones.
-    const bool broken = RWP == 0 && a.own.splits == 0;
-    join(a.own, rec.parts, [&](int x) {
-      const int64_t slot = int64_t(rec.slot) + (broken ? (x ? 2 * x - 1 : 0) : x);
-      return slot * (32 * RWO) + in_item;
-    });
   }
   if (wave > 0) {
     stats[wave - 1][lane] = f32x2{m, l};
