@@ -122,7 +122,8 @@ int paged_entry(const char* what, const dx_paged_call* call, bool prefix) {
   DX_CHECK_ARG(c.Lk == c.Lq || (!c.causal && c.n_blocks == 0),
                "%s: k/v length %lld must equal q length %lld with block starts or causal", what,
                (long long)c.Lk, (long long)c.Lq);
-  DX_CHECK_ARG(std::isfinite(float(c.softmax_scale)), "%s: softmax scale must be finite", what);
+  const float scale_log2 = float(c.softmax_scale * 1.4426950408889634);
+  DX_CHECK_ARG(std::isfinite(scale_log2), "%s: softmax scale must be finite", what);
   if (c.B == 0 || c.Lq == 0) return DX_OK;
   const int64_t es = c.dtype == DX_F32 ? 4 : 2, per16 = 16 / es;
   auto al = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
@@ -178,7 +179,7 @@ int paged_entry(const char* what, const dx_paged_call* call, bool prefix) {
   a.B = int(c.B); a.H = int(c.H); a.Hkv = int(c.Hkv); a.group = int(group);
   a.Lq = int(c.Lq); a.Lk = int(c.Lk); a.causal = c.causal != 0;
   a.R = int(R);
-  a.scale_log2 = float(c.softmax_scale * 1.4426950408889634);
+  a.scale_log2 = scale_log2;
   a.own.splits = p.own_splits;
   a.own.by_item = p.own_recs == p.own_items;  // no records: nothing is left to join
   a.pre.by_item = p.pre_recs > 0;

@@ -17,7 +17,7 @@
 #include "dx_common.h"
 
 #include <algorithm>
-#include <new>
+#include <exception>
 #include <vector>
 
 namespace dx {
@@ -221,7 +221,7 @@ extern "C" int dx_kv_page_copy(const void* const* pools, int64_t n_pools, int64_
     for (const int64_t p : from)
       DX_CHECK_ARG(!std::binary_search(to.begin(), to.end(), p),
                    "kv_page_copy: page %lld is both read and written", (long long)p);
-  } catch (const std::bad_alloc&) {
+  } catch (const std::exception&) {  // bad_alloc, length_error
     set_error("kv_page_copy: out of host memory");
     return DX_EINVAL;
   }

@@ -100,6 +100,9 @@ class KVCache:
     def _host_state(self):
         return self.length
 
+    def _captured_form(self):
+        return None
+
     def _restore_host(self, state) -> None:
         self.length = state
 

@@ -106,15 +106,20 @@ class PagedKVCache:
                                f"{self.pages} free")
         return shared, need
 
+    def _outside_a_capture(self, what: str) -> None:
+        """What the host decides a replay would not repeat."""
+        if self.block_table.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"PagedKVCache.{what} belongs before a capture, not inside one")
+
     def reserve(self, n: int) -> None:
         """Pages for the next ``n`` rows of every sequence, none of them shared. Nothing
         changes when they are there already, or (``RuntimeError``) when there are too few."""
+        if n < 0:
+            raise ValueError(f"cannot reserve {n} rows")
         shared, need = self._missing(n)
         if need == 0:
             return
-        if self.block_table.is_cuda and torch.cuda.is_current_stream_capturing():
-            raise RuntimeError(f"PagedKVCache.reserve({n}): pages are reserved before a capture, "
-                               "not inside one")
+        self._outside_a_capture(f"reserve({n})")
         src, dst = [], []
         for b in shared:
             at = self.lengths[b] // self.page_rows
@@ -141,6 +146,12 @@ class PagedKVCache:
 
     def commit(self, n: int) -> None:
         """Move every sequence's end once every layer has appended its chunk."""
+        if n < 0:
+            raise ValueError(f"cannot commit {n} rows")
+        for table, length in zip(self.tables, self.lengths):
+            if length + n > len(table) * self.page_rows:
+                raise RuntimeError(f"commit of {n} rows behind {length}, but only "
+                                   f"{len(table) * self.page_rows} are reserved: append first")
         self._advance(n)
         self.cache_lens.add_(n)
 
@@ -149,6 +160,7 @@ class PagedKVCache:
         """Sequence ``dst`` becomes a copy of ``src``, on the same pages."""
         if src == dst:
             return
+        self._outside_a_capture("fork")
         table, length = list(self.tables[src]), self.lengths[src]
         table = table[:-(-length // self.page_rows)]  # reserved pages behind the end stay src's
         for page in table:
@@ -161,6 +173,7 @@ class PagedKVCache:
 
     def free(self, seq: int) -> None:
         """Give a sequence's pages back; it starts again from nothing (and the prefix)."""
+        self._outside_a_capture("free")
         for page in self.tables[seq]:
             self._drop(page)
         self.tables[seq], self.lengths[seq] = [], 0
@@ -170,6 +183,7 @@ class PagedKVCache:
     def hold_prefix(self, seq: int) -> None:
         """The history of ``seq`` (behind a prefix held already, whose last page has to be
         full) becomes the prefix of every sequence; the sequences' own rows are freed."""
+        self._outside_a_capture("hold_prefix")
         if self.prefix_rows % self.page_rows:
             raise RuntimeError(f"a prefix of {self.prefix_rows} rows ends inside a page: nothing "
                                "can follow it in the prefix")
@@ -198,6 +212,7 @@ class PagedKVCache:
     def compact(self) -> int:
         """Move the pages in use to the lowest numbers, in every layer; returns how many
         moved. What is in use and what is free never overlap, so one pass does it."""
+        self._outside_a_capture("compact")
         live = sorted(self._users)
         n = len(live)
         src = [p for p in live if p >= n]
@@ -215,6 +230,7 @@ class PagedKVCache:
         return len(src)
 
     def reset(self) -> None:
+        self._outside_a_capture("reset")
         self.tables = [[] for _ in range(self.batch)]
         self.lengths = [0] * self.batch
         self.prefix, self.prefix_rows = [], 0
@@ -249,6 +265,9 @@ class PagedKVCache:
 
     def _host_state(self):
         return list(self.lengths)
+
+    def _captured_form(self) -> bool:
+        return bool(self.prefix)  # which operator attend() calls
 
     def _restore_host(self, state) -> None:
         self.lengths = list(state)

@@ -33,6 +33,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+from array import array
 
 import torch
 
@@ -178,13 +179,14 @@ def kv_page_copy(pools, src, dst) -> None:
         ptrs.append(p.data_ptr())
     if n == 0:
         return
+    src, dst = array("q", src), array("q", dst)  # OverflowError, not a page modulo 2^64
     if _elsewhere(device):
         with _on(device):
             return kv_page_copy(pools, src, dst)
     ids = ctypes.c_int64 * n
     rc = _lib.load().dx_kv_page_copy(
         (ctypes.c_void_p * len(ptrs))(*ptrs), len(ptrs), *steps[:4], _lib.dtype_code(dtype),
-        *shape[1:], ids(*src), ids(*dst), n, _lib.stream_handle(device))
+        *shape[1:], ids.from_buffer(src), ids.from_buffer(dst), n, _lib.stream_handle(device))
     _lib.check(rc, "kv_page_copy")
 
 

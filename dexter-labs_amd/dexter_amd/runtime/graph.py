@@ -116,7 +116,8 @@ class CachedStepGraph:
     statuses as they found them; rows the warm-up wrote past the cursor are
     rewritten by the first replay. A paged cache's pages for the next rows are
     reserved before each replay, outside the graph, which reads the table that
-    changed in place; whether it has a prefix is fixed by the capture.
+    changed in place. Whether it holds a prefix is fixed by the capture: ``RuntimeError``
+    when that has changed.
     """
 
     def __init__(self, fn: Callable[..., object], sample_inputs: Sequence[torch.Tensor],
@@ -141,8 +142,12 @@ class CachedStepGraph:
         # but no kernel: restore the host side only.
         for c, (host, _, _) in zip(self.caches, saved):
             c._restore_host(host)
+        self._forms = [c._captured_form() for c in self.caches]
 
     def __call__(self, *args: torch.Tensor) -> tuple[torch.Tensor, ...]:
+        if [c._captured_form() for c in self.caches] != self._forms:
+            raise RuntimeError("a cache has taken or lost its prefix since the step was captured: "
+                               "capture it again")
         for c in self.caches:
             c._check_room(self.rows)
         out = self.runner(*args)

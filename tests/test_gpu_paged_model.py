@@ -182,6 +182,52 @@ def test_captured_step_reserves_between_replays(device, built_lib):
     assert kv.lengths == kv.cache_lens.tolist() and not kv.overflowed()
 
 
+def test_captured_step_refuses_another_prefix(device, built_lib):
+    """Which attention a step calls is captured with it: a prefix that comes or goes after
+    the capture is refused, with nothing moved."""
+    layers = _layers(device)
+    kv = PagedKVCache(LAYERS, 2, 30, 16, HEADS, DIM // HEADS, device, DT)
+    _step(layers, kv, _x(device, 2, 20, 0), 0)
+    cos, sin = (t.to(device) for t in rope_table(torch.arange(20, 25), DIM // HEADS))
+
+    def last(x):
+        outs = [m(x, cos, sin, kv, i, write=True) for i, m in enumerate(layers)]
+        kv.commit(5)
+        return tuple(outs)
+    x = _x(device, 2, 5, 1)
+    step = CachedStepGraph(last, (x,), [kv], 5)
+    step(x)
+    kv.hold_prefix(0)
+    with pytest.raises(RuntimeError, match="capture it again"):
+        step(x)
+    assert kv.lengths == [0, 0] and kv.prefix_rows == 25
+    again = CachedStepGraph(last, (x,), [kv], 5)
+    again(x)
+    kv.reset()
+    with pytest.raises(RuntimeError, match="capture it again"):
+        again(x)
+    step(x)
+    assert kv.lengths == kv.cache_lens.tolist() == [5, 5]
+
+
+@pytest.mark.parametrize("name,args", [("fork", (0, 1)), ("free", (0,)), ("hold_prefix", (0,)),
+                                       ("compact", ()), ("reset", ())])
+def test_page_keeping_inside_a_capture_is_refused(device, built_lib, name, args):
+    kv = PagedKVCache(1, 2, 8, 16, HEADS, DIM // HEADS, device, DT)
+    k = _x(device, 2, 3, 0).view(2, 3, HEADS, DIM // HEADS)
+    kv.append(0, k, k)
+    kv.commit(3)
+    tables = [list(t) for t in kv.tables]
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        with torch.cuda.graph(graph, stream=side):
+            k2 = k + 1  # noqa: F841 (something to capture)
+            with pytest.raises(RuntimeError, match="before a capture"):
+                getattr(kv, name)(*args)
+    assert kv.tables == tables and kv.lengths == [3, 3] and kv.free_pages == 6
+
+
 def test_reserve_inside_a_capture_is_refused(device, built_lib):
     kv = PagedKVCache(1, 1, 4, 16, HEADS, DIM // HEADS, device, DT)
     graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()

@@ -173,6 +173,21 @@ def test_page_rows_are_checked():
             PagedKVCache(1, 1, 4, rows, 1, 4, "cpu", torch.float32)
 
 
+def test_commit_takes_only_what_is_reserved():
+    kv = _cache()
+    with pytest.raises(RuntimeError, match="commit of 1 rows behind 0, but only 0"):
+        kv.commit(1)
+    kv.reserve(10)
+    with pytest.raises(RuntimeError, match="commit of 17 rows"):
+        kv.commit(17)
+    kv.commit(16)  # the page's rows are there
+    assert kv.lengths == [16, 16, 16]
+    for call in (kv.commit, kv.reserve):
+        with pytest.raises(ValueError, match="-1 rows"):
+            call(-1)
+    assert kv.lengths == kv.cache_lens.tolist() == [16, 16, 16]
+
+
 @pytest.mark.parametrize("seed", range(6))
 def test_any_order_of_operations(seed):
     """Random appends, forks, frees, prefixes and compactions against plain lists."""

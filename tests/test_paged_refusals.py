@@ -103,6 +103,7 @@ def test_attention_refusals(built_lib):
         assert "row stride" in bad(p_sr=1 << 25)
         assert "finite" in bad(scale=float("inf"))
         assert "finite" in bad(scale=float("nan"))
+        assert "finite" in bad(scale=3e38)  # times log2 e
     assert "null prefix table" in _message(lib, _attend(lib, True, p_table=None))
     assert "null prefix length" in _message(lib, _attend(lib, True, p_len=None))
     # A shared prefix always joins parts: its workspace has to be there.
@@ -217,6 +218,10 @@ def test_copy_argument_checks():
     pool = _tensors()["pages"]
     with pytest.raises(ValueError, match="2 source pages for 1"):
         paged.kv_page_copy([pool], [0, 1], [2])
+    with pytest.raises(OverflowError):
+        paged.kv_page_copy([pool], [2 ** 64 + 1], [2])
+    with pytest.raises(TypeError):
+        paged.kv_page_copy([pool], [1.0], [2])
     with pytest.raises(ValueError, match="needs a pool"):
         paged.kv_page_copy([], [0], [2])
     with pytest.raises(ValueError, match="must agree"):
