@@ -1055,8 +1055,12 @@ __global__ __launch_bounds__(kThreads, (Shape<T, D, RWO>::per_cu)) void paged_at
     if (a.pre.splits == 0) {
       n_pre = wanted(pre_total, kCostP, grid);
       if (a.own.splits == 0 && n_pre + n_own > grid) {
-        // Both are cut: in proportion to their length.
-        const float part = float(pre_total) / (float(pre_total) + float(own.total));
+        // Both are cut: in proportion to their work. A tile takes four row waves 1.5 times
+        // as long as single ones (64 and 128 decoded tokens over prompts of 4,001 and 2,000
+        // rows, 8 and 24 K/V heads: 28.4 and 68.4 us counted alike, 26.9 and 59.8 so, 27.0
+        // and 57.6 counted double, which a prompt of 12,000 rows pays with 36.6 for 32.4).
+        const float pre_work = (RWP > RWO ? 1.5f : 1.0f) * float(pre_total);
+        const float part = pre_work / (pre_work + float(own.total));
         n_pre = uint32_t(part * float(grid) + 0.5f);
         n_pre = min(max(n_pre, 1u), grid - 1);
         n_own = grid - n_pre;

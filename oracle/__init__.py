@@ -18,6 +18,9 @@ under ``python/dexter/`` of raikonenfnu/dexter-labs):
                  residual (``ops/reference/norm.py:16-25``), with the reference's
                  per-op rounding, plus the single-rounding forms the fused
                  kernels compute.
+* ``paged``      attention over a cache in pages and a shared prefix, from its
+                 definition in fp64 (no counterpart in the reference), and the
+                 error that an evaluation with fp32 sums may have.
 * ``brute``      fp64 brute force (numpy, explicit loops) of attention, the
                  prologue and the adaLN/gated-residual pair, written
                  independently of the torch restatements;
@@ -25,7 +28,8 @@ under ``python/dexter/`` of raikonenfnu/dexter-labs):
                  ``torch.nn.functional.scaled_dot_product_attention`` and
                  against closed forms.
 
-Pinning status: every function here is pinned (tests/test_oracle.py); none is
+Pinning status: every function here is pinned (tests/test_oracle.py,
+tests/test_paged_oracle.py); none is
 "parity unpinned". The reference ships no golden vectors for this path, so
 the pins are the fp64 brute force, a library routine and closed-form cases.
 """
