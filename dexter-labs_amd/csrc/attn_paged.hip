@@ -8,18 +8,43 @@
 namespace dx {
 namespace {
 
+// Rows of 32 to a wave, one or four waves of them. Four single-wave streams for up to
+// 32 rows: 30.4 and 32.3 us against 33.0 and 34.9 with one stream (4 x 16 and 4 x 32 queries
+// of 24 heads over 300 to 3,000 rows; 64 decoded tokens over 0 to 100 rows 19.4 against
+// 21.9; alike where memory bounds it, 32 tokens of 8 K/V heads over 300 to 3,000). For 40
+// and 64 rows, two items of one wave read the keys twice: 46.8 and 47.2 against 33.9 and 36.6.
 int row_waves(int64_t rows) { return rows <= 32 ? 1 : 4; }
 
+// Own keys of one row tile per sequence and head, 16-bit, no prefix: up to this many
+// 32-key tiles the items are not cut, and there is nothing to join. Cut or whole, us,
+// over 0 to so many tiles, bf16, D 128:
+//                               8            16           32           48           64
+//   4 tokens, 8 K/V heads    15.8/ 9.2    15.2/11.8    16.4/16.9    16.6/21.6    16.2/25.7
+//   64 tokens                22.8/14.3    30.5/24.8    40.7/35.6    54.1/47.6    64.0/61.0
+//   256 tokens               53.8/44.5    69.2/61.8     114/105      159/151      206/202
+//   4 x 83, 24 heads         21.6/15.6    24.6/22.2    25.7/33.3    27.2/42.9    30.3/55.8
+//   16 x 83                  34.1/22.0    39.6/30.4    50.1/44.2    58.1/57.4    70.2/73.3
+// Longer ragged ones leave workgroups idle (128 tokens over 300 to 3,000 rows: 169/179).
+// D 256 runs half as many workgroups, each twice as long: 16 x 83 74.9/64.8 at 16 tiles, but
+// 256 tokens 201/212 at 32, 16 x 83 160/175 at 64. In fp32 a tile takes four times as long:
+// 4 x 99 over 16 tiles 45.8/79.5.
+int64_t whole_tiles(int64_t items, int64_t D, int64_t slots) {
+  return D > 128 ? 16 : std::min<int64_t>(64, std::max<int64_t>(16, 64 * items / slots));
+}
+
 // Key ranges per item of a split line: `tiles` per item, rounds of `slots`
-// workgroups, each with the cost of some tiles for its start and end. The
-// smallest of the counts that are within 2% of the best.
+// workgroups, each with the cost of some tiles for its start and end, and the join. The
+// smallest of the counts that are within 2% of the best. 16 x 83 rows of 24 heads over
+// 8,217 shared ones: 3, 5 and 7 ranges take 220, 212 and 218 us (it says 5). 1, 2 and 3
+// ranges under a causal mask over 400 to 1,000 cached rows: 2 x 1,500 queries, 16 heads of
+// 8, 80, 92 and 92 us (it says 1), half of them 60, 50 and 49 (2).
 int range_count(int64_t items, int64_t tiles, int64_t slots) {
   auto cost = [&](int64_t s) {
     const int64_t rounds = (items * s + slots - 1) / slots;
     return double(rounds) * (double((tiles + s - 1) / s) + 8) + (s > 1 ? 8 : 0);
   };
   double best = cost(1);
-  const int64_t most = std::min<int64_t>(16, std::max<int64_t>(1, tiles / 8));
+  const int64_t most = std::min<int64_t>(64, std::max<int64_t>(1, tiles / 8));
   for (int64_t s = 2; s <= most; ++s) best = std::min(best, cost(s));
   int s = 1;
   while (cost(s) > 1.02 * best) ++s;
@@ -27,7 +52,7 @@ int range_count(int64_t items, int64_t tiles, int64_t slots) {
 }
 
 PagedPlan plan_paged(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hkv, int64_t D,
-                     int64_t own_rows, int64_t pre_rows, bool prefix, int cus) {
+                     int64_t dtype, int64_t own_rows, int64_t pre_rows, bool prefix, int cus) {
   PagedPlan p{};
   const int64_t R = Lq * (H / Hkv);
   auto row_tiles = [](int64_t rows, int rw) { return (rows + 32 * rw - 1) / (32 * rw); };
@@ -46,7 +71,12 @@ PagedPlan plan_paged(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hkv, 
   // Workgroups that run at once.
   const int64_t slots = (D == 256 ? 1 : 2) * int64_t(cus);
   if (prefix && row_tiles(B * R, p.rw_pre) > 1) p.pre_splits = range_count(p.pre_items, pre_tiles, slots);
-  if (row_tiles(R, p.rw_own) > 1) p.own_splits = range_count(p.own_items, own_tiles, slots);
+  const bool halves = dtype != DX_F32;
+  if (row_tiles(R, p.rw_own) > 1 || (B == 1 && halves && !prefix))
+    p.own_splits = range_count(p.own_items, own_tiles, slots);
+  else if (halves && !prefix && own_tiles <= whole_tiles(p.own_items, D, slots) &&
+           grid_fits(p.own_items, kPagedThreads))
+    p.own_splits = 1;
   // A cut line: no more of them than it has tiles and items.
   p.own_n = p.own_splits ? p.own_items * p.own_splits : std::min(slots, p.own_items * (own_tiles + 1));
   const int64_t pre_n = p.pre_splits ? p.pre_items * p.pre_splits
@@ -143,7 +173,7 @@ int paged_entry(const char* what, const dx_paged_call* call, bool prefix) {
     DX_CHECK_ARG(s >= 0 && s * es < (int64_t(1) << 26), "%s: row stride %lld out of range", what,
                  (long long)s);
 
-  const PagedPlan p = plan_paged(c.B, c.Lq, c.Lk, c.H, c.Hkv, c.D, c.width * c.page_rows,
+  const PagedPlan p = plan_paged(c.B, c.Lq, c.Lk, c.H, c.Hkv, c.D, c.dtype, c.width * c.page_rows,
                                  c.prefix_width * c.page_rows, prefix, device_cus());
   const int64_t need = plan_bytes(p, c.D);
   if (need > c.workspace_bytes || (need > 0 && !c.workspace)) {
@@ -222,7 +252,7 @@ extern "C" int64_t dx_paged_attention_workspace_bytes(int dtype, int64_t B, int6
                               prefix_width);
   if (bad) return -bad;
   if (B == 0 || Lq == 0) return 0;
-  const PagedPlan p = plan_paged(B, Lq, Lk, H, Hkv, D, width * page_rows,
+  const PagedPlan p = plan_paged(B, Lq, Lk, H, Hkv, D, dtype, width * page_rows,
                                  prefix_width * page_rows, has_prefix != 0, device_cus());
   return plan_bytes(p, D);
 }

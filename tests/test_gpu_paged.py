@@ -72,13 +72,15 @@ def _check(got, want, dtype, dim, keys, vmax, what):
 
 def _case(device, dtype, dim, *, lens, lq, heads=2, kv=2, rows=16, prefix_len=0, lk=None, bb=None,
           causal=False, scale=None, seed=0, tables=None, prefix=None, poison=True, what="",
-          device_lens=None, strided=False, own=True):
+          device_lens=None, strided=False, own=True, wide=False):
     """One attention call against the oracle."""
     b = len(lens)
     lk = lq if lk is None else lk
     count, t0, p0 = _tables(lens, rows, seed, prefix_rows=prefix_len)
     tables = t0 if tables is None else tables
     prefix = p0 if prefix is None else prefix
+    if wide:  # room for 66 more 32-key tiles: the launch is planned for long sequences
+        tables = [t + [-1] * (-(-66 * 32 // rows)) for t in tables]
     q = _rand((b, lq, heads, dim), dtype, seed + 1)
     k = _rand((b, lk, kv, dim), dtype, seed + 2)
     v = _rand((b, lk, kv, dim), dtype, seed + 3)
@@ -233,6 +235,29 @@ def test_rows_per_kv_head(device, built_lib, dtype, dim, lq, heads, kv):
           what=f"lq {lq} {heads}/{kv} D{dim} {dtype}")
 
 
+@pytest.mark.parametrize("dtype,dim", TYPES, ids=IDS)
+@pytest.mark.parametrize("mask", list(MASKS))
+@pytest.mark.parametrize("lq", [9, 45])
+def test_short_rows_in_wide_tables(device, built_lib, dtype, dim, mask, lq):
+    """What is planned for long sequences holds short ones: pieces of several items, items of
+    several pieces, and more workgroups than there is work."""
+    kw = dict(MASKS[mask])
+    if "bb" in kw:
+        kw["bb"] = [min(x, lq) for x in kw["bb"]]
+    _case(device, dtype, dim, lens=[0, 1, 77, 160, 700], lq=lq, wide=True,
+          what=f"wide {mask} {lq} D{dim} {dtype}", **kw)
+
+
+@pytest.mark.parametrize("dtype,dim", TYPES, ids=IDS)
+@pytest.mark.parametrize("lq,heads,kv,n,wide", [
+    (1, 8, 2, 3000, False), (20, 2, 2, 2049, False), (83, 3, 3, 5000, False), (1, 2, 1, 40, True),
+    (83, 1, 1, 0, True), (40, 2, 1, 33, True)])
+def test_one_sequence_in_ranges(device, built_lib, dtype, dim, lq, heads, kv, n, wide):
+    """A single sequence's keys are split evenly: more ranges than tiles, or many of each."""
+    _case(device, dtype, dim, lens=[n], lq=lq, heads=heads, kv=kv, causal=lq == 83, wide=wide,
+          what=f"one sequence {n} + {lq} D{dim} {dtype}")
+
+
 @pytest.mark.parametrize("rows", [16, 32, 48, 80, 112, 256, 1024])
 def test_page_sizes(device, built_lib, rows):
     """Pages that end inside a tile, are whole tiles, or hold several."""
@@ -314,12 +339,13 @@ def test_all_pages_dropped(device, built_lib):
 @pytest.mark.parametrize("dtype,dim", TYPES, ids=IDS)
 @pytest.mark.parametrize("lq,prefix_len", [(9, 0), (45, 0), (200, 0), (45, 70)])
 @pytest.mark.parametrize("mask", ["causal", "blocks"])
-def test_nothing_unseen_is_taken(device, built_lib, dtype, dim, lq, prefix_len, mask):
+@pytest.mark.parametrize("width", [None, 160])
+def test_nothing_unseen_is_taken(device, built_lib, dtype, dim, lq, prefix_len, mask, width):
     """Infinities and NaN in keys and values that a query does not see, in the same tile as
     some that it does: its result is bit for bit what it was. Queries that see them get a
     result that is not finite in the columns that are not, and the others' bits elsewhere."""
     b, heads, rows, lens = 2, 2, 16, [21, 40]
-    count, tables, prefix = _tables(lens, rows, 1, prefix_rows=prefix_len)
+    count, tables, prefix = _tables(lens, rows, 1, prefix_rows=prefix_len, width=width)
     pages = _rand((2, count, rows, heads, dim), dtype, 2).to(device)
     q, k, v = (_rand((b, lq, heads, dim), dtype, s).to(device) for s in (3, 4, 5))
     args = dict(pages=pages, block_table=_i32(tables, device), cache_lens=_i32(lens, device))
