@@ -19,7 +19,8 @@
 //
 // Work. The unit is a 32-key tile of a work item (32 RW rows of one K/V head, of
 // one sequence or, for the prefix, of the whole batch). There are two lines of
-// items, the own keys' and the prefix's, in one launch, and two ways to deal one:
+// items, the own keys' and the prefix's, in one launch, and two ways to deal one
+// (attn_paged.hip chooses):
 //  * Cut (items that share no keys: one row tile per sequence and head). All
 //    tiles of all items form one line, which is cut into equal pieces, one per
 //    workgroup, whatever the lengths are: the device cuts it, by the lengths as
@@ -27,9 +28,9 @@
 //    at most two broken ones, whose partials paged_merge_kernel joins.
 //  * Split (several row tiles read the same keys): every item in S equal ranges
 //    of keys, a workgroup each, those of one head next to each other on one XCD,
-//    so that they read a key tile at about the same time, through one L2. Cut
-//    instead, 16 x 83 queries over a shared 8,217-row prefix (24 heads) took 597
-//    us, every workgroup at a place of its own in the keys.
+//    so that they read a key tile at about the same time, through one L2. 16 x 83
+//    queries over a shared 8,217-row prefix (24 heads) take 202 us so, and 242 cut
+//    (every workgroup at a place of its own in the keys).
 // With a prefix every row has parts of both lines, and the merge joins them all.
 //
 // Kernel. A wave owns 32 rows (S^T = K Q^T on 32 x 32 MFMAs, the formulation of
@@ -40,6 +41,18 @@
 // rows, so 16 rows lie in one page, the page's 64-bit address is scalar
 // arithmetic, and rows past the end (or of a table entry that names no page)
 // come back as zeros from the descriptor's bound.
+//
+// What it takes (bf16, D 128; kernel alone, the join 4-7 us more, 20 where said):
+//   32 tokens, 8 K/V heads, 300 to 3,000 cached rows each   48 us, 4.4 TB/s
+//   83 queries, 24 heads, 32,768 cached rows                 84 us, 4.8 TB/s
+//   64 tokens, 8 K/V heads, 1 to 500 rows, prefix of 4,001   27 us, 3.1 TB/s
+//   16 x 83, 24 heads, 0 to 332 rows, prefix of 8,217        202 us, 680 TFLOP/s (join 20)
+//   2 x 1,500 causal, 8 K/V heads, 400 to 1,000 rows         78 us, 420 TFLOP/s
+//   4 x 99 in fp32, 24 heads, 0 to 1,245 rows                64 us, 47 TFLOP/s
+// Many keys to a row tile: bound by memory. Otherwise by the chain of a tile (scores,
+// softmax, product) in the few waves that registers allow, and by the 4 to 8 us from
+// a workgroup's start to its first product: lengths, table, keys and queries, one
+// after the other.
 #pragma once
 
 #include "attn_paged.h"
@@ -53,7 +66,6 @@
 namespace dx {
 namespace {
 
-constexpr int kPN = 32;  // keys per tile of the line
 // The launch arguments where they lie. reread() hides where a pointer to them
 // comes from: what is read through its result is read there, and not kept in
 // scalar registers from the kernel's start on (they hold a third of what the
@@ -92,7 +104,7 @@ template <typename T, int D, int RW> struct Shape {
   // two stages of 64 keys (each wave then fetches 16 rows, which one page
   // holds), or of 32 where registers and LDS hold no more.
   // Head dim 256 (queries and sums of a wave alone take 192 registers) has a CU
-  // to itself: registers for one wave per SIMD, 32 of them spilled otherwise.
+  // to itself: registers for one wave per SIMD (two leave 256, which spill).
   static constexpr int per_cu = D == 256 ? 1 : 2;
   static constexpr int TK = RW == 1 || RB >= 512 ? 32 : 64;
   static constexpr int KW = RW == 1 ? (RB * per_cu >= 1024 ? 2 : 4) : kWaves / RW;
@@ -166,10 +178,14 @@ __device__ __forceinline__ int prefix_rows(Args& a) {
 }
 
 // Work on a line is counted in tiles; an item adds `kItemCost` to its tiles, for
-// its queries and its result (what a piece of so many tiles costs). A cut that
+// its queries and its result (what a piece of so many tiles costs: half, this and
+// twice it take 24.4, 22.0 and 22.8 us at 4 x 99 queries of 24 heads over 0 to 1,245
+// rows, 30.6, 30.4 and 32.2 with the join at 4 x 16 over 300 to 3,000). A cut that
 // falls among those is taken as one behind the item.
 template <typename T, int D, int RW>
 constexpr uint32_t kItemCost = Shape<T, D, RW>::KW * Shape<T, D, RW>::TK / kPN * 2;
+static_assert(kItemCost<float, 64, 1> <= kMaxItemCost && kItemCost<uint16_t, 64, 1> <= kMaxItemCost,
+              "the host's bound of a line's length");
 
 // A line of `total` cut into n pieces, the first `longer` of them q + 1 long.
 struct Cut {
@@ -1085,6 +1101,8 @@ __global__ __launch_bounds__(kThreads, (Shape<T, D, RWO>::per_cu)) void paged_at
 // Join the parts of 8 rows of an item, 64 of their values (blockIdx.z): a lane
 // holds 8 values of a row, and the four waves take every fourth part each, so
 // that a long list of parts is no long chain of loads; their sums meet in LDS.
+// Bound by memory: 20.4 us for the 106 MB of 16 x 83 rows of 24 heads in six parts, 5.2
+// TB/s; by its latency, 4-5 us, for decoded tokens.
 // blockIdx.x is a record. Prefix items are over all sequences' rows, so the rows
 // here may be those of two. A part that saw nothing has l = 0.
 template <typename T, int D, int RWP, int RWO>
