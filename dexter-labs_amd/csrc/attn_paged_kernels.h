@@ -759,8 +759,10 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
       return t >= t1 ? -64 : (cached ? keys.len : my_end) - j0 - 4 * g;
     };
     // Carefully the second time, if there is one: some sum is no number, and may come
-    // from a key that its row does not see.
-    const bool partly = !PREFIX && full_end < keys.fresh;
+    // from a key that its row does not see. A share behind the item's tiles sums nothing and
+    // casts no vote: what keeps the next item's votes behind this one's reads is the
+    // barriers of the results' way out, which such a share does not take.
+    const bool partly = !PREFIX && !behind && full_end < keys.fresh;
     for (bool careful = false;; careful = true) {
     ti.reset();
     if constexpr (RW == 1) {
