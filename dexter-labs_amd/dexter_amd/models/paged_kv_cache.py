@@ -76,10 +76,10 @@ class PagedKVCache:
             del self._users[page]
             heapq.heappush(self._free, page)
 
-    def _push_tables(self) -> None:
-        """The host's tables to the device, in place. A list that was never this long keeps
-        -1 (no page) behind its end."""
-        rows = [t + [-1] * (self.width - len(t)) for t in self.tables]
+    def _push_tables(self, tables: list[list[int]] | None = None) -> None:
+        """The host's tables (or these) to the device, in place. A list that was never this
+        long keeps -1 (no page) behind its end."""
+        rows = [t + [-1] * (self.width - len(t)) for t in tables or self.tables]
         self.block_table.copy_(torch.tensor(rows, dtype=torch.int32).view(self.batch, self.width))
 
     def _push_lengths(self) -> None:
@@ -120,20 +120,26 @@ class PagedKVCache:
         if need == 0:
             return
         self._outside_a_capture(f"reserve({n})")
+        # Pages change hands once everything that can fail has been done.
+        new = iter(heapq.nsmallest(need, self._free))
+        tables = [list(t) for t in self.tables]
         src, dst = [], []
         for b in shared:
             at = self.lengths[b] // self.page_rows
-            old, new = self.tables[b][at], self._take()
-            src.append(old)
-            dst.append(new)
-            self._drop(old)
-            self.tables[b][at] = new
-        for table, length in zip(self.tables, self.lengths):
+            src.append(tables[b][at])
+            tables[b][at] = next(new)
+            dst.append(tables[b][at])
+        for table, length in zip(tables, self.lengths):
             while len(table) * self.page_rows < length + n:
-                table.append(self._take())
+                table.append(next(new))
         if src:
             ops.kv_page_copy(self.pools, src, dst)
-        self._push_tables()
+        self._push_tables(tables)
+        for _ in range(need):
+            self._take()
+        for page in src:
+            self._drop(page)  # (no page's last user: the last of its sharers keeps it)
+        self.tables = tables
 
     _check_room = reserve
 
