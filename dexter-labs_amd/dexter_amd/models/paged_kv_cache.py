@@ -169,9 +169,10 @@ class PagedKVCache:
         self._outside_a_capture("fork")
         table, length = list(self.tables[src]), self.lengths[src]
         table = table[:-(-length // self.page_rows)]  # reserved pages behind the end stay src's
+        dropped = self.tables[dst]
         for page in table:
             self._users[page] += 1
-        for page in self.tables[dst]:
+        for page in dropped:
             self._drop(page)
         self.tables[dst], self.lengths[dst] = table, length
         self._push_tables()

@@ -37,3 +37,16 @@ def test_a_failed_copy_changes_nothing(monkeypatch):
     _step(kv, want, 3, 2000)
     _check(kv, want)
     assert len({t[1] for t in kv.tables}) == 3
+
+
+@pytest.mark.parametrize("name,args", [("fork", (0, 3)), ("fork", (3, 0)), ("fork", (0, -4)),
+                                       ("free", (3,)), ("hold_prefix", (3,))])
+def test_a_sequence_that_does_not_exist(name, args):
+    """IndexError with nothing changed: no page is counted for a sequence that is not there."""
+    kv, want = _cache(), [[], [], []]
+    _step(kv, want, 20, 0)
+    before = _state(kv)
+    with pytest.raises(IndexError):
+        getattr(kv, name)(*args)
+    assert _state(kv) == before
+    _check(kv, want)
