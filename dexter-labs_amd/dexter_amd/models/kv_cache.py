@@ -82,7 +82,7 @@ class KVCache:
 
     def commit(self, n: int) -> None:
         """Advance the write cursor once every layer has appended its block."""
-        self._advance(n)
+        self.length += n
         if self.cursor is not None:
             self.cursor.add_(n)
 
@@ -95,16 +95,3 @@ class KVCache:
     def overflowed(self) -> bool:
         """Whether a device-cursor append found no room (synchronises with the device)."""
         return bool(self.status is not None and int(self.status.item()) != 0)
-
-    # What runtime.CachedStepGraph keeps of a cache on the host.
-    def _host_state(self):
-        return self.length
-
-    def _captured_form(self):
-        return None
-
-    def _restore_host(self, state) -> None:
-        self.length = state
-
-    def _advance(self, n: int) -> None:
-        self.length += n

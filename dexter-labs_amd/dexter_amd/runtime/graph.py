@@ -105,6 +105,21 @@ def capture(fn: Callable[..., object], sample_inputs: Sequence[torch.Tensor],
     return _record(fn, tuple(t.clone() for t in sample_inputs), warmup)
 
 
+def _host_state(cache):
+    return cache._host_state() if isinstance(cache, PagedKVCache) else cache.length
+
+
+def _restore_host(cache, state) -> None:
+    if isinstance(cache, PagedKVCache):
+        cache._restore_host(state)
+    else:
+        cache.length = state
+
+
+def _captured_form(cache):
+    return cache._captured_form() if isinstance(cache, PagedKVCache) else None
+
+
 class CachedStepGraph:
     """A captured step that appends ``rows`` rows to device-cursor KV caches (or to paged
     ones, whose lengths are on the device always) and commits them.
@@ -128,11 +143,11 @@ class CachedStepGraph:
         self.rows = int(rows)
         for c in self.caches:
             c._check_room(self.rows)
-        saved = [(c._host_state(), c.cursor.clone(), c.status.clone()) for c in self.caches]
+        saved = [(_host_state(c), c.cursor.clone(), c.status.clone()) for c in self.caches]
 
         def restore():
             for c, (host, cursor, status) in zip(self.caches, saved):
-                c._restore_host(host)
+                _restore_host(c, host)
                 c.cursor.copy_(cursor)
                 c.status.copy_(status)
 
@@ -141,16 +156,19 @@ class CachedStepGraph:
         # Recording ran fn's host code once (its commits moved the host lengths)
         # but no kernel: restore the host side only.
         for c, (host, _, _) in zip(self.caches, saved):
-            c._restore_host(host)
-        self._forms = [c._captured_form() for c in self.caches]
+            _restore_host(c, host)
+        self._forms = [_captured_form(c) for c in self.caches]
 
     def __call__(self, *args: torch.Tensor) -> tuple[torch.Tensor, ...]:
-        if [c._captured_form() for c in self.caches] != self._forms:
+        if [_captured_form(c) for c in self.caches] != self._forms:
             raise RuntimeError("a cache has taken or lost its prefix since the step was captured: "
                                "capture it again")
         for c in self.caches:
             c._check_room(self.rows)
         out = self.runner(*args)
         for c in self.caches:
-            c._advance(self.rows)
+            if isinstance(c, PagedKVCache):
+                c._advance(self.rows)
+            else:
+                c.length += self.rows
         return out
