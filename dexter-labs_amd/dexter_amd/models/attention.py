@@ -19,6 +19,10 @@ append and attention in one call.
 With a ``PagedKVCache`` the same steps run over pages: the projections and the
 prologue as above, then ``PagedKVCache.append`` and ``PagedKVCache.attend``
 (``ops.paged_attention``, or ``ops.shared_prefix_attention`` when it holds a prefix).
+Its rows are always appended by a launch of their own (``fused_append`` says how a
+``KVCache`` is written, and changes nothing here). The sequences of a paged cache may
+stand at different positions: ``cos`` and ``sin`` are then ``[B, L, D/2]``, a table for
+each. Tables of ``[L, D/2]`` rotate every sequence by the same positions, whatever its length.
 """
 
 from __future__ import annotations
@@ -114,18 +118,29 @@ class SelfAttention(nn.Module):
 
     def _paged(self, x, cos, sin, kv_cache, layer, block_boundaries, write, fused_qkv):
         b, seq, dim = x.shape
+        own = cos.dim() != 2 or sin.dim() != 2  # a table per sequence
+        if own:
+            for t in (cos, sin):
+                if t.shape != (b, seq, self.head_dim // 2):
+                    raise ValueError(f"cos/sin must be [L, D/2], or [B, L, D/2] = "
+                                     f"[{b}, {seq}, {self.head_dim // 2}], got {tuple(t.shape)}")
         if write:
             kv_cache.reserve(seq)  # "KV cache full" before anything is written
+        if own:
+            # The prologue goes row by row: the batch as one long chunk.
+            x, cos, sin = x.reshape(1, b * seq, dim), cos.flatten(0, 1), sin.flatten(0, 1)
         if fused_qkv and b * seq <= 128 and dim % 512 == 0 and self.head_dim % 16 == 0:
             q, k, v = ops.qkv_norm_rope(
                 x, self.q.weight, self.q.bias, self.k.weight, self.k.bias, self.v.weight,
                 self.v.bias, self.q_norm, self.k_norm, cos, sin, self.heads, self.eps)
         else:
-            shape = (b, seq, self.heads, self.head_dim)
+            shape = (*x.shape[:2], self.heads, self.head_dim)
             q = F.linear(x, self.q.weight, self.q.bias).view(shape)
             k = F.linear(x, self.k.weight, self.k.bias).view(shape)
             v = F.linear(x, self.v.weight, self.v.bias).view(shape)
             q, k = ops.qk_norm_rope(q, k, self.q_norm, self.k_norm, cos, sin, self.eps)
+        if own:
+            q, k, v = (t.view(b, seq, self.heads, self.head_dim) for t in (q, k, v))
         if write:
             kv_cache.append(layer, k, v)
         return self._project_out(kv_cache.attend(layer, q, k, v, block_boundaries))
