@@ -68,7 +68,8 @@ PagedPlan plan_paged(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hkv, 
     pre_tiles = std::max<int64_t>(tiles(pre_rows), 1);
     p.pre_work = p.pre_items * (pre_tiles + kMaxItemCost);
   }
-  // Workgroups that run at once.
+  // Workgroups that run at once. Lines of more than one row tile per sequence and head are
+  // never cut (range_count is at least 1): the kernel's cut lines rely on it.
   const int64_t slots = (D == 256 ? 1 : 2) * int64_t(cus);
   if (prefix && row_tiles(B * R, p.rw_pre) > 1) p.pre_splits = range_count(p.pre_items, pre_tiles, slots);
   const bool halves = dtype != DX_F32;
@@ -187,6 +188,9 @@ int paged_entry(const char* what, const dx_paged_call* call, bool prefix) {
   // Lines are counted in 32 bits.
   DX_CHECK_ARG(p.own_work < (int64_t(1) << 31) && p.pre_work < (int64_t(1) << 31),
                "%s: too many queries and keys for one launch", what);
+  DX_CHECK_ARG((p.own_splits || p.own_items == c.B * c.Hkv) &&
+                   (!prefix || p.pre_splits || p.pre_items == c.Hkv),
+               "%s: a line of several row tiles was to be cut", what);
   DX_CHECK_ARG(grid_fits(p.own_recs, 256) && grid_fits(p.grid, kPagedThreads) && p.own_items < (int64_t(1) << 30) &&
                    p.pre_items < (int64_t(1) << 30),
                "%s: the call exceeds one launch", what);

@@ -21,11 +21,11 @@
 // one sequence or, for the prefix, of the whole batch). There are two lines of
 // items, the own keys' and the prefix's, in one launch, and two ways to deal one
 // (attn_paged.hip chooses):
-//  * Cut (items that share no keys: one row tile per sequence and head). All
-//    tiles of all items form one line, which is cut into equal pieces, one per
-//    workgroup, whatever the lengths are: the device cuts it, by the lengths as
-//    they are. A piece covers whole items, whose results it writes itself, and
-//    at most two broken ones, whose partials paged_merge_kernel joins.
+//  * Cut (items that share no keys: one row tile per sequence and head, or for
+//    the prefix per head). All tiles of all items form one line, which is cut into
+//    equal pieces, one per workgroup, whatever the lengths are: the device cuts it,
+//    by the lengths as they are. A piece covers whole items, whose results it writes
+//    itself, and at most two broken ones, whose partials paged_merge_kernel joins.
 //  * Split (several row tiles read the same keys): every item in S equal ranges
 //    of keys, a workgroup each, those of one head next to each other on one XCD,
 //    so that they read a key tile at about the same time, through one L2. 16 x 83
@@ -128,30 +128,6 @@ template <typename T, int D, int RW> struct Shape {
 
 __device__ __forceinline__ int tiles_of(int rows) { return (rows + kPN - 1) / kPN; }
 
-// Tiles of the new keys that row tile rt sees (at least 1, so that every item
-// has a tile and a workgroup), rt differing between lanes: end_bounds' hi.
-template <int RW>
-__device__ __forceinline__ int new_tiles(Args& a, int rt) {
-  const int q_last = (min((rt + 1) * (32 * RW), a.R) - 1) / a.group;
-  int hi;
-  if (a.causal) {
-    hi = q_last + 1;
-  } else if (a.n_blocks == 0) {
-    hi = a.Lk;
-  } else {
-    bool ascending = true;
-    int prev = 0;
-    hi = 0;
-    for_each_block(a, [&](int lo, int end) __attribute__((always_inline)) {
-      ascending = ascending && lo >= prev;
-      prev = lo;
-      if (q_last >= slice_at(lo, a.Lq) && q_last < slice_at(end, a.Lq)) hi = max(hi, min(end, a.Lq));
-    });
-    if (!ascending) hi = a.Lq;
-  }
-  return max(tiles_of(hi), 1);
-}
-
 __device__ __forceinline__ uint32_t scan(uint32_t x, int lane) {  // inclusive, over a wave
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
@@ -199,23 +175,14 @@ struct Cut {
   }
 };
 
-// The line of the own keys: items (sequence, K/V head, row tile), in this order.
-// The host holds its length below 2^31.
-template <int RW>
+// The line of the own keys: items (sequence, K/V head), in this order, all rows of one in
+// one row tile (attn_paged.hip cuts no other line). The host holds its length below 2^31.
 struct OwnLine {
-  uint32_t n_rt;
-  uint32_t fresh;  // new-key tiles and costs of a (sequence, head): of all its row tiles
+  uint32_t fresh;  // an item's tiles of new keys that some row sees (at least 1, so that it has a
+                   // tile and a workgroup), and its cost
   uint32_t total;
   __device__ __forceinline__ void init(Args& a, int lane, uint32_t cost) {
-    n_rt = uniform(uint32_t(a.R + 32 * RW - 1) / (32 * RW));
-    uint32_t tiles = 0;
-    if (a.causal || a.n_blocks) {
-      for (uint32_t r0 = 0; r0 < n_rt; r0 += 64)
-        tiles += lane_of(scan(r0 + lane < n_rt ? new_tiles<RW>(a, int(r0) + lane) : 0, lane), 63);
-    } else {
-      tiles = n_rt * uint32_t(max(tiles_of(a.Lk), 1));
-    }
-    fresh = uniform(tiles + n_rt * cost);
+    fresh = uniform(uint32_t(max(tiles_of(end_bounds(a, 0, a.Lq - 1).hi), 1)) + cost);
     uint32_t cached = 0;
     if (a.B == 1) {
       cached = uint32_t(tiles_of(own_rows(a, 0)));
@@ -223,11 +190,10 @@ struct OwnLine {
       for (int b0 = 0; b0 < a.B; b0 += 64)
         cached += lane_of(scan(b0 + lane < a.B ? tiles_of(own_rows(a, b0 + lane)) : 0, lane), 63);
     }
-    total = uniform(uint32_t(a.Hkv) * (n_rt * cached + uint32_t(a.B) * fresh));
+    total = uniform(uint32_t(a.Hkv) * (cached + uint32_t(a.B) * fresh));
   }
   // The item that holds position `at` of the line, and the place in it.
-  __device__ __forceinline__ void locate(Args& a, int lane, uint32_t cost, uint32_t at, int& b, int& hk,
-                                         int& rt, int& t) const {
+  __device__ __forceinline__ void locate(Args& a, int lane, uint32_t at, int& b, int& hk, int& t) const {
     b = 0;
     uint32_t before = 0;  // what the sequences before b have, per head
     if (a.B > 1) {
@@ -237,44 +203,22 @@ struct OwnLine {
         const uint32_t own = b0 + lane < a.B ? tiles_of(own_rows(a, b0 + lane)) : 0;
         const uint32_t upto = cached + scan(own, lane);
         // Up to and with this lane's sequence.
-        const uint32_t end = n_rt * upto + uint32_t(b0 + lane + 1) * fresh;
+        const uint32_t end = upto + uint32_t(b0 + lane + 1) * fresh;
         const uint64_t hit = __ballot(b0 + lane < a.B && end > want);
         if (hit) {
           const int j = __builtin_ctzll(hit);
           b = b0 + j;
-          before = lane_of(end, j) - n_rt * lane_of(own, j) - fresh;
+          before = lane_of(end, j) - lane_of(own, j) - fresh;
           break;
         }
         cached = lane_of(upto, 63);
       }
     }
     b = __builtin_amdgcn_readfirstlane(b);
-    const uint32_t n_ct = uniform(uint32_t(tiles_of(own_rows(a, b))));
     const uint32_t in_seq = at - before * uint32_t(a.Hkv);
-    const uint32_t per_head = n_rt * n_ct + fresh;
+    const uint32_t per_head = uniform(uint32_t(tiles_of(own_rows(a, b)))) + fresh;
     hk = int(in_seq / per_head);
-    uint32_t r = in_seq - uint32_t(hk) * per_head;
-    rt = 0;
-    if (a.causal || a.n_blocks) {
-      uint32_t base = 0;
-      for (uint32_t r0 = 0; r0 < n_rt; r0 += 64) {
-        const uint32_t w = r0 + lane < n_rt ? n_ct + new_tiles<RW>(a, int(r0) + lane) + cost : 0;
-        const uint32_t upto = base + scan(w, lane);
-        const uint64_t hit = __ballot(r0 + lane < n_rt && upto > r);
-        if (hit) {
-          const int j = __builtin_ctzll(hit);
-          rt = int(r0) + j;
-          r -= lane_of(upto, j) - lane_of(w, j);
-          break;
-        }
-        base = lane_of(upto, 63);
-      }
-    } else {
-      const uint32_t w = n_ct + uint32_t(max(tiles_of(a.Lk), 1)) + cost;
-      rt = int(r / w);
-      r -= uint32_t(rt) * w;
-    }
-    t = int(r);
+    t = int(in_seq - uint32_t(hk) * per_head);
   }
 };
 
@@ -619,13 +563,10 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
       if (todo > 0) {
         if (PREFIX) {
           const uint32_t weight = uint32_t(max(tiles_of(prefix_rows(a)), 1)) + kCost;
-          const uint32_t item = at / weight;
-          t0 = int(at - item * weight);
-          hk = int(item / uint32_t(n_rt));
-          rt = int(item - uint32_t(hk) * uint32_t(n_rt));
+          hk = int(at / weight);
+          t0 = int(at - uint32_t(hk) * weight);
         } else {
-          const OwnLine<RW> line{uint32_t(n_rt), line_fresh, total};
-          line.locate(a, lane, kCost, at, b, hk, rt, t0);
+          OwnLine{line_fresh, total}.locate(a, lane, at, b, hk, t0);
         }
       }
     } else {
@@ -1008,12 +949,9 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
     at += uint32_t(used);
     todo = __builtin_amdgcn_readfirstlane(todo - used);
     t0 = 0;
-    if (++rt == n_rt) {
-      rt = 0;
-      if (++hk == reread(args)->Hkv) {
-        hk = 0;
-        ++b;
-      }
+    if (++hk == reread(args)->Hkv) {
+      hk = 0;
+      ++b;
     }
   }
   if (!SHARED && splits == 0 && !args->own.by_item && threadIdx.x == 0) args->own.rec[w] = left;
@@ -1051,17 +989,17 @@ __global__ __launch_bounds__(kThreads, (Shape<T, D, RWO>::per_cu)) void paged_at
   // The prefix's workgroups come first.
   uint32_t w = blockIdx.x, n_pre = 0, pre_total = 0;
   if constexpr (RWP > 0) {
-    const uint32_t pre_items = uint32_t(a.Hkv) * (uint32_t(a.B * a.R + 32 * RWP - 1) / (32 * RWP));
-    pre_total = uniform(pre_items * (uint32_t(max(tiles_of(prefix_rows(a)), 1)) + kCostP));
     if (a.pre.splits) {
-      n_pre = pre_items * uint32_t(a.pre.splits);
+      n_pre = uint32_t(a.Hkv) * (uint32_t(a.B * a.R + 32 * RWP - 1) / (32 * RWP)) * uint32_t(a.pre.splits);
       if (w < n_pre) {
-        run_line<T, D, RWP, true, true>(args, smem, w, n_pre, pre_total, 0);
+        run_line<T, D, RWP, true, true>(args, smem, w, n_pre, 0, 0);
         return;
       }
+    } else {
+      pre_total = uniform(uint32_t(a.Hkv) * (uint32_t(max(tiles_of(prefix_rows(a)), 1)) + kCostP));
     }
   }
-  OwnLine<RWO> own{};
+  OwnLine own{};
   uint32_t n_own;
   if (a.own.splits) {
     n_own = uint32_t(a.B * a.Hkv) * (uint32_t(a.R + 32 * RWO - 1) / (32 * RWO)) * uint32_t(a.own.splits);
