@@ -1,4 +1,4 @@
-"""A KV cache in pages: sequences that grow on their own, fork, share a prefix and are freed.
+"""A KV cache in pages: sequences of different lengths that fork, share a prefix and are freed.
 
 ``KVCache`` (``kv_cache.py``) gives a batch one row range and one cursor, as the
 reference does (``models/dreamzero/model.py:35-65``). Here every layer has a pool
@@ -6,13 +6,16 @@ reference does (``models/dreamzero/model.py:35-65``). Here every layer has a poo
 of page numbers and a length of its own:
 
 * ``append(layer, k, v)`` writes one chunk per sequence at its own end and does not
-  move it; ``commit(n)`` does, once every layer has appended. Both as ``KVCache``.
+  move it; ``commit(n)`` does, once every layer has appended. Both as ``KVCache``: a
+  step is one of the whole batch, ``n`` rows for every sequence. Lengths come to differ
+  through ``free`` and ``fork``; ``SelfAttention`` then takes a rotary table per sequence.
 * ``fork(src, dst)`` makes sequence ``dst`` a copy of ``src`` by sharing its pages: no
   bytes move. The partly filled last page is copied when one of the two next writes
   to it (``kv_page_copy``, one launch for all layers).
 * ``hold_prefix(seq)`` turns the history of one sequence into a prefix of the whole
   batch (several candidate futures of one episode): it is kept once, and attention
-  computes it once for all sequences (``shared_prefix_attention``).
+  computes it once for all sequences (``shared_prefix_attention``). Until then it
+  takes pages in every sequence, for a step writes them all.
 * ``free(seq)`` gives a sequence's pages back; ``compact()`` moves what is in use to
   the lowest page numbers.
 
@@ -22,7 +25,10 @@ Which page is whose is decided on the host, before anything is launched:
 numbers and lengths from ``block_table`` ``[batch, W]`` and ``cache_lens`` ``[batch]``,
 int32 tensors on the device that are changed in place, so a graph captured once
 (``runtime.CachedStepGraph``) follows them; a captured step cannot reserve, so pages
-are reserved before it is replayed.
+are reserved before it is replayed. A ``reserve`` that takes pages sends the whole
+table, ``batch`` x ``W`` entries, with a copy that waits for what the stream holds (64 x
+256 entries take about a millisecond of the host's time): ``max_rows`` keeps ``W`` small,
+and one ``reserve`` of many rows ahead spares the steps after it.
 """
 
 from __future__ import annotations

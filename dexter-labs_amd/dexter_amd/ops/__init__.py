@@ -261,7 +261,7 @@ def kv_page_append(pages: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     ``block_table`` ``[B, W]`` and ``starts`` ``[B]`` are int32 on the device, read by
     the kernel when it runs. A row without a page (past the table, a start below 0, an
     entry outside ``[0, P)``) is not written, and ``status`` (one int32, optional) set
-    to 1. Sequences that write one page's same row in one call leave either's.
+    to 1. Sequences that write the same row of a page in one call leave a mix of theirs.
     """
     return select("cache", "page_append", pages, k, v)(pages, k, v, block_table, starts, status)
 

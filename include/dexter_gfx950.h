@@ -533,8 +533,10 @@ typedef struct dx_paged_call {
  * with cache_lens[b] (clamped to [0, width * page_rows]) as the cache length.
  * Keys of a table entry that holds no rows are not seen. Lk may be 0; width may
  * be 0 (block_table and cache_lens NULL). page_rows: a multiple of 16 up to 1024.
- * dtype: DX_BF16 or DX_F16 at D 64, 128 or 256, DX_F32 at D 64 or 128; sums and
- * softmax in fp32, one rounding to dtype. Sequences hold fewer than 2^30 rows;
+ * dtype: DX_BF16 or DX_F16 at D 64, 128 or 256, DX_F32 at D 64 or 128. Scores,
+ * softmax statistics, sums and partial results in fp32; in 16 bits each
+ * probability is rounded to dtype for its product with V (their sum is that of
+ * the rounded ones), then the result is. Sequences hold fewer than 2^30 rows;
  * the pool may exceed 4 GB. Row strides of the pool, k and v are below 2^26
  * bytes. workspace: dx_paged_attention_workspace_bytes(...) bytes, 16-byte
  * aligned, no initialisation (NULL when 0); calls that share one must not

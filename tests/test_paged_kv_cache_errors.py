@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from dexter_amd import ops
+from dexter_amd.models import PagedKVCache
 from test_paged_kv_cache import _cache, _check, _step, plain_ops  # noqa: F401
 
 
@@ -50,3 +51,22 @@ def test_a_sequence_that_does_not_exist(name, args):
         getattr(kv, name)(*args)
     assert _state(kv) == before
     _check(kv, want)
+
+
+def test_a_step_takes_pages_in_every_sequence():
+    """The sizes of the integration notes: 16 rollouts, 400 pages of 64 rows hold an episode of
+    1,600 rows until it is held as a prefix, which frees the other 15 copies."""
+    kv = PagedKVCache(1, 16, 400, 64, 1, 4, "cpu", torch.float32, max_rows=2048)
+    with pytest.raises(RuntimeError, match="KV cache full: 416 pages needed, 400 of 400 free"):
+        kv.reserve(1601)
+    kv.reserve(1600)
+    kv.commit(1600)
+    assert kv.free_pages == 0
+    kv.hold_prefix(0)
+    assert kv.free_pages == 375 and kv.prefix_rows == 1600 and kv.lengths == [0] * 16
+    kv.reserve(83)
+    kv.commit(83)
+    kv.fork(3, 5)
+    kv.free(7)
+    kv.compact()
+    assert kv.lengths == [83] * 7 + [0] + [83] * 8
