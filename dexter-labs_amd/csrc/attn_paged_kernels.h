@@ -29,8 +29,8 @@
 //  * Split (several row tiles read the same keys): every item in S equal ranges
 //    of keys, a workgroup each, those of one head next to each other on one XCD,
 //    so that they read a key tile at about the same time, through one L2. 16 x 83
-//    queries over a shared 8,217-row prefix (24 heads) take 202 us so, and 242 cut
-//    (every workgroup at a place of its own in the keys).
+//    queries over a shared 8,217-row prefix (24 heads) took 205 us so, and 242 cut
+//    (every workgroup at a place of its own in the keys), both with the join.
 // With a prefix every row has parts of both lines, and the merge joins them all.
 //
 // Kernel. A wave owns 32 rows (S^T = K Q^T on 32 x 32 MFMAs, the formulation of
@@ -42,13 +42,20 @@
 // arithmetic, and rows past the end (or of a table entry that names no page)
 // come back as zeros from the descriptor's bound.
 //
-// What it takes (bf16, D 128; kernel alone, the join 4-7 us more, 20 where said):
+// What it takes (medians; bf16, D 128 where not said; kernel alone, the join 4-8 us
+// more where not said):
 //   32 tokens, 8 K/V heads, 300 to 3,000 cached rows each   48 us, 4.4 TB/s
+//   the same at D 256                                        84 us, 5.1 TB/s
 //   83 queries, 24 heads, 32,768 cached rows                 84 us, 4.8 TB/s
-//   64 tokens, 8 K/V heads, 1 to 500 rows, prefix of 4,001   27 us, 3.1 TB/s
-//   16 x 83, 24 heads, 0 to 332 rows, prefix of 8,217        202 us, 680 TFLOP/s (join 20)
-//   2 x 1,500 causal, 8 K/V heads, 400 to 1,000 rows         78 us, 420 TFLOP/s
-//   4 x 99 in fp32, 24 heads, 0 to 1,245 rows                64 us, 47 TFLOP/s
+//   64 tokens, 8 K/V heads, 1 to 500 rows, prefix of 4,001   26 us, 3.2 TB/s
+//   the same at D 256                                        62 us, 2.6 TB/s
+//   the same in fp32                                         95 us, 1.7 TB/s
+//   16 x 83, 24 heads, 0 to 332 rows, prefix of 8,217        200 us, 690 TFLOP/s (join 20)
+//   8 x 83, 24 heads, D 256, 0 to 332 rows, prefix of 4,001  185 us, 373 TFLOP/s (join 17)
+//   4 x 99 in fp32, 24 heads, 0 to 332 rows, prefix of 2,000 157 us, 69 TFLOP/s (join 10)
+//   2 x 1,500 causal, 8 K/V heads, 400 to 1,000 rows         79 us, 418 TFLOP/s (no join)
+//   the same at D 256                                        178 us, 369 TFLOP/s (join 23)
+//   4 x 99 in fp32, 24 heads, 0 to 1,245 rows                62 us, 48 TFLOP/s
 // Many keys to a row tile: bound by memory. Otherwise by the chain of a tile (scores,
 // softmax, product) in the few waves that registers allow, and by the 4 to 8 us from
 // a workgroup's start to its first product: lengths, table, keys and queries, one
@@ -347,6 +354,12 @@ struct Tile {
       }
       __builtin_amdgcn_sched_barrier(0);
     } else {
+      // Probabilities in 16 bits: a lane's scores are then, packed, the operand of the
+      // 16-bit product as they lie. Kept in 32 they would need fp32 products, a sixteenth of
+      // the peak rate, or a second product of what the rounding left. l sums the rounded ones, so
+      // that a row's weights still add up to 1. Against 64 bits, relative to the
+      // outputs' norm: 0.0023 in bf16 and 2.9e-4 in f16, of which the result's own rounding
+      // is 0.0017 and 2.1e-4.
       u32x4 pk[2 * NS];
       float part[2] = {0.f, 0.f};
 #pragma unroll
