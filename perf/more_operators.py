@@ -307,7 +307,8 @@ def _run_own(kind, case, s):
                                      cache_lens=s["lens"])
     if kind == "keep":
         return ops.kv_keep_rows(s["weights"], s["lens"], case["keep"], case["recent"])
-    ops.kv_page_gather(s["pages"], s["table"], s["rows"], s["to"], s["weights"])
+    ops.kv_page_gather(s["pages"], s["table"], s["rows"], s["to"], s["weights"],
+                       head_dim=case["dim"] if case["fp4"] else None)
     return _pool_values(case, s), s["weights"]
 
 
