@@ -41,6 +41,7 @@ struct PagedArgs {
   float scale_log2;             // signed
   int own_n;                    // workgroups for the own line at most, where it alone is cut
   Line own, pre;
+  float* lse;                   // [B, Lq, H], or null
 };
 
 constexpr int64_t kMaxItemCost = 16;  // kItemCost at most
@@ -56,9 +57,15 @@ struct PagedPlan {
   bool merge;
 };
 
-// Launch the plan (head dims: attn_paged.hip's checks).
+// Launch the plan (head dims: attn_paged.hip's checks). _lse: with the queries' log-sum-exps;
+// _fp4: over cached rows in 4 bits.
 hipError_t launch_paged_bf16(const PagedArgs& a, const PagedPlan& p, int D, hipStream_t st);
 hipError_t launch_paged_f16(const PagedArgs& a, const PagedPlan& p, int D, hipStream_t st);
 hipError_t launch_paged_f32(const PagedArgs& a, const PagedPlan& p, int D, hipStream_t st);
+hipError_t launch_paged_bf16_lse(const PagedArgs& a, const PagedPlan& p, int D, hipStream_t st);
+hipError_t launch_paged_f16_lse(const PagedArgs& a, const PagedPlan& p, int D, hipStream_t st);
+hipError_t launch_paged_f32_lse(const PagedArgs& a, const PagedPlan& p, int D, hipStream_t st);
+hipError_t launch_paged_bf16_fp4(const PagedArgs& a, const PagedPlan& p, int D, hipStream_t st);
+hipError_t launch_paged_f16_fp4(const PagedArgs& a, const PagedPlan& p, int D, hipStream_t st);
 
 }  // namespace dx

@@ -135,9 +135,19 @@ int check_sizes(const char* what, int64_t B, int64_t Lq, int64_t Lk, int64_t H, 
   return DX_OK;
 }
 
-int paged_entry(const char* what, const dx_paged_call* call, bool prefix) {
+// What a call reads and writes besides: the queries' log-sum-exps, cached rows in 4 bits.
+struct Form {
+  bool prefix, fp4, with_lse;
+  void* lse;
+};
+
+int paged_entry(const char* what, const dx_paged_call* call, Form form) {
+  const bool prefix = form.prefix;
   DX_CHECK_ARG(call, "%s: null call", what);
   dx_paged_call c = *call;
+  DX_CHECK_ARG(!form.fp4 || c.dtype == DX_BF16 || c.dtype == DX_F16,
+               "%s: dtype code %lld unsupported (a 4-bit cache serves bf16 and f16)", what,
+               (long long)c.dtype);
   if (!prefix) {
     c.prefix_table = c.prefix_len = nullptr;
     c.prefix_width = 0;
@@ -164,11 +174,18 @@ int paged_entry(const char* what, const dx_paged_call* call, bool prefix) {
   DX_CHECK_ARG(!prefix || c.prefix_len, "%s: null prefix length", what);
   DX_CHECK_ARG(c.prefix_width == 0 || c.prefix_table, "%s: null prefix table", what);
   DX_CHECK_ARG(c.n_pages == 0 || c.pages, "%s: null pages", what);
+  DX_CHECK_ARG(!form.with_lse || (form.lse && (reinterpret_cast<uintptr_t>(form.lse) & 3u) == 0),
+               "%s: null or misaligned lse", what);
   DX_CHECK_ARG(al(c.q) && al(c.k) && al(c.v) && al(c.pages) && al(c.out),
                "%s: pointers must be 16-byte aligned", what);
+  // A pool's element size; one in 4 bits is bytes, with its rows where the format has them.
+  const int64_t pe = form.fp4 ? 1 : es;
+  if (form.fp4) c.p_sr = c.D / 2;
   for (const int64_t s : {c.q_sb, c.q_sl, c.q_sh, c.k_sb, c.k_sl, c.k_sh, c.v_sb, c.v_sl, c.v_sh,
-                          c.p_plane, c.p_sp, c.p_sr, c.p_sh, c.o_sb, c.o_sl, c.o_sh})
+                          c.o_sb, c.o_sl, c.o_sh})
     DX_CHECK_ARG(s % per16 == 0, "%s: strides must keep head rows 16-byte aligned", what);
+  for (const int64_t s : {c.p_plane, c.p_sp, c.p_sr, c.p_sh})
+    DX_CHECK_ARG(s % (16 / pe) == 0, "%s: strides must keep head rows 16-byte aligned", what);
   // 16 rows of keys lie within one buffer descriptor (below 2^31 bytes).
   for (const int64_t s : {c.p_sr, c.k_sl, c.v_sl})
     DX_CHECK_ARG(s >= 0 && s * es < (int64_t(1) << 26), "%s: row stride %lld out of range", what,
@@ -198,8 +215,9 @@ int paged_entry(const char* what, const dx_paged_call* call, bool prefix) {
   a.q = static_cast<const char*>(c.q); a.q_sb = c.q_sb * es; a.q_sl = c.q_sl * es; a.q_sh = c.q_sh * es;
   a.k = static_cast<const char*>(c.k); a.k_sb = c.k_sb * es; a.k_sl = c.k_sl * es; a.k_sh = c.k_sh * es;
   a.v = static_cast<const char*>(c.v); a.v_sb = c.v_sb * es; a.v_sl = c.v_sl * es; a.v_sh = c.v_sh * es;
-  a.pk = static_cast<const char*>(c.pages); a.pv = a.pk + c.p_plane * es;
-  a.p_sp = c.p_sp * es; a.p_sr = c.p_sr * es; a.p_sh = c.p_sh * es;
+  a.pk = static_cast<const char*>(c.pages); a.pv = a.pk + c.p_plane * pe;
+  a.p_sp = c.p_sp * pe; a.p_sr = c.p_sr * pe; a.p_sh = c.p_sh * pe;
+  a.lse = static_cast<float*>(form.lse);
   a.out = static_cast<char*>(c.out); a.o_sb = c.o_sb * es; a.o_sl = c.o_sl * es; a.o_sh = c.o_sh * es;
   a.table = static_cast<const int32_t*>(c.block_table); a.t_sb = c.t_sb;
   a.lens = static_cast<const int32_t*>(c.cache_lens);
@@ -233,9 +251,18 @@ int paged_entry(const char* what, const dx_paged_call* call, bool prefix) {
   a.pre.rec = reinterpret_cast<Record*>(take(p.pre_recs * int64_t(sizeof(Record))));
   const hipStream_t st = static_cast<hipStream_t>(c.stream);
   const int D = int(c.D);
-  const hipError_t e = c.dtype == DX_F32    ? launch_paged_f32(a, p, D, st)
-                       : c.dtype == DX_BF16 ? launch_paged_bf16(a, p, D, st)
-                                            : launch_paged_f16(a, p, D, st);
+  const bool bf16 = c.dtype == DX_BF16;
+  hipError_t e;
+  if (form.fp4)
+    e = bf16 ? launch_paged_bf16_fp4(a, p, D, st) : launch_paged_f16_fp4(a, p, D, st);
+  else if (form.with_lse)
+    e = c.dtype == DX_F32 ? launch_paged_f32_lse(a, p, D, st)
+        : bf16            ? launch_paged_bf16_lse(a, p, D, st)
+                          : launch_paged_f16_lse(a, p, D, st);
+  else
+    e = c.dtype == DX_F32 ? launch_paged_f32(a, p, D, st)
+        : bf16            ? launch_paged_bf16(a, p, D, st)
+                          : launch_paged_f16(a, p, D, st);
   if (e != hipSuccess) {
     set_error("%s: launch failed: %s", what, hipGetErrorString(e));
     return DX_ELAUNCH;
@@ -262,9 +289,25 @@ extern "C" int64_t dx_paged_attention_workspace_bytes(int dtype, int64_t B, int6
 }
 
 extern "C" int dx_paged_attention(const dx_paged_call* call) {
-  return paged_entry("paged_attention", call, false);
+  return paged_entry("paged_attention", call, {false, false, false, nullptr});
 }
 
 extern "C" int dx_shared_prefix_attention(const dx_paged_call* call) {
-  return paged_entry("shared_prefix_attention", call, true);
+  return paged_entry("shared_prefix_attention", call, {true, false, false, nullptr});
+}
+
+extern "C" int dx_paged_attention_lse(const dx_paged_call* call, void* lse) {
+  return paged_entry("paged_attention", call, {false, false, true, lse});
+}
+
+extern "C" int dx_shared_prefix_attention_lse(const dx_paged_call* call, void* lse) {
+  return paged_entry("shared_prefix_attention", call, {true, false, true, lse});
+}
+
+extern "C" int dx_paged_attention_fp4(const dx_paged_call* call, void* lse) {
+  return paged_entry("paged_attention_fp4", call, {false, true, lse != nullptr, lse});
+}
+
+extern "C" int dx_shared_prefix_attention_fp4(const dx_paged_call* call, void* lse) {
+  return paged_entry("shared_prefix_attention_fp4", call, {true, true, lse != nullptr, lse});
 }

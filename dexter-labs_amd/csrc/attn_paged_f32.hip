@@ -5,8 +5,8 @@ namespace dx {
 
 hipError_t launch_paged_f32(const PagedArgs& a, const PagedPlan& p, int D, hipStream_t st) {
   switch (D) {
-    case 64: return launch_paged<float, 64>(a, p, st);
-    case 128: return launch_paged<float, 128>(a, p, st);
+    case 64: return launch_paged<float, 64, kPlain>(a, p, st);
+    case 128: return launch_paged<float, 128, kPlain>(a, p, st);
     default: return hipErrorInvalidValue;
   }
 }

@@ -64,6 +64,7 @@
 
 #include "attn_paged.h"
 #include "attn_tile.h"
+#include "kv_fp4.h"
 
 #include <float.h>
 #include <limits.h>
@@ -85,6 +86,10 @@ __device__ __forceinline__ Args* reread(Args* a) {
 
 template <typename T> struct Elem { static constexpr int bytes = 2; };
 template <> struct Elem<float> { static constexpr int bytes = 4; };
+
+// What a launch reads and writes besides: kLse, each query's log-sum-exp; kFp4, cached
+// rows in 4 bits (kv_fp4.h), and the log-sum-exp where it is asked for.
+enum Mode { kPlain, kLse, kFp4 };
 
 // Tile rows of RB bytes in LDS: 16-byte chunk c of row r sits at c ^ kswz(r)
 // (K) or c ^ vswz(r) (V). K: the swizzles of attn_fwd.hip and attn_wide.hip,
@@ -132,6 +137,11 @@ template <typename T, int D, int RW> struct Shape {
   static constexpr int lds = votes + 16;
   static_assert(lds * per_cu <= 160 * 1024, "the LDS of a CU");
 };
+
+// ln of l 2^m, of base-2 scores: -inf where a row saw no key (m = -inf, l = 0).
+__device__ __forceinline__ float log_sum(float m, float l) {
+  return 0.69314718055994531f * (m + __builtin_amdgcn_logf(l));
+}
 
 __device__ __forceinline__ int tiles_of(int rows) { return (rows + kPN - 1) / kPN; }
 
@@ -230,7 +240,7 @@ struct OwnLine {
 };
 
 // One wave's S tile (TK / 32 blocks of 32 keys), softmax step and PV product.
-template <typename T, int D, int NS>
+template <typename T, int D, int NS, Mode M>
 struct Tile {
   static constexpr bool F32 = Elem<T>::bytes == 4;
   static constexpr int RB = D * Elem<T>::bytes, KS = RB / 32, DT = D / 32;
@@ -246,10 +256,12 @@ struct Tile {
   // S^T = K Q^T of the tile, K fragments read W ahead of the products that use
   // them: left alone the compiler reads each right before its product, which
   // then waits out the LDS latency.
-  static __device__ __forceinline__ void scores(uint32_t ka, const u32x4 (&qr)[KS], f32x16 (&s)[NS]) {
+  // chunk(i): of the row, less this lane's, what product i takes.
+  template <typename Chunk>
+  static __device__ __forceinline__ void scores(uint32_t ka, const u32x4 (&qr)[KS], f32x16 (&s)[NS], Chunk chunk) {
     constexpr int N = KS * NS, W = F32 ? 2 : 4;
     auto frag = [&](int i) __attribute__((always_inline)) {
-      return lds_read_b128_at((ka ^ (32u * (i / NS))) + 32 * RB * (i % NS));
+      return lds_read_b128_at((ka ^ (16u * chunk(i / NS))) + 32 * RB * (i % NS));
     };
     __builtin_amdgcn_sched_barrier(0);
     u32x4 kf[W];
@@ -360,6 +372,9 @@ struct Tile {
       // that a row's weights still add up to 1. Against 64 bits, relative to the
       // outputs' norm: 0.0023 in bf16 and 2.9e-4 in f16, of which the result's own rounding
       // is 0.0017 and 2.1e-4.
+      // With a log-sum-exp, a result in 32 bits, l sums them as they were before that rounding
+      // (2^-9 of each in bf16), and a row's weights add up to 1 but for what their roundings
+      // come to.
       u32x4 pk[2 * NS];
       float part[2] = {0.f, 0.f};
 #pragma unroll
@@ -368,7 +383,10 @@ struct Tile {
         for (int e = 0; e < 4; ++e) {
           const uint32_t p = Mfma<T>::pack(s[u / 2][8 * (u % 2) + 2 * e], s[u / 2][8 * (u % 2) + 2 * e + 1]);
           pk[u][e] = p;
-          part[e & 1] = Mfma<T>::sum2(p, part[e & 1]);
+          if constexpr (M == kPlain)
+            part[e & 1] = Mfma<T>::sum2(p, part[e & 1]);
+          else
+            part[e & 1] += s[u / 2][8 * (u % 2) + 2 * e] + s[u / 2][8 * (u % 2) + 2 * e + 1];
         }
       l += part[0] + part[1];
 #pragma unroll
@@ -498,8 +516,10 @@ struct Keys {
   int n_ct;        // 32-key tiles of the cached rows; the new ones' follow
 
   // The 16 rows from row r0 of the cached ones, or of the new ones: addresses,
-  // and how many exist. True where the table names no page for them.
-  __device__ __forceinline__ bool find(bool cached, int r0, uint64_t& k, uint64_t& v, int& rows) const {
+  // and how many exist. True where the table names no page for them. in_page: where a
+  // cached one's page has the first.
+  __device__ __forceinline__ bool find(bool cached, int r0, uint64_t& k, uint64_t& v, int& rows,
+                                       uint32_t& in_page) const {
     rows = max(min((cached ? len : fresh) - r0, 16), 0);
     bool gone = false;
     if (cached) {
@@ -510,7 +530,8 @@ struct Keys {
       const int page = rows > 0 ? ((const_i32*)table)[e] : 0;
       gone = uint32_t(page) >= uint32_t(n_pages);
       rows = gone ? 0 : rows;
-      const uint64_t off = uint64_t(page * p_sp) + uint64_t(uint32_t(r0) - e * uint32_t(page_rows)) * uint32_t(p_sr);
+      in_page = uint32_t(r0) - e * uint32_t(page_rows);
+      const uint64_t off = uint64_t(page * p_sp) + uint64_t(in_page) * uint32_t(p_sr);
       k = pk + off;
       v = pv + off;
     } else {
@@ -521,6 +542,95 @@ struct Keys {
     v = uniform(v);
     rows = __builtin_amdgcn_readfirstlane(rows);
     return gone;
+  }
+  __device__ __forceinline__ bool find(bool cached, int r0, uint64_t& k, uint64_t& v, int& rows) const {
+    uint32_t in_page = 0;
+    return find(cached, r0, k, v, rows, in_page);
+  }
+};
+
+// NR rows of 16 in 4 bits, from row r0 of the 16 on, on their way through a wave's
+// registers into a tile of T in LDS. A lane takes 16 bytes of codes, which are one
+// block, and its scale: the 16 rows' codes are one piece of a page, as are their scales.
+// Of the 16 only `rows` exist: the others come back as zeros from the descriptors' bounds.
+template <typename T, int D, int NR>
+struct Coded {
+  static constexpr int BR = D / 32, N = (NR * BR + 63) / 64;  // blocks of a row, of a lane
+  u32x4 code[N];
+  uint32_t scale[N];
+
+  __device__ __forceinline__ void load(uint64_t codes, uint64_t scales, int rows, int r0, int lane) {
+    const __amdgpu_buffer_rsrc_t rc = __builtin_amdgcn_make_buffer_rsrc(
+        reinterpret_cast<char*>(codes), (short)0, rows * (D / 2), kBufWord3);
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+        reinterpret_cast<char*>(scales), (short)0, rows * BR, kBufWord3);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint32_t blk = uint32_t(r0 * BR + i * 64 + lane);
+      const uint32_t past = i * 64 + lane < NR * BR ? 0u : 0x80000000u;
+      code[i] = __builtin_amdgcn_raw_buffer_load_b128(rc, int((16 * blk) | past), 0, 0);
+      scale[i] = uint32_t(__builtin_amdgcn_raw_buffer_load_b8(rs, int(blk | past), 0, 0)) & 255u;
+    }
+  }
+  // To the rows from tr0 on of the tile at `to`.
+  template <bool K>
+  __device__ __forceinline__ void store(uint32_t to, int tr0, int lane) const {
+    constexpr int RB = 2 * D;
+    typedef __attribute__((address_space(3))) u32x4 lds_u32x4_w;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int at = i * 64 + lane;
+      if (at >= NR * BR) continue;
+      const int tr = tr0 + at / BR, swz = K ? kswz<RB>(tr) : vswz<RB, false>(tr);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        *reinterpret_cast<lds_u32x4_w*>(to + tr * RB + 16 * ((4 * (at % BR) + e) ^ swz)) =
+            fp4_values<T>(code[i][e], fp4_scale(scale[i]));
+    }
+  }
+};
+
+// 32 keys in 4 bits as the first operand of their products: a lane holds half of a
+// key's dims, blocks 2 i + g, and needs no LDS. Rows of a page that are not the
+// sequence's are read too: their scores are hidden, whatever they are. Where no row of
+// the 16 exists their lanes read D / 2 bytes at `safe`.
+template <typename T, int D>
+struct CodedKeys {
+  static constexpr int N = D / 64;  // blocks of a lane
+  u32x4 code[N];
+  uint32_t scale[N == 4 ? 2 : 1];   // of the row's blocks, a byte each
+
+  __device__ __forceinline__ void load(uint64_t k0, uint64_t s0, int rows0, uint64_t k1, uint64_t s1,
+                                       int rows1, uint64_t safe, int lane) {
+    k0 = rows0 > 0 ? k0 : safe;
+    k1 = rows1 > 0 ? k1 : safe;
+    s0 = rows0 > 0 ? s0 : safe;
+    s1 = rows1 > 0 ? s1 : safe;
+    const int row = (lane & 16 ? rows1 : rows0) > 0 ? lane & 15 : 0, g = lane >> 5;
+    const uint64_t k = (lane & 16 ? k1 : k0) + uint32_t(row * (D / 2) + 16 * g);
+    const uint64_t s = (lane & 16 ? s1 : s0) + uint32_t(row * (D / 32));
+#pragma unroll
+    for (int i = 0; i < N; ++i) code[i] = *reinterpret_cast<const u32x4*>(k + 32 * i);
+    if constexpr (N == 1) {
+      scale[0] = *reinterpret_cast<const uint16_t*>(s);
+    } else if constexpr (N == 2) {
+      scale[0] = *reinterpret_cast<const uint32_t*>(s);
+    } else {
+      const u32x2 x = *reinterpret_cast<const u32x2*>(s);
+      scale[0] = x[0];
+      scale[1] = x[1];
+    }
+  }
+  // S^T = K Q^T; qr as load_queries leaves it for these blocks.
+  __device__ __forceinline__ void scores(const u32x4 (&qr)[D / 16], f32x16& s, int lane) const {
+    s = f32x16{};
+    const int g = lane >> 5;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float sc = fp4_scale((scale[i / 2] >> (16 * (i % 2) + 8 * g)) & 255u);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s = Mfma<T>::run(fp4_values<T>(code[i][e], sc), qr[4 * i + e], s);
+    }
   }
 };
 
@@ -544,12 +654,16 @@ __device__ __forceinline__ void send_rows(uint64_t from, int rows, int step, uin
 }
 
 // One workgroup's share of a line: workgroup w of n.
-template <typename T, int D, int RW, bool PREFIX, bool SHARED>
+template <typename T, int D, int RW, bool PREFIX, bool SHARED, Mode M>
 __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uint32_t n,
                                          uint32_t total, uint32_t line_fresh) {
   using Sh = Shape<T, D, RW>;
   constexpr int RB = Sh::RB, KW = Sh::KW, TK = Sh::TK, CR = RB / 16, RPP = 64 / CR;
-  using Ti = Tile<T, D, TK / 32>;
+  using Ti = Tile<T, D, TK / 32, M>;
+  // Single row waves over 4 bits: a key's dims go to lanes by blocks (CodedKeys), 8 dims
+  // of product s being chunk chunk_of(s) + 4 g of the row; else chunk 2 s + g.
+  constexpr bool kByBlocks = M == kFp4 && RW == 1;
+  auto chunk_of = [](int s) { return kByBlocks ? 8 * (s / 4) + s % 4 : 2 * s; };
   constexpr bool F32 = Ti::F32;
   constexpr int KS = Ti::KS;
   constexpr int UT = TK / kPN;  // 32-key tiles that a stream takes at a time
@@ -619,8 +733,10 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
     const bool first = t0 == 0;  // this share holds the item's first tile: it leaves the record
     bool active, behind = false;
     int history;  // what the masks call the cache
+    uint64_t safe = 0;  // memory of this call: a query, 2 D bytes
     {
       Args& a = *reread(args);
+      if (kByBlocks) safe = reinterpret_cast<uint64_t>(a.q);
       const int nrows = PREFIX ? a.B * a.R : a.R;
       const int pre_len = __builtin_amdgcn_readfirstlane(prefix_rows(a));
       const int own_len = PREFIX ? 0 : __builtin_amdgcn_readfirstlane(own_rows(a, b));
@@ -684,15 +800,15 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
       }
       const int qi = int(rr / uint32_t(a.group));
       const int hq = hk * a.group + int(rr - uint32_t(qi) * uint32_t(a.group));
-      const char* const qp = a.q + bq * a.q_sb + qi * a.q_sl + hq * a.q_sh + 16 * g;
+      const char* const qp = a.q + bq * a.q_sb + qi * a.q_sl + hq * a.q_sh + (kByBlocks ? 64 : 16) * g;
       const uint32_t flip = a.scale_log2 < 0.f ? (F32 ? 0x80000000u : 0x80008000u) : 0u;
 #pragma unroll
-      for (int s = 0; s < KS; ++s) qr[s] = *reinterpret_cast<const u32x4*>(qp + 32 * s) ^ flip;
+      for (int s = 0; s < KS; ++s) qr[s] = *reinterpret_cast<const u32x4*>(qp + 16 * chunk_of(s)) ^ flip;
       if (!PREFIX && rvalid) my_end = visible_end(a, qi, history);  // new keys seen
     };
 
     const uint32_t base = lds_addr(smem) + stream * Sh::stream;
-    const uint32_t ka = base + nl * RB + 16 * (g ^ kswz<RB>(nl));
+    const uint32_t ka = base + nl * RB + 16 * ((kByBlocks ? 4 * g : g) ^ kswz<RB>(nl));
     uint32_t va;
     if (F32) {
       va = base + Sh::tile + 4 * g * RB + 4 * nl + 128 * g;
@@ -719,7 +835,75 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
     const bool partly = !PREFIX && !behind && full_end < keys.fresh;
     for (bool careful = false;; careful = true) {
     ti.reset();
-    if constexpr (RW == 1) {
+    if constexpr (kByBlocks) {
+      // Streams of one wave: no barriers. Cached tiles' codes wait in registers, one tile ahead;
+      // K is converted there, V on its way into LDS. New tiles come by DMA.
+      constexpr int HP = 16 / RPP;
+      uint64_t v0, v1;
+      int rows0, rows1, sv = 0;
+      uint32_t gone = 0;
+      CodedKeys<T, D> kc;
+      Coded<T, D, 16> vc0, vc1;
+      auto next = [&](int t) __attribute__((always_inline)) {  // K's place, kc and vc are free
+        const bool cached = t < keys.n_ct;
+        const int r0 = (cached ? t : t - keys.n_ct) * kPN;
+        uint64_t k0, k1;
+        uint32_t in0 = 0, in1 = 0;
+        gone = keys.find(cached, r0, k0, v0, rows0, in0) ? 1 : 0;
+        gone |= keys.find(cached, r0 + 16, k1, v1, rows1, in1) ? 2 : 0;
+        if (cached) {
+          const uint64_t s0 = fp4_scales_behind<D>(keys.page_rows, in0);
+          const uint64_t s1 = fp4_scales_behind<D>(keys.page_rows, in1);
+          kc.load(k0, k0 + s0, rows0, k1, k1 + s1, rows1, safe, lane);
+          vc0.load(v0, v0 + s0, rows0, 0, lane);
+          vc1.load(v1, v1 + s1, rows1, 0, lane);
+        } else {
+          sv = __builtin_amdgcn_readfirstlane(keys.v_sl);
+          send_rows<RB, F32, true>(k0, rows0, keys.k_sl, base, 0, 0, HP, lane);
+          send_rows<RB, F32, true>(k1, rows1, keys.k_sl, base + 16 * RB, 0, 16, HP, lane);
+        }
+      };
+      auto send_v = [&]() __attribute__((always_inline)) {
+        send_rows<RB, F32, false>(v0, rows0, sv, base + Sh::tile, 0, 0, HP, lane);
+        send_rows<RB, F32, false>(v1, rows1, sv, base + Sh::tile + 16 * RB, 0, 16, HP, lane);
+      };
+      if (nt > 0) {
+        next(tile_at(0));
+        if (tile_at(0) >= keys.n_ct) send_v();
+      }
+      if (!careful) load_queries();
+      for (int i = 0; i < nt; ++i) {
+        const int t = tile_at(i);
+        const bool cached = t < keys.n_ct, more = i + 1 < nt;
+        const uint32_t bad = gone;
+        f32x16 s[1];
+        if (cached) {
+          vc0.template store<false>(base + Sh::tile, 0, lane);
+          vc1.template store<false>(base + Sh::tile, 16, lane);
+          kc.scores(qr, s[0], lane);
+        } else {
+          wait_vmcnt<2 * HP>();  // K (V was sent last)
+          Ti::scores(ka, qr, s, chunk_of);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (more) next(tile_at(i + 1));
+        bool masked;
+        const int lim = limits(t, masked);
+        ti.softmax(s, masked, lim, bad, c);
+        if (!cached) {
+          if (more) wait_vmcnt<2 * HP>();  // V (the next K was sent last)
+          else wait_vmcnt<0>();
+          if (!PREFIX && careful && masked && Ti::poisoned(base + Sh::tile, lane)) {
+            ti.take_poison(base + Sh::tile, s, {lim + 4 * g}, lane);
+            Ti::clear_poison(base + Sh::tile, 0, Sh::tile, lane);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+          }
+        }
+        ti.pv(va, s);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (more && tile_at(i + 1) >= keys.n_ct) send_v();
+      }
+    } else if constexpr (RW == 1) {
       // Streams of one wave: no barriers, each wave waits for its own pieces.
       constexpr int HP = 16 / RPP;  // pieces of a 16-row group
       uint64_t k0, v0, k1, v1;
@@ -749,7 +933,7 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
         const uint32_t bad = gone;
         wait_vmcnt<2 * HP>();  // K of tile i (its V was sent last)
         f32x16 s[1];
-        Ti::scores(ka, qr, s);
+        Ti::scores(ka, qr, s, chunk_of);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K is read: its place is free
         if (more) find(tile_at(i + 1));
         bool masked;
@@ -771,6 +955,18 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
       constexpr int WR = TK / RW;
       static_assert(16 % WR == 0 && WR % RPP == 0, "a wave's rows lie in one 16-row group");
       uint32_t* const flags = reinterpret_cast<uint32_t*>(smem + Sh::flags) + stream * 2 * 4;
+      // Cached rows in 4 bits go through registers: take_tile writes what send_tile read to the
+      // stage that is sent to, any time before the barrier that publishes it.
+      Coded<T, D, M == kFp4 ? WR : 16> kc, vc;
+      bool coming = false;
+      auto take_tile = [&](int i) __attribute__((always_inline)) {
+        if constexpr (M == kFp4) {
+          if (!coming) return;
+          const uint32_t to = base + (i & 1) * 2 * Sh::tile;
+          kc.template store<true>(to, wave * WR, lane);
+          vc.template store<false>(to + Sh::tile, wave * WR, lane);
+        }
+      };
       auto send_tile = [&](int i) __attribute__((always_inline)) {
         const int st = i & 1;
         const int tr = wave * WR;                 // this wave's first row of the tile
@@ -781,16 +977,27 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
         const int r0 = t < t1 ? (cached ? t : t - keys.n_ct) * kPN + tr % kPN / 16 * 16 : INT_MAX;
         uint64_t k, v;
         int rows;
-        const bool gone = keys.find(cached, r0, k, v, rows);
+        uint32_t in_page = 0;
+        const bool gone = keys.find(cached, r0, k, v, rows, in_page);
         if (lane == 0) flags[4 * st + wave] = gone ? 1u : 0u;
         const int sk = __builtin_amdgcn_readfirstlane(cached ? keys.p_sr : keys.k_sl);
         const int sv = __builtin_amdgcn_readfirstlane(cached ? keys.p_sr : keys.v_sl);
         const uint32_t to = base + st * 2 * Sh::tile + tr * RB;
+        if constexpr (M == kFp4) {
+          coming = cached;
+          if (cached) {
+            const uint64_t sc = fp4_scales_behind<D>(keys.page_rows, in_page);
+            kc.load(k, k + sc, rows, tr % 16, lane);
+            vc.load(v, v + sc, rows, tr % 16, lane);
+            return;
+          }
+        }
         send_rows<RB, F32, true>(k, rows, sk, to, tr % 16, tr, WR / RPP, lane);
         send_rows<RB, F32, false>(v, rows, sv, to + Sh::tile, tr % 16, tr, WR / RPP, lane);
       };
       if (nt > 0) send_tile(0);
       if (!careful) load_queries();
+      if (nt > 0) take_tile(0);
       for (int i = 0; i < iters; ++i) {
         // This wave's pieces of tile i have landed; past the barrier the tile
         // is whole, and reads of the stage that is sent to next have returned.
@@ -823,10 +1030,11 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
         };
         if (!active) {
           if (poison) clear();
+          if (i + 1 < nt) take_tile(i + 1);
           continue;
         }
         f32x16 s[UT];
-        Ti::scores(ka + st, qr, s);
+        Ti::scores(ka + st, qr, s, chunk_of);
         const u32x4 fl = *reinterpret_cast<const u32x4*>(flags + 4 * (i & 1));
         int seen[UT];
         seen[0] = masked ? lim + 4 * g : kPN;
@@ -857,6 +1065,7 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
           clear();
         }
         ti.pv(va + st, s);
+        if (i + 1 < nt) take_tile(i + 1);
       }
     }
     if (!partly || careful) break;
@@ -923,11 +1132,14 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
           }
           const int col = pass * Sh::DP + 8 * ch;
           if (!SHARED && whole) {
-            // The result. No visible key: 0 * inf = NaN, as the reference's softmax.
+            // The result. No visible key: 0 * inf = NaN, as the reference's softmax (and a
+            // log-sum-exp of -inf).
             const float inv = 1.0f / l;
             const uint32_t rr = uint32_t(row0 + r);
             const int qo = int(rr / uint32_t(a.group));
             const int ho = hk * a.group + int(rr - uint32_t(qo) * uint32_t(a.group));
+            if constexpr (M != kPlain)
+              if (a.lse && col == 0) a.lse[(int64_t(b) * a.Lq + qo) * a.H + ho] = log_sum(mm, l);
             char* const op = a.out + b * a.o_sb + qo * a.o_sl + ho * a.o_sh + col * Elem<T>::bytes;
             if constexpr (F32) {
               reinterpret_cast<f32x4*>(op)[0] = o[0] * inv;
@@ -970,7 +1182,7 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
   if (!SHARED && splits == 0 && !args->own.by_item && threadIdx.x == 0) args->own.rec[w] = left;
 }
 
-template <typename T, int D, int RWP, int RWO>
+template <typename T, int D, int RWP, int RWO, Mode M>
 __global__ __launch_bounds__(kThreads, (Shape<T, D, RWO>::per_cu)) void paged_attn_kernel(PagedArgs) {
   Args* const args = (Args*)(uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
   // Touch every line of the arguments up front: one wait instead of one for
@@ -1005,7 +1217,7 @@ __global__ __launch_bounds__(kThreads, (Shape<T, D, RWO>::per_cu)) void paged_at
     if (a.pre.splits) {
       n_pre = uint32_t(a.Hkv) * (uint32_t(a.B * a.R + 32 * RWP - 1) / (32 * RWP)) * uint32_t(a.pre.splits);
       if (w < n_pre) {
-        run_line<T, D, RWP, true, true>(args, smem, w, n_pre, 0, 0);
+        run_line<T, D, RWP, true, true, M>(args, smem, w, n_pre, 0, 0);
         return;
       }
     } else {
@@ -1036,7 +1248,7 @@ __global__ __launch_bounds__(kThreads, (Shape<T, D, RWO>::per_cu)) void paged_at
       }
       n_pre = uniform(n_pre);
       if (w < n_pre) {
-        run_line<T, D, RWP, true, true>(args, smem, in_runs(w, n_pre), n_pre, pre_total, 0);
+        run_line<T, D, RWP, true, true, M>(args, smem, in_runs(w, n_pre), n_pre, pre_total, 0);
         return;
       }
     }
@@ -1048,7 +1260,7 @@ __global__ __launch_bounds__(kThreads, (Shape<T, D, RWO>::per_cu)) void paged_at
     return;
   }
   if (a.own.splits == 0) w = in_runs(w, n_own);
-  run_line<T, D, RWO, false, (RWP > 0)>(args, smem, w, n_own, own.total, own.fresh);
+  run_line<T, D, RWO, false, (RWP > 0), M>(args, smem, w, n_own, own.total, own.fresh);
 }
 
 // Join the parts of 8 rows of an item, 64 of their values (blockIdx.z): a lane
@@ -1058,7 +1270,7 @@ __global__ __launch_bounds__(kThreads, (Shape<T, D, RWO>::per_cu)) void paged_at
 // TB/s; by its latency, 4-5 us, for decoded tokens.
 // blockIdx.x is a record. Prefix items are over all sequences' rows, so the rows
 // here may be those of two. A part that saw nothing has l = 0.
-template <typename T, int D, int RWP, int RWO>
+template <typename T, int D, int RWP, int RWO, Mode M>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
   __shared__ f32x4 sums[3][64][2];
   __shared__ f32x2 stats[3][64];
@@ -1150,6 +1362,8 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
   for (int x = 0; x < 3; ++x) add(stats[x][lane], sums[x][lane], ref);
   const float inv = 1.0f / l;  // no visible key: 0 * inf = NaN
   const int qi = int(uint32_t(row) / uint32_t(a.group)), hq = hk * a.group + row - qi * a.group;
+  if constexpr (M != kPlain)
+    if (a.lse && ch == 0) a.lse[(int64_t(b) * a.Lq + qi) * a.H + hq] = log_sum(m, l);
   char* const op = a.out + b * a.o_sb + qi * a.o_sl + hq * a.o_sh + 8 * ch * Elem<T>::bytes;
   if constexpr (Elem<T>::bytes == 4) {
     reinterpret_cast<f32x4*>(op)[0] = o[0] * inv;
@@ -1161,28 +1375,28 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
   }
 }
 
-template <typename T, int D, int RWP, int RWO>
+template <typename T, int D, int RWP, int RWO, Mode M>
 hipError_t launch_form(const PagedArgs& a, const PagedPlan& p, hipStream_t st) {
   constexpr int lds_own = Shape<T, D, RWO>::lds, lds_pre = RWP ? Shape<T, D, RWP ? RWP : 1>::lds : 0;
   constexpr int lds = lds_own > lds_pre ? lds_own : lds_pre;
-  const void* fn = reinterpret_cast<const void*>(&paged_attn_kernel<T, D, RWP, RWO>);
+  const void* fn = reinterpret_cast<const void*>(&paged_attn_kernel<T, D, RWP, RWO, M>);
   hipError_t e = opt_in_lds(fn, lds);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((paged_attn_kernel<T, D, RWP, RWO>), dim3(unsigned(p.grid)), dim3(kThreads), lds,
+  hipLaunchKernelGGL((paged_attn_kernel<T, D, RWP, RWO, M>), dim3(unsigned(p.grid)), dim3(kThreads), lds,
                      st, a);
   e = hipGetLastError();
   if (e != hipSuccess || !p.merge) return e;
-  hipLaunchKernelGGL((paged_merge_kernel<T, D, RWP, RWO>), dim3(unsigned(p.own_recs), 4 * RWO, D / 64),
+  hipLaunchKernelGGL((paged_merge_kernel<T, D, RWP, RWO, M>), dim3(unsigned(p.own_recs), 4 * RWO, D / 64),
                      dim3(256), 0, st, a);
   return hipGetLastError();
 }
 
-template <typename T, int D>
+template <typename T, int D, Mode M>
 hipError_t launch_paged(const PagedArgs& a, const PagedPlan& p, hipStream_t st) {
   if (p.rw_pre == 0)
-    return p.rw_own == 1 ? launch_form<T, D, 0, 1>(a, p, st) : launch_form<T, D, 0, 4>(a, p, st);
-  if (p.rw_pre == 1) return launch_form<T, D, 1, 1>(a, p, st);
-  return p.rw_own == 1 ? launch_form<T, D, 4, 1>(a, p, st) : launch_form<T, D, 4, 4>(a, p, st);
+    return p.rw_own == 1 ? launch_form<T, D, 0, 1, M>(a, p, st) : launch_form<T, D, 0, 4, M>(a, p, st);
+  if (p.rw_pre == 1) return launch_form<T, D, 1, 1, M>(a, p, st);
+  return p.rw_own == 1 ? launch_form<T, D, 4, 1, M>(a, p, st) : launch_form<T, D, 4, 4, M>(a, p, st);
 }
 
 }  // namespace

@@ -33,6 +33,15 @@ and calls it, exactly as dexter's dispatchers do (``python/dexter/ops/__init__.p
   (no counterpart in the reference, whose cache is one contiguous history per
   sequence, ``models/dreamzero/model.py:35-65``: a cache in pages that
   sequences can share, and attention over it)
+* ``kv_page_append_fp4``         -> ``select("cache", "page_append_fp4", pages, k, v)``,
+  ``kv_page_read_fp4``           -> ``select("cache", "page_read_fp4", pages, ...)``,
+  ``paged_attention_fp4``        -> ``select("attention", "paged_fp4", q, k, v)``,
+  ``shared_prefix_attention_fp4`` -> ``select("attention", "shared_prefix_fp4", q, k, v)``
+  (no counterpart: the same cache with its rows in 4 bits)
+* ``paged_key_weights``          -> ``select("cache", "key_weights", q, lse, weights, pages)``,
+  ``kv_keep_rows``               -> ``select("cache", "keep_rows", weights)``,
+  ``kv_page_gather``             -> ``select("cache", "page_gather", pages, rows)``
+  (no counterpart: a cache that keeps the rows which attention weighs most)
 
 Importing this module registers the gfx950 HIP kernels. Nothing else is
 registered, so on a machine without an MI355X every call raises
@@ -51,7 +60,9 @@ __all__ = ["qk_norm_rope", "blockwise_causal_attention", "kv_cache_append",
            "qk_norm_rope_append", "blockwise_causal_attention_varlen",
            "adaln_modulate", "gated_residual", "qkv_norm_rope", "qk_norm_rope_attention",
            "linear_chunk", "kv_page_append", "kv_page_copy", "paged_attention",
-           "shared_prefix_attention"]
+           "shared_prefix_attention", "kv_page_append_fp4", "kv_page_read_fp4",
+           "paged_attention_fp4", "shared_prefix_attention_fp4", "paged_key_weights",
+           "kv_keep_rows", "kv_page_gather"]
 
 
 def qkv_norm_rope(
@@ -290,7 +301,8 @@ def paged_attention(
     block_boundaries: torch.Tensor | None = None,
     softmax_scale: float | None = None,
     causal: bool = False,
-) -> torch.Tensor:
+    return_lse: bool = False,
+) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
     """``blockwise_causal_attention`` with each sequence's cached rows in pages.
 
     Sequence ``b`` attends to rows ``[0, cache_lens[b])`` of its pages (``block_table``
@@ -302,9 +314,16 @@ def paged_attention(
     seen (a sequence may drop pages of its history), and a graph captured once follows
     both. A narrower ``block_table[:, :w]`` plans the launch for fewer rows. A query
     that sees no key gives NaN, as in ``blockwise_causal_attention``.
+
+    With ``return_lse`` also each query's log-sum-exp, fp32 ``[B, L, H]``: ``ln`` of the
+    sum of ``exp(softmax_scale * q.k)`` over the keys it sees, ``-inf`` where it sees none
+    (``paged_key_weights`` takes it). In 16 bits the result's last bits may then differ:
+    the weights are divided by a sum of what they were before their rounding.
     """
-    return select("attention", "paged", q, k, v)(
-        q, k, v, pages, block_table, cache_lens, block_boundaries, softmax_scale, causal)
+    impl = select("attention", "paged", q, k, v)
+    more = {"return_lse": True} if return_lse else {}
+    return impl(q, k, v, pages, block_table, cache_lens, block_boundaries, softmax_scale, causal,
+                **more)
 
 
 def shared_prefix_attention(
@@ -320,7 +339,8 @@ def shared_prefix_attention(
     block_boundaries: torch.Tensor | None = None,
     softmax_scale: float | None = None,
     causal: bool = False,
-) -> torch.Tensor:
+    return_lse: bool = False,
+) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
     """``paged_attention`` for a batch that shares a prefix, computed once for all.
 
     Every sequence attends to rows ``[0, prefix_len)`` of the pages ``prefix_table``
@@ -330,9 +350,132 @@ def shared_prefix_attention(
     sequence's own (when the prefix fills its pages), but its keys and values are read
     once for all queries of the batch instead of once per sequence.
     """
-    return select("attention", "shared_prefix", q, k, v)(
+    impl = select("attention", "shared_prefix", q, k, v)
+    more = {"return_lse": True} if return_lse else {}
+    return impl(q, k, v, pages, prefix_table, prefix_len, block_table, cache_lens, block_boundaries,
+                softmax_scale, causal, **more)
+
+
+def kv_page_append_fp4(pages: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                       block_table: torch.Tensor, starts: torch.Tensor,
+                       status: torch.Tensor | None = None) -> None:
+    """``kv_page_append`` into pages in 4 bits, ``pages`` uint8 ``[2, P, H, R * (D/2 + D/32)]``.
+
+    Of each page and head first ``R`` rows of ``D/2`` code bytes (element ``2 i`` in the low
+    half of byte ``i``), then ``R`` rows of ``D/32`` scale bytes. A code is a sign and one of
+    0, 0.5, 1, 1.5, 2, 3, 4, 6; 32 elements share a scale ``2**(byte - 127)``, ``2**e`` for the
+    least ``e`` with all of them within ``7 * 2**e`` (``-127 <= e <= 125`` for bf16, ``-23 <=
+    e <= 13`` for f16), and are rounded to the nearest code, ties to even. A block that holds
+    an infinity or NaN reads as NaN (scale byte 255). ``k`` and ``v`` are bf16 or f16 with a
+    head dim of 64, 128 or 256; ``R`` is a multiple of 16 up to 1024. Rows without a page and
+    ``status`` as in ``kv_page_append``.
+    """
+    return select("cache", "page_append_fp4", pages, k, v)(pages, k, v, block_table, starts, status)
+
+
+def kv_page_read_fp4(pages: torch.Tensor, block_table: torch.Tensor, starts: torch.Tensor, n: int,
+                     head_dim: int, dtype: torch.dtype = torch.bfloat16,
+                     status: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows ``[starts[b], starts[b] + n)`` of pages in 4 bits as new ``k``, ``v`` ``[B, n, H, D]``
+    of ``dtype`` (bf16 or f16; exact where it is the type that the rows were written from).
+
+    A row without a page becomes zeros, and ``status`` (one int32, optional) 1.
+    """
+    return select("cache", "page_read_fp4", pages, block_table, starts, n, head_dim, dtype)(
+        pages, block_table, starts, n, head_dim, dtype, status)
+
+
+def paged_attention_fp4(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    *,
+    pages: torch.Tensor,
+    block_table: torch.Tensor,
+    cache_lens: torch.Tensor,
+    block_boundaries: torch.Tensor | None = None,
+    softmax_scale: float | None = None,
+    causal: bool = False,
+    return_lse: bool = False,
+) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
+    """``paged_attention`` with the cached rows in 4 bits (``pages`` as ``kv_page_append_fp4``
+    has them); ``q`` and the chunk's own ``k``/``v`` are bf16 or f16. The cached values are
+    exact in that type: what they lost they lost when they were written."""
+    return select("attention", "paged_fp4", q, k, v)(
+        q, k, v, pages, block_table, cache_lens, block_boundaries, softmax_scale, causal, return_lse)
+
+
+def shared_prefix_attention_fp4(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    *,
+    pages: torch.Tensor,
+    prefix_table: torch.Tensor,
+    prefix_len: torch.Tensor,
+    block_table: torch.Tensor | None = None,
+    cache_lens: torch.Tensor | None = None,
+    block_boundaries: torch.Tensor | None = None,
+    softmax_scale: float | None = None,
+    causal: bool = False,
+    return_lse: bool = False,
+) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
+    """``shared_prefix_attention`` with the prefix and the cached rows in 4 bits."""
+    return select("attention", "shared_prefix_fp4", q, k, v)(
         q, k, v, pages, prefix_table, prefix_len, block_table, cache_lens, block_boundaries,
-        softmax_scale, causal)
+        softmax_scale, causal, return_lse)
+
+
+def paged_key_weights(
+    q: torch.Tensor,
+    lse: torch.Tensor,
+    weights: torch.Tensor | None = None,
+    *,
+    pages: torch.Tensor,
+    block_table: torch.Tensor,
+    cache_lens: torch.Tensor,
+    softmax_scale: float | None = None,
+) -> torch.Tensor:
+    """The softmax weight that each cached row received from ``q`` ``[B, L, H, D]``, with the
+    ``lse`` ``[B, L, H]`` that attention returned for it: ``[B, Hkv, W * R]``, fp32, summed over
+    the queries and the query heads of a K/V head.
+
+    Row ``r`` of sequence ``b`` gets the sum of ``exp(softmax_scale * q.k_r - lse)``. Rows past
+    ``cache_lens[b]`` and rows without a page get 0. ``weights``, when given, is added to in
+    place and returned (such rows keep what they have): over the steps of an episode it
+    accumulates. A query whose ``lse`` is ``-inf`` gives nothing. ``pages`` are a pool of q's
+    type (16 bits, or fp32) or one in 4 bits. Every bit is the same from call to call.
+    """
+    return select("cache", "key_weights", q, lse, weights, pages)(
+        q, lse, weights, pages, block_table, cache_lens, softmax_scale)
+
+
+def kv_keep_rows(weights: torch.Tensor, cache_lens: torch.Tensor, keep: int,
+                 recent: int = 0) -> torch.Tensor:
+    """Which rows to keep, by the ``weights`` ``[B, H, N]`` that they received: int32 row numbers
+    ``[B, H, keep]``, ascending, then -1.
+
+    Of the ``n = min(cache_lens[b], N)`` rows of sequence ``b``, ``c = min(n, keep)``: the last
+    ``min(recent, c)`` and those with the largest weights before them; of equal ones the
+    lowest, and NaN counts as ``-inf``.
+    """
+    return select("cache", "keep_rows", weights)(weights, cache_lens, keep, recent)
+
+
+def kv_page_gather(pages: torch.Tensor, block_table: torch.Tensor, rows: torch.Tensor,
+                   dst_table: torch.Tensor | None = None, weights: torch.Tensor | None = None,
+                   head_dim: int | None = None) -> None:
+    """Row ``rows[b, h, i]`` of head ``h`` of sequence ``b``'s pages becomes row ``i`` of the pages
+    ``dst_table`` names (default: ``block_table``'s own, in place), in both planes; ``weights``
+    ``[B, H, N]`` move with their rows and are 0 behind them.
+
+    ``rows`` is what ``kv_keep_rows`` returned: in place it has to be ascending with ``rows[b,
+    h, i] >= i``. Entries below 0, past a table or without a page move nothing. Pages that
+    ``dst_table`` names and ``block_table`` does not at the same place must not be read by any
+    sequence of the call. ``head_dim`` is needed for pages in 4 bits.
+    """
+    return select("cache", "page_gather", pages, rows)(pages, block_table, rows, dst_table, weights,
+                                                       head_dim)
 
 
 # Importing the implementation package is what populates the registry.

@@ -17,10 +17,10 @@ import torch
 
 LIB_NAME = "libdexter_gfx950.so"
 LIB_PATH = Path(__file__).resolve().parents[2] / LIB_NAME
-ABI_VERSION = 13
+ABI_VERSION = 14
 
 DX_OK, DX_EINVAL, DX_ELAUNCH, DX_EFULL, DX_EWORKSPACE = 0, 1, 2, 3, 4
-DX_BF16, DX_F16, DX_F32, DX_I32, DX_I64 = 0, 1, 2, 3, 4
+DX_BF16, DX_F16, DX_F32, DX_I32, DX_I64, DX_FP4 = 0, 1, 2, 3, 4, 5
 # dx_set_tuning keys (launch-schedule overrides for measurement and tests).
 (TUNE_ATTN_SPLITS, TUNE_ATTN_KERNEL, TUNE_NORM_WAVES, TUNE_QKV_SPLITS, TUNE_QKV_WAVES,
  TUNE_ATTN_MERGE, TUNE_ATTN_PMERGE) = range(7)
@@ -176,6 +176,34 @@ _SIGNATURES: dict[str, tuple[type, list]] = {
         _l, _l, _i, _l]),          # rows per page, table width, has prefix, prefix width
     "dx_paged_attention": (_i, [_p]),          # a packed dx_paged_call (PAGED_CALL)
     "dx_shared_prefix_attention": (_i, [_p]),
+    "dx_paged_attention_lse": (_i, [_p, _p]),  # call, lse
+    "dx_shared_prefix_attention_lse": (_i, [_p, _p]),
+    "dx_paged_attention_fp4": (_i, [_p, _p]),
+    "dx_shared_prefix_attention_fp4": (_i, [_p, _p]),
+    "dx_kv_page_append_fp4": (_i, [
+        _p, _l, _l, _l,            # k
+        _p, _l, _l, _l,            # v
+        _p, _l, _l, _l,            # pages, plane, page, head strides (bytes)
+        _i, _l, _l,                # dtype, pages, rows per page
+        _p, _l, _l, _p, _p,        # block table, its row stride, width, starts, status
+        _l, _l, _l, _l, _p]),      # B, n, H, D, stream
+    "dx_kv_page_read_fp4": (_i, [
+        _p, _l, _l, _l,            # pages, plane, page, head strides (bytes)
+        _i, _l, _l,                # dtype, pages, rows per page
+        _p, _l, _l, _p, _p,        # block table, its row stride, width, starts, status
+        _p, _p,                    # k, v
+        _l, _l, _l, _l, _p]),      # B, n, H, D, stream
+    "dx_paged_key_weights": (_i, [_p]),        # a packed dx_weights_call (WEIGHTS_CALL)
+    "dx_kv_keep_rows": (_i, [
+        _p, _l, _l, _l, _p,        # weights, strides, width, lens
+        _l, _l, _p, _l, _l, _p]),  # keep, recent, rows, B, H, stream
+    "dx_kv_page_gather": (_i, [
+        _p, _l, _l, _l, _l,        # pages, plane, page, row, head strides
+        _i, _l, _l,                # dtype, pages, rows per page
+        _p, _l, _l, _p, _l, _l,    # source and destination tables: row stride, width
+        _p, _l,                    # rows, keep
+        _p, _l, _l, _l,            # weights, strides, width
+        _l, _l, _l, _p]),          # B, H, D, stream
     "dx_adaln_modulate": (_i, [
         _p, _l, _l, _i,            # x, sb, sl, x dtype
         _p, _l, _l,                # scale, sb, sl
@@ -201,6 +229,16 @@ PAGED_CALL = struct.Struct(
     "7q"         # dtype, B, Lq, Lk, H, Hkv, D
     "3qqd"       # starts, starts dtype, n_blocks; causal; scale
     "2qq")       # workspace, bytes; stream
+
+# struct dx_weights_call, likewise.
+WEIGHTS_CALL = struct.Struct(
+    "="
+    "4qq"        # q: pointer, batch, row, head strides; lse
+    "6q"         # pages, page, row, head strides, pages, rows per page
+    "3qq"        # block table, its row stride, width; cache lengths
+    "3q"         # weights, batch, head strides
+    "7q"         # dtype, fp4, B, Lq, H, Hkv, D
+    "qdq")       # add; scale; stream
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None

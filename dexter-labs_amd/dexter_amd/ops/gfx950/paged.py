@@ -39,7 +39,7 @@ import torch
 
 from ...registry import Priority, register
 from . import _lib
-from ._common import CDNA4, strides
+from ._common import CDNA4, MATRIX_DTYPES, strides
 from .attention import _starts
 
 _APPEND_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
@@ -47,6 +47,7 @@ _APPEND_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 _HEAD_DIMS = {torch.bfloat16: (64, 128, 256), torch.float16: (64, 128, 256),
               torch.float32: (64, 128)}
 PAGE_ROWS_MULTIPLE, PAGE_ROWS_MAX = 16, 1024
+FP4_HEAD_DIMS = (64, 128, 256)
 
 
 def _on(device: torch.device):
@@ -210,8 +211,28 @@ def _workspace_bytes(device_index, code, b, q_len, kv_len, heads, kv_heads, dim,
     return n
 
 
+def _fp4_rows(pages: torch.Tensor, dim: int, what: str) -> int:
+    """Rows of a page of a 4-bit pool, whose heads' blocks the kernels can read in place."""
+    if dim not in FP4_HEAD_DIMS:
+        raise ValueError(f"{what}: head_dim {dim} (a 4-bit cache takes {FP4_HEAD_DIMS})")
+    shape, steps, row = pages.shape, pages.stride(), dim // 2 + dim // 32
+    if pages.dtype is not torch.uint8 or len(shape) != 4 or shape[0] != 2:
+        raise ValueError(f"{what}: pages in 4 bits must be uint8 [2, P, H, R * {row}], got "
+                         f"{pages.dtype} {tuple(shape)}")
+    rows, rest = divmod(shape[3], row)
+    if rest or rows == 0 or rows % PAGE_ROWS_MULTIPLE or rows > PAGE_ROWS_MAX or shape[2] == 0:
+        raise ValueError(f"{what}: pages {tuple(shape)} are not R * {row} bytes of a head with R a "
+                         f"multiple of {PAGE_ROWS_MULTIPLE} up to {PAGE_ROWS_MAX}")
+    s0, s1, s2, s3 = steps
+    if s3 != 1 or pages.data_ptr() % 16 or (s0 | s1 | s2) % 16:
+        raise ValueError(f"{what}: pages must have contiguous, 16-byte aligned heads")
+    if not (s0 and (s1 or shape[1] <= 1) and (s2 or shape[2] == 1)):
+        raise ValueError(f"{what}: pages must not be expanded (a stride is 0)")
+    return rows
+
+
 def _attend(what, q, k, v, pages, prefix, block_table, cache_lens, block_boundaries,
-            softmax_scale, causal):
+            softmax_scale, causal, return_lse=False, fp4=False):
     """``prefix``: None, or (prefix_table, prefix_len)."""
     if q.dim() != 4 or k.shape != v.shape or k.dim() != 4:
         raise ValueError("q, k, v must be [B, L, H, D] with k and v of one shape")
@@ -226,11 +247,20 @@ def _attend(what, q, k, v, pages, prefix, block_table, cache_lens, block_boundar
     if kv_len != q_len and (block_boundaries is not None or causal):
         raise ValueError(f"k/v length {kv_len} must equal q length {q_len} with block_boundaries "
                          "or causal")
-    s0, s1, s2, s3, _ = _check_pool(pages, what)
-    _, n_pages, rows, p_heads, p_dim = pages.shape
-    if p_heads != kv_heads or p_dim != dim or pages.dtype is not dtype:
-        raise ValueError(f"pages must be [2, P, R, {kv_heads}, {dim}] of {dtype}, got "
-                         f"{tuple(pages.shape)} of {pages.dtype}")
+    if fp4:
+        if dtype not in MATRIX_DTYPES:
+            raise ValueError(f"{what}: a 4-bit cache serves bf16 and f16, got {dtype}")
+        rows = _fp4_rows(pages, dim, what)
+        (s0, s1, s3, _), s2 = pages.stride(), 0
+        n_pages = pages.shape[1]
+        if pages.shape[2] != kv_heads:
+            raise ValueError(f"{what}: pages of {pages.shape[2]} heads for {kv_heads} k/v heads")
+    else:
+        s0, s1, s2, s3, _ = _check_pool(pages, what)
+        _, n_pages, rows, p_heads, p_dim = pages.shape
+        if p_heads != kv_heads or p_dim != dim or pages.dtype is not dtype:
+            raise ValueError(f"pages must be [2, P, R, {kv_heads}, {dim}] of {dtype}, got "
+                             f"{tuple(pages.shape)} of {pages.dtype}")
     if rows % PAGE_ROWS_MULTIPLE or rows > PAGE_ROWS_MAX:
         raise ValueError(f"attention takes pages of a multiple of {PAGE_ROWS_MULTIPLE} rows up to "
                          f"{PAGE_ROWS_MAX}, got {rows}")
@@ -255,10 +285,11 @@ def _attend(what, q, k, v, pages, prefix, block_table, cache_lens, block_boundar
     if _elsewhere(device):
         with _on(device):
             return _attend(what, q, k, v, pages, prefix, block_table, cache_lens, block_boundaries,
-                           softmax_scale, causal)
+                           softmax_scale, causal, return_lse, fp4)
     out = torch.empty((b, q_len, heads, dim), device=device, dtype=dtype)
+    lse = torch.empty((b, q_len, heads), device=device) if return_lse else None
     if b == 0 or q_len == 0:
-        return out
+        return (out, lse) if return_lse else out
     scale = float(softmax_scale) if softmax_scale is not None else 1.0 / math.sqrt(dim)
     q, *q_at = _rows(q)
     k, *k_at = _rows(k)
@@ -281,23 +312,30 @@ def _attend(what, q, k, v, pages, prefix, block_table, cache_lens, block_boundar
         starts_ptr, starts_dt, n_blocks, 1 if causal else 0, scale,
         0 if ws is None else ws.data_ptr(), ws_bytes, _lib.stream_handle(device))
     lib = _lib.load()
-    rc = (lib.dx_paged_attention if prefix is None else lib.dx_shared_prefix_attention)(call)
+    if fp4:
+        entry = lib.dx_paged_attention_fp4 if prefix is None else lib.dx_shared_prefix_attention_fp4
+        rc = entry(call, _lib.ptr(lse))
+    elif return_lse:
+        entry = lib.dx_paged_attention_lse if prefix is None else lib.dx_shared_prefix_attention_lse
+        rc = entry(call, lse.data_ptr())
+    else:
+        rc = (lib.dx_paged_attention if prefix is None else lib.dx_shared_prefix_attention)(call)
     if rc:
         _lib.check(rc, what)
-    return out
+    return (out, lse) if return_lse else out
 
 
 @register("attention", "paged", name="hip_paged_attention_gfx950",
           capability=CDNA4, priority=Priority.SPECIALISED, accepts=_attn_accepts)
 def paged_attention(q, k, v, pages, block_table, cache_lens, block_boundaries, softmax_scale,
-                    causal=False):
+                    causal=False, return_lse=False):
     return _attend("paged_attention", q, k, v, pages, None, block_table, cache_lens,
-                   block_boundaries, softmax_scale, causal)
+                   block_boundaries, softmax_scale, causal, return_lse)
 
 
 @register("attention", "shared_prefix", name="hip_shared_prefix_attention_gfx950",
           capability=CDNA4, priority=Priority.SPECIALISED, accepts=_attn_accepts)
 def shared_prefix_attention(q, k, v, pages, prefix_table, prefix_len, block_table, cache_lens,
-                            block_boundaries, softmax_scale, causal=False):
+                            block_boundaries, softmax_scale, causal=False, return_lse=False):
     return _attend("shared_prefix_attention", q, k, v, pages, (prefix_table, prefix_len),
-                   block_table, cache_lens, block_boundaries, softmax_scale, causal)
+                   block_table, cache_lens, block_boundaries, softmax_scale, causal, return_lse)

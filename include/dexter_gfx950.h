@@ -45,13 +45,20 @@
  *                            no counterpart (the reference's cache is one
  *                            contiguous history per sequence,
  *                            models/dreamzero/model.py:35-65)
+ *   dx_kv_page_append_fp4, dx_kv_page_read_fp4, dx_paged_attention_fp4,
+ *   dx_shared_prefix_attention_fp4
+ *                            the same with the cache in 4 bits (no counterpart)
+ *   dx_paged_attention_lse, dx_shared_prefix_attention_lse, dx_paged_key_weights,
+ *   dx_kv_keep_rows, dx_kv_page_gather
+ *                            a cache that keeps the rows which attention weighs
+ *                            most (no counterpart)
  *
  * Conventions
  *  - Tensors are device pointers with explicit element strides; the last
  *    (head_dim) dimension must be contiguous. [B, L, H, D] tensors take
  *    strides (sb, sl, sh). A KV cache [2, B, S, H, D] takes (plane, sb, ss, sh):
  *    plane 0 holds K, plane 1 holds V.
- *  - dtype codes: DX_BF16, DX_F16, DX_F32.
+ *  - dtype codes: DX_BF16, DX_F16, DX_F32; of a pool in 4 bits, DX_FP4.
  *  - stream is a hipStream_t (NULL = the legacy default stream). Every entry
  *    point only enqueues work: no allocation, no host synchronisation, so the
  *    calls are safe under HIP graph capture. Functions are re-entrant and may
@@ -79,13 +86,14 @@ extern "C" {
 #define DX_F32 2
 #define DX_I32 3
 #define DX_I64 4
+#define DX_FP4 5
 
 /* Message for the calling thread's last failed call ("" if none). */
 const char* dx_last_error(void);
 
 /* ABI revision of this header; the Python loader checks it. */
 int dx_abi_version(void);
-#define DX_ABI_VERSION 13
+#define DX_ABI_VERSION 14
 
 /*
  * Launch-schedule overrides, for measurement and tests only: process-wide,
@@ -560,6 +568,115 @@ int dx_shared_prefix_attention(const dx_paged_call* call);
 int64_t dx_paged_attention_workspace_bytes(int dtype, int64_t B, int64_t Lq, int64_t Lk, int64_t H,
                                            int64_t Hkv, int64_t D, int64_t page_rows,
                                            int64_t width, int has_prefix, int64_t prefix_width);
+
+/*
+ * dx_paged_attention and dx_shared_prefix_attention that also write each query's
+ * log-sum-exp: lse (float [B, Lq, H], contiguous, not NULL) = ln of the sum of
+ * exp(scale q.k) over the keys it sees, -inf where it sees none. In 16 bits the
+ * weights are divided by the sum of the probabilities as they were before their
+ * rounding, so out may differ from the other entry points' in its last bits.
+ * Workspace as theirs.
+ */
+int dx_paged_attention_lse(const dx_paged_call* call, void* lse);
+int dx_shared_prefix_attention_lse(const dx_paged_call* call, void* lse);
+
+/*
+ * A KV cache's pages in 4 bits. A pool is bytes [2, n_pages, H, page_rows *
+ * (D / 2 + D / 32)] through byte strides (p_plane, p_sp per page, p_sh per head;
+ * multiples of 16): of each page and head first page_rows rows of D / 2 code
+ * bytes (element 2 i in the low half of byte i), then as many of D / 32 scale
+ * bytes. A code is a sign bit and an E2M1 number (0, 0.5, 1, 1.5, 2, 3, 4, 6);
+ * 32 consecutive ones share the scale 2^(byte - 127), and 255 makes them NaN.
+ * D is 64, 128 or 256, page_rows a multiple of 16 up to 1024. Tables, lengths and
+ * start rows as above.
+ *
+ * Append: each block is stored with the least scale 2^e for which 7 * 2^e is at
+ * least its largest magnitude (e in [-127, 125] for DX_BF16, [-23, 13] for
+ * DX_F16), its elements as the nearest codes, ties to even; a block that holds an
+ * infinity or NaN reads as NaN. Rows without a page and *status: as
+ * dx_kv_page_append.
+ *
+ * Read: rows starts[b] + t to k and v [B, n, H, D] of dtype, contiguous. Exact
+ * where the type holds the values, as it does for rows that were appended in it.
+ * Rows without a page become zeros, and *status (may be NULL) 1.
+ */
+int dx_kv_page_append_fp4(const void* k, int64_t k_sb, int64_t k_sl, int64_t k_sh,
+                          const void* v, int64_t v_sb, int64_t v_sl, int64_t v_sh,
+                          void* pages, int64_t p_plane, int64_t p_sp, int64_t p_sh,
+                          int dtype, int64_t n_pages, int64_t page_rows,
+                          const void* block_table, int64_t t_sb, int64_t width,
+                          const void* starts, void* status,
+                          int64_t B, int64_t n, int64_t H, int64_t D, void* stream);
+int dx_kv_page_read_fp4(const void* pages, int64_t p_plane, int64_t p_sp, int64_t p_sh,
+                        int dtype, int64_t n_pages, int64_t page_rows,
+                        const void* block_table, int64_t t_sb, int64_t width,
+                        const void* starts, void* status, void* k, void* v,
+                        int64_t B, int64_t n, int64_t H, int64_t D, void* stream);
+
+/*
+ * dx_paged_attention_lse and dx_shared_prefix_attention_lse with the cached rows
+ * (and the prefix) in a 4-bit pool: pages, p_plane, p_sp and p_sh of the call are
+ * its bytes and byte strides, p_sr is not read; q, k, v and out are of dtype,
+ * DX_BF16 or DX_F16. lse may be NULL. The rows' values are exact in dtype and
+ * enter the products as they are. Workspace as theirs.
+ */
+int dx_paged_attention_fp4(const dx_paged_call* call, void* lse);
+int dx_shared_prefix_attention_fp4(const dx_paged_call* call, void* lse);
+
+/*
+ * A call of dx_paged_key_weights; every field 8 bytes wide, as dx_paged_call.
+ * pages is a pool of dtype (strides in elements) or, with fp4, a 4-bit one (byte
+ * strides, p_sr not read).
+ */
+typedef struct dx_weights_call {
+  const void* q; int64_t q_sb, q_sl, q_sh;          /* [B, Lq, H, D] */
+  const void* lse;                                  /* float [B, Lq, H] */
+  const void* pages; int64_t p_sp, p_sr, p_sh, n_pages, page_rows;  /* plane 0 */
+  const void* block_table; int64_t t_sb, width;
+  const void* cache_lens;
+  void* weights; int64_t w_sb, w_sh;                /* float [B, Hkv, width * page_rows] */
+  int64_t dtype, fp4, B, Lq, H, Hkv, D;
+  int64_t add;
+  double softmax_scale;
+  void* stream;
+} dx_weights_call;
+
+/*
+ * The softmax weight that each cached row received: weights[b][hk][r] = (with add:
+ * +=) the sum over the sequence's queries t and the heads h of K/V head hk of
+ * exp(scale q[b][t][h].k[r] - lse[b][t][h]), for r < cache_lens[b]; fp32, summed in
+ * one order. Rows that a table entry gives no page, and rows past a length,
+ * receive 0 (with add they are left as they are). A query whose lse is -inf gives
+ * nothing. No workspace.
+ */
+int dx_paged_key_weights(const dx_weights_call* call);
+
+/*
+ * Which rows to keep. Of sequence b's n = lens[b] rows (clamped to [0, width]),
+ * per head: the last min(recent, c) of them and the c - min(recent, c) others with
+ * the largest weights[b][h] (float [B, H, width]), c = min(n, keep); of equal ones
+ * the lowest rows, and NaN counts as -inf. rows (int32 [B, H, keep]): their
+ * numbers in order, then -1. No workspace.
+ */
+int dx_kv_keep_rows(const void* weights, int64_t w_sb, int64_t w_sh, int64_t width,
+                    const void* lens, int64_t keep, int64_t recent, void* rows,
+                    int64_t B, int64_t H, void* stream);
+
+/*
+ * Row i of sequence b's head h in the pages dst_table becomes row rows[b][h][i]
+ * (int32 [B, H, keep], contiguous) of the pages src_table, in both planes; entries
+ * that are negative, past a table or without a page move nothing. dst_table may
+ * name the source's own pages at their places, where rows[b][h][i] >= i and
+ * ascending (as dx_kv_keep_rows gives them), or pages that no sequence of the call
+ * reads. weights (float [B, H, w_width], may be NULL) move with their rows, and are 0
+ * behind them. dtype: the pool's, or DX_FP4 (byte strides, p_sr not read).
+ */
+int dx_kv_page_gather(void* pages, int64_t p_plane, int64_t p_sp, int64_t p_sr, int64_t p_sh,
+                      int dtype, int64_t n_pages, int64_t page_rows, const void* src_table,
+                      int64_t s_sb, int64_t width, const void* dst_table, int64_t d_sb,
+                      int64_t dst_width, const void* rows, int64_t keep, void* weights,
+                      int64_t w_sb, int64_t w_sh, int64_t w_width, int64_t B, int64_t H,
+                      int64_t D, void* stream);
 
 #ifdef __cplusplus
 }

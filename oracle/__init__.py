@@ -21,6 +21,9 @@ under ``python/dexter/`` of raikonenfnu/dexter-labs):
 * ``paged``      attention over a cache in pages and a shared prefix, from its
                  definition in fp64 (no counterpart in the reference), and the
                  error that an evaluation with fp32 sums may have.
+* ``fp4``        a cache's pages in 4 bits: codes, scales and what they stand for, and
+* ``keep``       the softmax weight of each cached row, which rows a cache keeps by it, and
+                 their move, from the definitions in fp64 (no counterparts in the reference).
 * ``brute``      fp64 brute force (numpy, explicit loops) of attention, the
                  prologue and the adaLN/gated-residual pair, written
                  independently of the torch restatements;
@@ -29,7 +32,7 @@ under ``python/dexter/`` of raikonenfnu/dexter-labs):
                  against closed forms.
 
 Pinning status: every function here is pinned (tests/test_oracle.py,
-tests/test_paged_oracle.py); none is
+tests/test_paged_oracle.py, tests/test_fp4_oracle.py, tests/test_keep_oracle.py); none is
 "parity unpinned". The reference ships no golden vectors for this path, so
 the pins are the fp64 brute force, a library routine and closed-form cases.
 """
