@@ -18,6 +18,14 @@ of page numbers and a length of its own:
   takes pages in every sequence, for a step writes them all.
 * ``free(seq)`` gives a sequence's pages back; ``compact()`` moves what is in use to
   the lowest page numbers.
+* ``fp4=True`` holds the rows in 4 bits (``kv_page_append_fp4``): 68 bytes of a head's row
+  of 128 where bf16 takes 256. ``dtype`` is then that of the rows written and of attention.
+* ``track_weights=True`` has ``attend`` add up the softmax weight that each row of a
+  sequence received (``paged_key_weights``; ``weights[layer]`` ``[batch, H, W * R]``), by which
+  ``evict(keep, recent)`` brings every longer sequence down to ``keep`` rows: the last
+  ``recent`` and the heaviest before them, each layer and head by its own weights. Rows carry
+  their positions in their rotated keys: the caller goes on counting positions from where
+  the sequence was, not from its new length. A prefix keeps all of its rows.
 
 Which page is whose is decided on the host, before anything is launched:
 ``reserve(n)`` finds pages for the next ``n`` rows of every sequence or raises
@@ -44,12 +52,19 @@ from .. import ops
 class PagedKVCache:
     def __init__(self, layers: int, batch: int, pages: int, page_rows: int, heads: int,
                  head_dim: int, device: torch.device | str, dtype: torch.dtype,
-                 max_rows: int | None = None) -> None:
+                 max_rows: int | None = None, fp4: bool = False,
+                 track_weights: bool = False) -> None:
         """``max_rows``: rows a sequence may hold (default: all pages); it sets the width of
         ``block_table``, for which attention launches are planned."""
         if page_rows <= 0 or page_rows % 16 or page_rows > 1024:
             raise ValueError(f"page_rows must be a multiple of 16 up to 1024, got {page_rows}")
-        self.pools = [torch.zeros(2, pages, page_rows, heads, head_dim, device=device, dtype=dtype)
+        if fp4 and (dtype not in (torch.bfloat16, torch.float16) or head_dim not in (64, 128, 256)):
+            raise ValueError(f"a cache in 4 bits serves bf16 and f16 at head dims 64, 128 and 256, got "
+                             f"{dtype} at {head_dim}")
+        self.fp4, self.dtype, self.head_dim = fp4, dtype, head_dim
+        shape = ((2, pages, heads, page_rows * (head_dim // 2 + head_dim // 32)) if fp4 else
+                 (2, pages, page_rows, heads, head_dim))
+        self.pools = [torch.zeros(shape, device=device, dtype=torch.uint8 if fp4 else dtype)
                       for _ in range(layers)]
         self.pages, self.page_rows, self.batch = pages, page_rows, batch
         self.width = pages if max_rows is None else -(-max_rows // page_rows)
@@ -65,6 +80,15 @@ class PagedKVCache:
         self.prefix_table = torch.full((self.width,), -1, **i32)
         self.prefix_len = torch.zeros(1, **i32)
         self.status = torch.zeros(1, **i32)
+        # What the rows received: of every layer, a sequence's tail behind its length is 0.
+        self.weights = (torch.zeros(layers, batch, heads, self.width * page_rows, device=device)
+                        if track_weights else None)
+
+    def _copy_pages(self, src: list[int], dst: list[int]) -> None:
+        pools = self.pools
+        if self.fp4:  # a page's bytes, as rows of 16-bit elements, one for each head
+            pools = [p.view(torch.bfloat16).unsqueeze(3) for p in pools]
+        ops.kv_page_copy(pools, src, dst)
 
     # -- pages ---------------------------------------------------------------
     @property
@@ -139,7 +163,7 @@ class PagedKVCache:
             while len(table) * self.page_rows < length + n:
                 table.append(next(new))
         if src:
-            ops.kv_page_copy(self.pools, src, dst)
+            self._copy_pages(src, dst)
         self._push_tables(tables)
         for _ in range(need):
             self._take()
@@ -154,7 +178,8 @@ class PagedKVCache:
         """Write one chunk's ``k``/``v`` ``[batch, n, H, D]`` for ``layer`` at each sequence's
         end (lengths unchanged)."""
         self.reserve(k.shape[1])
-        ops.kv_page_append(self.pools[layer], k, v, self.block_table, self.cache_lens, self.status)
+        write = ops.kv_page_append_fp4 if self.fp4 else ops.kv_page_append
+        write(self.pools[layer], k, v, self.block_table, self.cache_lens, self.status)
 
     def commit(self, n: int) -> None:
         """Move every sequence's end once every layer has appended its chunk."""
@@ -183,6 +208,8 @@ class PagedKVCache:
         self.tables[dst], self.lengths[dst] = table, length
         self._push_tables()
         self._push_lengths()
+        if self.weights is not None:
+            self.weights[:, dst] = self.weights[:, src]
 
     def free(self, seq: int) -> None:
         """Give a sequence's pages back; it starts again from nothing (and the prefix)."""
@@ -192,6 +219,8 @@ class PagedKVCache:
         self.tables[seq], self.lengths[seq] = [], 0
         self._push_tables()
         self._push_lengths()
+        if self.weights is not None:
+            self.weights[:, seq] = 0
 
     def hold_prefix(self, seq: int) -> None:
         """The history of ``seq`` (behind a prefix held already, whose last page has to be
@@ -216,6 +245,51 @@ class PagedKVCache:
         self._push_prefix()
         self._push_tables()
         self._push_lengths()
+        if self.weights is not None:
+            self.weights.zero_()
+
+    def evict(self, keep: int, recent: int = 0) -> int:
+        """Bring every sequence that holds more than ``keep`` rows down to ``keep``: its last
+        ``recent`` rows (at most ``keep``) and the heaviest before them, in their order, each
+        layer and head by its own weights. Returns how many sequences that was. Rows stay
+        where their pages are the sequence's alone; the others' go to new pages
+        (``RuntimeError`` with nothing changed when there are too few)."""
+        if self.weights is None:
+            raise RuntimeError("evict needs PagedKVCache(track_weights=True)")
+        if keep < 0 or recent < 0:
+            raise ValueError(f"cannot keep {keep} rows, {recent} of them the last")
+        self._outside_a_capture("evict")
+        long = [b for b, length in enumerate(self.lengths) if length > keep]
+        if not long:
+            return 0
+        count = -(-keep // self.page_rows)
+        need = sum(self._users[p] > 1 for b in long for p in self.tables[b][:count])
+        if need > len(self._free):
+            raise RuntimeError(f"KV cache full: {need} pages needed, {len(self._free)} of "
+                               f"{self.pages} free")
+        new = iter(heapq.nsmallest(need, self._free))
+        tables = [list(t) for t in self.tables]
+        for b in long:
+            tables[b] = [next(new) if self._users[p] > 1 else p for p in tables[b][:count]]
+        to = self.block_table
+        if need:
+            to = torch.tensor([t + [-1] * (self.width - len(t)) for t in tables], dtype=torch.int32)
+            to = to.to(self.block_table.device)
+        for pool, weights in zip(self.pools, self.weights):
+            rows = ops.kv_keep_rows(weights, self.cache_lens, keep, recent)
+            ops.kv_page_gather(pool, self.block_table, rows, to, weights, self.head_dim)
+        for _ in range(need):
+            self._take()
+        for b in long:
+            kept = set(tables[b])
+            for page in self.tables[b]:
+                if page not in kept:
+                    self._drop(page)
+            self.lengths[b] = keep
+        self.tables = tables
+        self._push_tables()
+        self._push_lengths()
+        return len(long)
 
     def _push_prefix(self) -> None:
         row = self.prefix + [-1] * (self.width - len(self.prefix))
@@ -232,7 +306,7 @@ class PagedKVCache:
         held = set(live)
         dst = [p for p in range(n) if p not in held]
         if src:
-            ops.kv_page_copy(self.pools, src, dst)
+            self._copy_pages(src, dst)
             new = dict(zip(src, dst))
             self.tables = [[new.get(p, p) for p in t] for t in self.tables]
             self.prefix = [new.get(p, p) for p in self.prefix]
@@ -253,6 +327,8 @@ class PagedKVCache:
         self._push_lengths()
         self._push_prefix()
         self.status.zero_()
+        if self.weights is not None:
+            self.weights.zero_()
 
     # -- attention -----------------------------------------------------------
     def attend(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -262,10 +338,17 @@ class PagedKVCache:
         kw = dict(pages=self.pools[layer], block_table=self.block_table,
                   cache_lens=self.cache_lens, block_boundaries=block_boundaries,
                   softmax_scale=softmax_scale, causal=causal)
-        if not self.prefix:
-            return ops.paged_attention(q, k, v, **kw)
-        return ops.shared_prefix_attention(q, k, v, prefix_table=self.prefix_table,
-                                           prefix_len=self.prefix_len, **kw)
+        attention = ops.paged_attention_fp4 if self.fp4 else ops.paged_attention
+        if self.prefix:
+            attention = ops.shared_prefix_attention_fp4 if self.fp4 else ops.shared_prefix_attention
+            kw.update(prefix_table=self.prefix_table, prefix_len=self.prefix_len)
+        if self.weights is None:
+            return attention(q, k, v, **kw)
+        out, lse = attention(q, k, v, return_lse=True, **kw)
+        ops.paged_key_weights(q, lse, self.weights[layer], pages=self.pools[layer],
+                              block_table=self.block_table, cache_lens=self.cache_lens,
+                              softmax_scale=softmax_scale)
+        return out
 
     def overflowed(self) -> bool:
         """Whether a captured append found a row without a page (synchronises)."""
@@ -284,6 +367,11 @@ class PagedKVCache:
 
     def _restore_host(self, state) -> None:
         self.lengths = list(state)
+
+    def _device_state(self) -> list[torch.Tensor]:
+        """What a step changes on the device and a warm-up has to put back."""
+        kept = [self.cache_lens, self.status]
+        return kept if self.weights is None else [*kept, self.weights]
 
     def _advance(self, n: int) -> None:
         self.lengths = [length + n for length in self.lengths]

@@ -116,6 +116,10 @@ def _restore_host(cache, state) -> None:
         cache.length = state
 
 
+def _device_state(cache) -> list[torch.Tensor]:
+    return cache._device_state() if isinstance(cache, PagedKVCache) else [cache.cursor, cache.status]
+
+
 def _captured_form(cache):
     return cache._captured_form() if isinstance(cache, PagedKVCache) else None
 
@@ -127,8 +131,8 @@ class CachedStepGraph:
     ``fn(*inputs)`` runs one step: its layers append at each cache's cursor
     (``KVCache.append`` / ``append_fused``) and read ``cache_len`` from it, and it
     calls ``commit(rows)`` on every cache in ``caches`` once, at its end. The
-    eager warm-up and the capture leave the caches' cursors, host lengths and
-    statuses as they found them; rows the warm-up wrote past the cursor are
+    eager warm-up and the capture leave the caches' cursors, host lengths, statuses
+    and row weights as they found them; rows the warm-up wrote past the cursor are
     rewritten by the first replay. A paged cache's pages for the next rows are
     reserved before each replay, outside the graph, which reads the table that
     changed in place. Whether it holds a prefix is fixed by the capture: ``RuntimeError``
@@ -143,19 +147,19 @@ class CachedStepGraph:
         self.rows = int(rows)
         for c in self.caches:
             c._check_room(self.rows)
-        saved = [(_host_state(c), c.cursor.clone(), c.status.clone()) for c in self.caches]
+        saved = [(_host_state(c), [t.clone() for t in _device_state(c)]) for c in self.caches]
 
         def restore():
-            for c, (host, cursor, status) in zip(self.caches, saved):
+            for c, (host, state) in zip(self.caches, saved):
                 _restore_host(c, host)
-                c.cursor.copy_(cursor)
-                c.status.copy_(status)
+                for t, was in zip(_device_state(c), state):
+                    t.copy_(was)
 
         self.runner = _record(fn, tuple(t.clone() for t in sample_inputs), warmup,
                               after_each_warmup=restore)
         # Recording ran fn's host code once (its commits moved the host lengths)
         # but no kernel: restore the host side only.
-        for c, (host, _, _) in zip(self.caches, saved):
+        for c, (host, _) in zip(self.caches, saved):
             _restore_host(c, host)
         self._forms = [_captured_form(c) for c in self.caches]
 
