@@ -5,15 +5,18 @@
 // with the largest weights; ties go to the lowest row, NaN counts as the lowest weight. The
 // k-th largest is found digit by digit: weights as integers of the same order, largest
 // first, a histogram of 11, 11, then 10 bits of those that agree with the digits found
-// before. One more pass counts per wave what lies above it and at it, a last one writes the
-// rows in order. One workgroup per (sequence, head): five passes over 4 n bytes, which
-// stay in its XCD's L2 (128 KB of 32,768 rows); latency bounds it, each pass a round trip.
+// before, until a digit's rows are wanted all. Then the rows above it and at it are counted per
+// wave and written in order. One workgroup per (sequence, head), whose weights stay in
+// LDS (up to 32,768 rows): they are read once. (In registers the unrolled passes over 32
+// of them are 30 KB of code, which takes longer to fetch than to run.)
 //
 // kv_page_gather. Row i of a head becomes row rows[i], which is i at least and ascending in
-// i. A workgroup moves a column of the rows of one (sequence, head, plane), kRows rows at a
-// time and in order: all loads of a step are done (a barrier) before its first store, and
-// what later steps read lies behind the rows that this one writes. So it may run in place,
-// on the pages it reads. Bound by memory: kept rows are read and written once.
+// i. A workgroup moves a column of the rows of one (sequence, head, plane), step by step in
+// their order: all loads of a step are done (a barrier) before its first store, and what
+// later steps read lies behind the rows that this one writes. So it may run in place, on the
+// pages it reads. Bound by memory: kept rows are read and written once; the next step's loads
+// are under way while one is stored, and the lookups of 1,024 rows are made at once.
+#include "attn_common.h"
 #include "kv_fp4.h"
 
 #include <algorithm>
@@ -23,15 +26,17 @@ namespace {
 
 constexpr int kKeepThreads = 1024, kKeepWaves = kKeepThreads / 64;
 constexpr int kBits = 11, kBins = 1 << kBits;
+constexpr int kHeld = 32 * kKeepThreads;  // weights in LDS at most: 128 KB
 
 struct KeepArgs {
   const float* w; int64_t w_sb, w_sh;
   const int32_t* lens;
   int32_t* rows;  // [B, H, keep]
   int H, width, keep, recent;
+  int held;       // weights that fit in LDS
 };
 
-// Unsigned integers in the weights' order, -0 as 0, NaN as the lowest.
+// Unsigned integers in the weights' order, -0 as 0, NaN as the lowest. Never 0.
 __device__ __forceinline__ uint32_t rank_of(float x) {
   const uint32_t u = __float_as_uint(x);
   if ((u & 0x7fffffffu) > 0x7f800000u) return 0x007fffffu;  // that of -inf
@@ -39,16 +44,31 @@ __device__ __forceinline__ uint32_t rank_of(float x) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+// Inclusive sums over a wave: shifts by 1, 2, 4, 8 within rows of 16 lanes, then each
+// row's last to the next row, and the first half's to the second.
+template <int kCtrl, int kRows>
+__device__ __forceinline__ uint32_t scan_add(uint32_t x) {
+  return x + uint32_t(__builtin_amdgcn_update_dpp(0, int(x), kCtrl, kRows, 0xf, false));
+}
+__device__ __forceinline__ uint32_t scan64(uint32_t x) {
+  x = scan_add<0x111, 0xf>(x);
+  x = scan_add<0x112, 0xf>(x);
+  x = scan_add<0x114, 0xf>(x);
+  x = scan_add<0x118, 0xf>(x);
+  x = scan_add<0x142, 0xa>(x);
+  return scan_add<0x143, 0xc>(x);
+}
+
 __global__ __launch_bounds__(kKeepThreads) void kv_keep_rows_kernel(KeepArgs a) {
   __shared__ uint32_t hist[kBins];
-  __shared__ uint32_t found[2];               // digit, how many are left to find among its rows
+  __shared__ uint32_t found[3];     // digit, how many are left to find among its rows, its rows
   __shared__ uint32_t above[kKeepWaves], at[kKeepWaves];
   const int tid = int(threadIdx.x), lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int bh = int(blockIdx.x), b = bh / a.H, h = bh - b * a.H;
   const float* const w = a.w + b * a.w_sb + h * a.w_sh;
   int32_t* const out = a.rows + int64_t(bh) * a.keep;
-  const int n = min(max(a.lens[b], 0), a.width);
+  const int n = __builtin_amdgcn_readfirstlane(min(max(a.lens[b], 0), a.width));
   const int c = min(n, a.keep), last = min(a.recent, c), m = n - last;
   const uint32_t k = uint32_t(c - last);
   for (int i = c + tid; i < a.keep; i += kKeepThreads) out[i] = -1;
@@ -59,80 +79,117 @@ __global__ __launch_bounds__(kKeepThreads) void kv_keep_rows_kernel(KeepArgs a) 
     return;
   }
 
+  // A wave has a run of `steps` 64 rows, as integers in LDS, 0 past the end (its own, so no
+  // barrier), four of which are read together. Longer sequences than fit are read again each
+  // time.
+  const int steps = (m + 4 * kKeepThreads - 1) / (4 * kKeepThreads) * 4;
+  const int from = wave * steps * 64 + lane;
+  extern __shared__ uint32_t held[];
+  const bool hold = steps * kKeepThreads <= a.held;
+  auto read = [&](uint32_t (&x)[4], int s) __attribute__((always_inline)) {
+    float f[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] = from + (s + j) * 64 < m ? w[from + (s + j) * 64] : 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = from + (s + j) * 64 < m ? rank_of(f[j]) : 0u;
+  };
+  auto each = [&](auto&& fn) __attribute__((always_inline)) {
+#pragma unroll 1
+    for (int s = 0; s < steps; s += 4) {
+      uint32_t x[4];
+      if (hold) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = held[from + (s + j) * 64];
+      } else {
+        read(x, s);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) fn(x[j], from + (s + j) * 64);
+    }
+  };
+  if (hold) {
+#pragma unroll 2
+    for (int s = 0; s < steps; s += 4) {
+      uint32_t x[4];
+      read(x, s);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) held[from + (s + j) * 64] = x[j];
+    }
+  }
+
   // The k-th largest: `prefix` are its bits found so far, `want` its place among those.
   uint32_t prefix = 0, mask = 0, want = k;
 #pragma unroll 1
   for (int shift = 21; ; shift = shift == 21 ? 10 : 0) {
-    const int bits = shift ? kBits : 10;
+    const uint32_t digits = shift ? kBins - 1 : (1u << 10) - 1;
     for (int i = tid; i < kBins; i += kKeepThreads) hist[i] = 0;
     __syncthreads();
-    for (int i = tid; i < m; i += kKeepThreads) {
-      const uint32_t x = rank_of(w[i]);
-      if ((x & mask) == prefix) atomicAdd(&hist[(x >> shift) & ((1u << bits) - 1)], 1u);
-    }
-    __syncthreads();
-    // From the largest digit down: the first whose rows and all above reach `want`. A
-    // wave takes it, 32 bins to a lane.
-    if (wave == 0) {
-      constexpr int per = kBins / 64;
-      const int top = kBins - 1 - lane * per;  // this lane's bins: top, top - 1, ...
-      uint32_t mine = 0;
-      for (int j = 0; j < per; ++j) mine += hist[top - j];
-      uint32_t upto = mine;
-#pragma unroll
-      for (int d = 1; d < 64; d *= 2) {
-        const uint32_t y = __shfl_up(upto, d);
-        if (lane >= d) upto += y;
+    each([&](uint32_t v, int) __attribute__((always_inline)) {
+      if (v != 0u && (v & mask) == prefix) {
+        const uint32_t d = (v >> shift) & digits;
+        atomicAdd(&hist[d], 1u);
       }
-      const uint64_t hit = __ballot(upto >= want);
-      if (lane == __builtin_ctzll(hit)) {
-        uint32_t before = upto - mine;
-        int j = 0;
-        while (before + hist[top - j] < want) before += hist[top - j++];
-        found[0] = uint32_t(top - j);
-        found[1] = want - before;
+    });
+    __syncthreads();
+    // From the largest digit down: the first whose rows and all above reach `want`. Lanes
+    // take 32 digits each, then the lanes' scan its 32.
+    if (wave == 0) {
+      const int group = 63 - lane;
+      uint32_t mine = 0;
+#pragma unroll
+      for (int j = 0; j < 32; ++j) mine += hist[32 * group + ((j + lane) & 31)];  // (banks apart)
+      const uint32_t upto = scan64(mine);
+      const int l = __builtin_ctzll(__ballot(upto >= want));
+      const uint32_t before = __shfl(upto - mine, l);
+      const uint32_t one = lane < 32 ? hist[32 * (63 - l) + 31 - lane] : 0u;
+      const uint32_t in = before + scan64(one);
+      if (lane == __builtin_ctzll(__ballot(in >= want))) {
+        found[0] = uint32_t(32 * (63 - l) + 31 - lane);
+        found[1] = want - (in - one);
+        found[2] = one;
       }
     }
     __syncthreads();
     prefix |= found[0] << shift;
-    mask |= ((1u << bits) - 1) << shift;
+    mask |= digits << shift;
     want = found[1];
+    if (found[2] == want) {  // all of these: whatever is at least as large as the digits found
+      prefix -= 1;
+      want = 0;
+      break;
+    }
     if (shift == 0) break;
   }
 
-  // Rows above it, and the first `want` of those at it. A wave takes a run of rows.
-  const int run = (m + kKeepThreads - 1) / kKeepThreads * 64;
-  const int from = min(wave * run, m), to = min(from + run, m);
+  // Rows above it, and the first `want` of those at it.
   uint32_t n_above = 0, n_at = 0;
-  for (int i = from; i < to; i += 64) {
-    const uint32_t x = i + lane < to ? rank_of(w[i + lane]) : 0u;
-    n_above += uint32_t(__popcll(__ballot(x > prefix)));
-    n_at += uint32_t(__popcll(__ballot(i + lane < to && x == prefix)));
-  }
+  each([&](uint32_t v, int) __attribute__((always_inline)) {
+    n_above += uint32_t(__popcll(__ballot(v > prefix)));
+    n_at += uint32_t(__popcll(__ballot(v == prefix)));
+  });
   if (lane == 0) {
     above[wave] = n_above;
     at[wave] = n_at;
   }
   __syncthreads();
-  uint32_t pos = 0, seen = 0;  // kept and met at it before this wave's run
+  uint32_t pos = 0, seen = 0;  // kept, and met at it, before this wave's run
   for (int i = 0; i < wave; ++i) {
     pos += above[i];
     seen += at[i];
   }
   pos += min(seen, want);
   const uint64_t below = (uint64_t(1) << lane) - 1;
-  for (int i = from; i < to; i += 64) {
-    const uint32_t x = i + lane < to ? rank_of(w[i + lane]) : 0u;
-    const uint64_t same = __ballot(i + lane < to && x == prefix);
-    const bool take = x > prefix || (same >> lane & 1 && seen + uint32_t(__popcll(same & below)) < want);
+  each([&](uint32_t v, int i) __attribute__((always_inline)) {
+    const uint64_t same = __ballot(v == prefix);
+    const bool take = v > prefix || (v == prefix && seen + uint32_t(__popcll(same & below)) < want);
     const uint64_t taken = __ballot(take);
-    if (take) out[pos + uint32_t(__popcll(taken & below))] = i + lane;
+    if (take) out[pos + uint32_t(__popcll(taken & below))] = i;
     pos += uint32_t(__popcll(taken));
     seen += uint32_t(__popcll(same));
-  }
+  });
 }
 
-constexpr int kGatherThreads = 256, kChunks = 8;  // 16-byte chunks of a thread in a step
+constexpr int kUnits = 4;  // of a thread in a step, and of a row in a column
 
 struct GatherArgs {
   char* pages; int64_t p_plane, p_sp, p_sr, p_sh;  // bytes
@@ -140,92 +197,138 @@ struct GatherArgs {
   const int32_t* dst; int64_t d_sb;
   const int32_t* rows;             // [B, H, keep]
   float* w; int64_t w_sb, w_sh;    // null: none
-  int H, keep, width, dst_width, n_pages, page_rows, w_width;
+  int BH, H, keep, width, dst_width, n_pages, page_rows, w_width;
   int chunks, slice;               // 16-byte chunks of a row; of a workgroup's column (a power of two)
   int slices;                      // columns of a plane; a 4-bit one's last holds its scales
   int tail;                        // scale bytes of a row (0: a 16- or 32-bit pool)
 };
 
-// Where row r of a table's pages lies: the page, or none.
-__device__ __forceinline__ int page_at(const int32_t* table, int r, int rows, int width, int n_pages) {
-  if (uint32_t(r) >= uint32_t(width) * uint32_t(rows)) return -1;
-  const int page = table[r / rows];
-  return uint32_t(page) < uint32_t(n_pages) ? page : -1;
+// Where a row goes from and to, in bytes from a plane's head; from < 0: it does not move.
+struct Place { int64_t from, to; };
+
+// Byte offset of row r of a table's pages, or -1.
+__device__ __forceinline__ int64_t place_of(const GatherArgs& a, const int32_t* table, int r, int width,
+                                            int64_t row_bytes) {
+  if (uint32_t(r) >= uint32_t(width) * uint32_t(a.page_rows)) return -1;
+  const int e = int(uint32_t(r) / uint32_t(a.page_rows));
+  const int page = table[e];
+  if (uint32_t(page) >= uint32_t(a.n_pages)) return -1;
+  return page * a.p_sp + (r - e * a.page_rows) * row_bytes;
 }
 
-// One step after the other: UNIT bytes of a row to a lane at a time.
-template <typename U, int N>
-__device__ __forceinline__ void move_column(const GatherArgs& a, char* plane, const int32_t* rows,
-                                            const int32_t* src, const int32_t* dst, int64_t head,
-                                            int64_t first, int64_t row_bytes, int per, int units) {
-  // `units` a row in this column; `per` (a power of two, units at least) lanes to a row.
-  const int step = N * kGatherThreads / per;
-  const int lr = int(threadIdx.x) / per, lu = int(threadIdx.x) % per;
-#pragma unroll 1
-  for (int i0 = 0; i0 < a.keep; i0 += step) {
-    U x[N];
-    char* to[N];
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const int i = i0 + j * (kGatherThreads / per) + lr;
-      to[j] = nullptr;
-      if (i >= a.keep || lu >= units) continue;
-      const int r = rows[i];
-      if (r < 0) continue;
-      const int from = page_at(src, r, a.page_rows, a.width, a.n_pages);
-      const int into = page_at(dst, i, a.page_rows, a.dst_width, a.n_pages);
-      if (from < 0 || into < 0) continue;
-      const char* const p = plane + from * a.p_sp + head + first + (r % a.page_rows) * row_bytes + lu * int(sizeof(U));
-      char* const q = plane + into * a.p_sp + head + first + (i % a.page_rows) * row_bytes + lu * int(sizeof(U));
-      if (p == q) continue;  // (another sequence may read it)
-      x[j] = *reinterpret_cast<const U*>(p);
-      to[j] = q;
+// A column of the rows, `units` Us of each; `per` (a power of two, units at least, kUnits at
+// most) lanes to a row. kThreads rows to a step. Their places are looked up (two reads that
+// wait for one another) by a thread each, one step ahead; a step's loads go out before the
+// last one's stores: its rows lie behind those that are written then. No wave stores a step
+// before all have read it.
+template <int kThreads, typename U>
+__device__ __forceinline__ void move_column(const GatherArgs& a, Place (*list)[kThreads], char* column,
+                                            const int32_t* rows, const int32_t* src, const int32_t* dst,
+                                            int64_t row_bytes, int per, int units) {
+  const int tid = int(threadIdx.x), lr = tid / per, lu = tid % per, row_step = kThreads / per;
+  auto number = [&](int i) __attribute__((always_inline)) { return i < a.keep ? rows[i] : -1; };
+  auto look = [&](int r, int i) __attribute__((always_inline)) {
+    Place p{-1, -1};
+    if (r >= 0) {
+      p.from = place_of(a, src, r, a.width, row_bytes);
+      p.to = place_of(a, dst, i, a.dst_width, row_bytes);
+      if (p.to < 0 || p.from == p.to) p.from = -1;  // (what stays may be another sequence's too)
     }
-    wait_vmcnt<0>();  // every load of this wave has returned,
-    __syncthreads();  // and of the others
+    return p;
+  };
+  U x[2][kUnits];
+  int64_t to[2][kUnits];  // below 0: nothing
+  auto load = [&](const Place* l, U (&y)[kUnits], int64_t (&t)[kUnits]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < N; ++j)
-      if (to[j]) *reinterpret_cast<U*>(to[j]) = x[j];
+    for (int j = 0; j < kUnits; ++j) {
+      t[j] = -1;
+      if (j < per && lu < units) {
+        const Place p = l[j * row_step + lr];
+        if (p.from >= 0) {
+          y[j] = *reinterpret_cast<const U*>(column + p.from + lu * int(sizeof(U)));
+          t[j] = p.to;
+        }
+      }
+    }
+  };
+  list[0][tid] = look(number(tid), tid);
+  int r = number(kThreads + tid);
+  __syncthreads();
+  load(list[0], x[0], to[0]);
+#pragma unroll 1
+  for (int i0 = 0; i0 < a.keep; i0 += 2 * kThreads) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int next = i0 + (u + 1) * kThreads;  // first row of the next step
+      if (next - kThreads >= a.keep) break;
+      list[1 - u][tid] = look(r, next + tid);
+      r = number(next + kThreads + tid);
+      wait_vmcnt<0>();  // this wave's loads have returned,
+      __syncthreads();  // and the others'
+      if (next < a.keep) load(list[1 - u], x[1 - u], to[1 - u]);
+#pragma unroll
+      for (int j = 0; j < kUnits; ++j)
+        if (to[u][j] >= 0) *reinterpret_cast<U*>(column + to[u][j] + lu * int(sizeof(U))) = x[u][j];
+    }
   }
 }
 
-__global__ __launch_bounds__(kGatherThreads) void kv_page_gather_kernel(GatherArgs a) {
-  const int bh = int(blockIdx.y), b = bh / a.H, h = bh - b * a.H;
+template <int kThreads>
+__global__ __launch_bounds__(kThreads) void kv_page_gather_kernel(GatherArgs a) {
+  __shared__ Place list[2][kThreads];
+  // The columns of a plane's head on one XCD (workgroup i runs on XCD i % 8), whose L2 then
+  // has the other half of each line that one of them reads.
+  uint32_t i = blockIdx.x, plane = 0;
+  uint32_t bh, col;
+  const uint32_t planes = 2u * uint32_t(a.BH), moves = planes * uint32_t(a.slices);
+  const bool weights = i >= moves;
+  if (weights) {
+    bh = i - moves;
+    col = 0;
+  } else {
+    const uint32_t in8 = planes % 8 == 0 ? 8u : 1u, at = i / in8;
+    plane = at / uint32_t(a.slices);
+    col = at - plane * uint32_t(a.slices);
+    plane = plane * in8 + i % in8;
+    bh = plane >> 1;
+  }
+  const int b = int(bh / uint32_t(a.H)), h = int(bh) - b * a.H;
   const int32_t* const rows = a.rows + int64_t(bh) * a.keep;
-  int col = int(blockIdx.x);
-  if (col == 2 * a.slices) {  // the weights: kept ones to the front, 0 behind
+  if (weights) {  // kept ones to the front, 0 behind
     float* const w = a.w + b * a.w_sb + h * a.w_sh;
+    constexpr int N = 8;
 #pragma unroll 1
-    for (int i0 = 0; i0 < a.w_width; i0 += 4 * kGatherThreads) {
-      float x[4];
+    for (int i0 = 0; i0 < a.w_width; i0 += N * kThreads) {
+      float x[N];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int i = i0 + j * kGatherThreads + int(threadIdx.x);
+      for (int j = 0; j < N; ++j) {
+        const int i = i0 + j * kThreads + int(threadIdx.x);
         const int r = i < a.keep ? rows[i] : -1;
         x[j] = uint32_t(r) < uint32_t(a.w_width) ? w[r] : 0.f;
       }
       wait_vmcnt<0>();
       __syncthreads();
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int i = i0 + j * kGatherThreads + int(threadIdx.x);
+      for (int j = 0; j < N; ++j) {
+        const int i = i0 + j * kThreads + int(threadIdx.x);
         if (i < a.w_width) w[i] = x[j];
       }
     }
     return;
   }
-  char* const plane = a.pages + (col >= a.slices ? a.p_plane : 0);
-  col = col >= a.slices ? col - a.slices : col;
+  char* column = a.pages + (plane & 1 ? a.p_plane : 0) + h * a.p_sh;
   const int32_t* const src = a.src + b * a.s_sb;
   const int32_t* const dst = a.dst + b * a.d_sb;
-  const int64_t head = h * a.p_sh;
-  if (a.tail && col == a.slices - 1) {
-    // Scales, 2 bytes at a time (a row has 2, 4 or 8), behind the page's codes.
-    const int units = a.tail / 2;
-    move_column<uint16_t, kChunks>(a, plane, rows, src, dst, head, int64_t(a.page_rows) * a.p_sr, a.tail, units, units);
+  if (a.tail && int(col) == a.slices - 1) {
+    // Scales, 2, 4 or 8 bytes of a row, behind the page's codes.
+    column += int64_t(a.page_rows) * a.p_sr;
+    if (a.tail == 2)
+      move_column<kThreads, uint16_t>(a, list, column, rows, src, dst, 2, 1, 1);
+    else
+      move_column<kThreads, uint32_t>(a, list, column, rows, src, dst, a.tail, a.tail / 4, a.tail / 4);
   } else {
-    move_column<u32x4, kChunks>(a, plane, rows, src, dst, head, int64_t(col) * a.slice * 16, a.p_sr, a.slice,
-                                min(a.slice, a.chunks - col * a.slice));
+    move_column<kThreads, u32x4>(a, list, column + int64_t(col) * a.slice * 16, rows, src, dst, a.p_sr, a.slice,
+                       min(a.slice, a.chunks - int(col) * a.slice));
   }
 }
 
@@ -254,7 +357,13 @@ extern "C" int dx_kv_keep_rows(const void* weights, int64_t w_sb, int64_t w_sh, 
   a.rows = static_cast<int32_t*>(rows);
   a.H = int(H); a.width = int(width); a.keep = int(keep);
   a.recent = int(std::min<int64_t>(recent, keep));
-  hipLaunchKernelGGL(kv_keep_rows_kernel, dim3(unsigned(B * H)), dim3(kKeepThreads), 0,
+  a.held = int(std::min<int64_t>(kHeld, (width + 4 * kKeepThreads - 1) / (4 * kKeepThreads) * (4 * kKeepThreads)));
+  const hipError_t e = opt_in_lds(reinterpret_cast<const void*>(&kv_keep_rows_kernel), kHeld * 4);
+  if (e != hipSuccess) {
+    set_error("%s: %s", what, hipGetErrorString(e));
+    return DX_ELAUNCH;
+  }
+  hipLaunchKernelGGL(kv_keep_rows_kernel, dim3(unsigned(B * H)), dim3(kKeepThreads), a.held * 4,
                      static_cast<hipStream_t>(stream), a);
   DX_CHECK_LAUNCH(what);
   return DX_OK;
@@ -297,17 +406,23 @@ extern "C" int dx_kv_page_gather(void* pages, int64_t p_plane, int64_t p_sp, int
   a.dst = static_cast<const int32_t*>(dst_table); a.d_sb = d_sb;
   a.rows = static_cast<const int32_t*>(rows);
   a.w = static_cast<float*>(weights); a.w_sb = w_sb; a.w_sh = w_sh;
-  a.H = int(H); a.keep = int(keep); a.width = int(width); a.dst_width = int(dst_width);
+  a.BH = int(B * H); a.H = int(H); a.keep = int(keep); a.width = int(width); a.dst_width = int(dst_width);
   a.n_pages = int(n_pages); a.page_rows = int(page_rows); a.w_width = int(w_width);
   a.chunks = int(fp4 ? D / 32 : D * es / 16);
   a.tail = int(fp4 ? D / 32 : 0);
   // Columns of 4 chunks (64 bytes), of less where a row has less: of one long sequence of
   // few heads there would be too few workgroups otherwise.
-  a.slice = std::min(4, a.chunks);
+  a.slice = std::min(kUnits, a.chunks);
   while (a.slice & (a.slice - 1)) --a.slice;
   a.slices = (a.chunks + a.slice - 1) / a.slice + (fp4 ? 1 : 0);
-  hipLaunchKernelGGL(kv_page_gather_kernel, dim3(unsigned(2 * a.slices + (weights ? 1 : 0)), unsigned(B * H)),
-                     dim3(kGatherThreads), 0, static_cast<hipStream_t>(stream), a);
+  const int64_t blocks = (2 * a.slices + (weights ? 1 : 0)) * B * H;
+  DX_CHECK_ARG(grid_fits(blocks, 1024), "%s: the call exceeds one launch", what);
+  const dim3 grid{unsigned(blocks)};
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (2 * a.slices * B * H <= 2 * device_cus())
+    hipLaunchKernelGGL(kv_page_gather_kernel<1024>, grid, dim3(1024), 0, st, a);
+  else
+    hipLaunchKernelGGL(kv_page_gather_kernel<256>, grid, dim3(256), 0, st, a);
   DX_CHECK_LAUNCH(what);
   return DX_OK;
 }
