@@ -375,6 +375,17 @@ struct Tile {
       // With a log-sum-exp, a result in 32 bits, l sums them as they were before that rounding
       // (2^-9 of each in bf16), and a row's weights add up to 1 but for what their roundings
       // come to.
+      //
+      // V fragments are read W ahead of their products, the first ones before the packing:
+      // left alone the compiler reads each right before its product, which then waits
+      // out the LDS latency (2 x 1,500 causal queries, 16 heads of 8, over 400 to 1,000 rows:
+      // 72.4 us a call so, 65.7 with them).
+      constexpr int N = 2 * NS * DT, W = 4;
+      u32x4 vf[W];
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < W; ++i) vf[i] = v_frag(va, i / DT, i % DT);
+      __builtin_amdgcn_sched_barrier(0);
       u32x4 pk[2 * NS];
       float part[2] = {0.f, 0.f};
 #pragma unroll
@@ -389,10 +400,18 @@ struct Tile {
             part[e & 1] += s[u / 2][8 * (u % 2) + 2 * e] + s[u / 2][8 * (u % 2) + 2 * e + 1];
         }
       l += part[0] + part[1];
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int u = 0; u < 2 * NS; ++u)
+      for (int i = 0; i < N; ++i) {
+        acc[i % DT] = Mfma<T>::run(vf[i % W], pk[i / DT], acc[i % DT]);
+        if (i + W < N) vf[i % W] = v_frag(va, (i + W) / DT, (i + W) % DT);
+      }
 #pragma unroll
-        for (int d = 0; d < DT; ++d) acc[d] = Mfma<T>::run(v_frag(va, u, d), pk[u], acc[d]);
+      for (int i = 0; i < N; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if (i + W < N) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
   // V^T operand: dims 32 d + lane % 32 of keys 16 u + {4 g .. 4 g + 3, 8 + 4 g .. 8 + 4 g + 3}.
@@ -505,6 +524,14 @@ struct Tile {
   }
 };
 
+// A load from device memory by its address. (Through a generic pointer it would be one that
+// may be of LDS, and every wait for LDS reads would wait for it.)
+template <typename T>
+__device__ __forceinline__ T load_global(uint64_t at) {
+  typedef __attribute__((address_space(1))) const T global_t;
+  return *(global_t*)at;
+}
+
 // Where an item's keys lie, in scalar registers.
 struct Keys {
   uint64_t pk, pv, nk, nv, table;  // pages and new keys of this head; the sequence's table
@@ -514,12 +541,16 @@ struct Keys {
   int page_rows, n_pages;
   int len, fresh;  // cached rows, new rows that some row of the item sees
   int n_ct;        // 32-key tiles of the cached rows; the new ones' follow
+  // The 64 table entries from ahead_from on, a lane each (none yet: it lies past any).
+  uint32_t ahead, ahead_from;
 
   // The 16 rows from row r0 of the cached ones, or of the new ones: addresses,
   // and how many exist. True where the table names no page for them. in_page: where a
-  // cached one's page has the first.
+  // cached one's page has the first. AHEAD: by entries that lanes hold, read 64 at a time: a
+  // read of the table for each tile is waited for 500 of the tile's 5,600 cycles.
+  template <bool AHEAD>
   __device__ __forceinline__ bool find(bool cached, int r0, uint64_t& k, uint64_t& v, int& rows,
-                                       uint32_t& in_page) const {
+                                       uint32_t& in_page) {
     rows = max(min((cached ? len : fresh) - r0, 16), 0);
     bool gone = false;
     if (cached) {
@@ -527,7 +558,21 @@ struct Keys {
       const uint32_t x16 = uint32_t(r0) >> 4;
       uint32_t e = magic ? uint32_t((uint64_t(x16) * magic) >> 32) : x16;
       e = rows > 0 ? e : 0;
-      const int page = rows > 0 ? ((const_i32*)table)[e] : 0;
+      int page = 0;
+      if constexpr (AHEAD) {
+        if (rows > 0) {
+          e = uniform(e);
+          if (e - ahead_from >= 64u) {
+            const uint32_t x = uint32_t(len - 1) >> 4;  // the last entry there is
+            const uint32_t last = magic ? uint32_t((uint64_t(x) * magic) >> 32) : x;
+            ahead = load_global<uint32_t>(table + 4 * uint64_t(min(e + (threadIdx.x & 63u), last)));
+            ahead_from = e;
+          }
+          page = int(lane_of(ahead, int(e - ahead_from)));
+        }
+      } else {
+        page = rows > 0 ? ((const_i32*)table)[e] : 0;
+      }
       gone = uint32_t(page) >= uint32_t(n_pages);
       rows = gone ? 0 : rows;
       in_page = uint32_t(r0) - e * uint32_t(page_rows);
@@ -542,10 +587,6 @@ struct Keys {
     v = uniform(v);
     rows = __builtin_amdgcn_readfirstlane(rows);
     return gone;
-  }
-  __device__ __forceinline__ bool find(bool cached, int r0, uint64_t& k, uint64_t& v, int& rows) const {
-    uint32_t in_page = 0;
-    return find(cached, r0, k, v, rows, in_page);
   }
 };
 
@@ -610,13 +651,13 @@ struct CodedKeys {
     const uint64_t k = (lane & 16 ? k1 : k0) + uint32_t(row * (D / 2) + 16 * g);
     const uint64_t s = (lane & 16 ? s1 : s0) + uint32_t(row * (D / 32));
 #pragma unroll
-    for (int i = 0; i < N; ++i) code[i] = *reinterpret_cast<const u32x4*>(k + 32 * i);
+    for (int i = 0; i < N; ++i) code[i] = load_global<u32x4>(k + 32 * i);
     if constexpr (N == 1) {
-      scale[0] = *reinterpret_cast<const uint16_t*>(s);
+      scale[0] = load_global<uint16_t>(s);
     } else if constexpr (N == 2) {
-      scale[0] = *reinterpret_cast<const uint32_t*>(s);
+      scale[0] = load_global<uint32_t>(s);
     } else {
-      const u32x2 x = *reinterpret_cast<const u32x2*>(s);
+      const u32x2 x = load_global<u32x2>(s);
       scale[0] = x[0];
       scale[1] = x[1];
     }
@@ -779,6 +820,8 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
       keys.magic = a.page_magic;
       keys.page_rows = a.page_rows;
       keys.n_pages = a.n_pages;
+      keys.ahead = 0;
+      keys.ahead_from = 0u - 64u;
       c = fmaxf(fabsf(a.scale_log2), FLT_MIN);
 
       active = row0 + wave * 32 < nrows && stream < KW;  // wave-uniform
@@ -849,8 +892,8 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
         const int r0 = (cached ? t : t - keys.n_ct) * kPN;
         uint64_t k0, k1;
         uint32_t in0 = 0, in1 = 0;
-        gone = keys.find(cached, r0, k0, v0, rows0, in0) ? 1 : 0;
-        gone |= keys.find(cached, r0 + 16, k1, v1, rows1, in1) ? 2 : 0;
+        gone = keys.find<true>(cached, r0, k0, v0, rows0, in0) ? 1 : 0;
+        gone |= keys.find<true>(cached, r0 + 16, k1, v1, rows1, in1) ? 2 : 0;
         if (cached) {
           const uint64_t s0 = fp4_scales_behind<D>(keys.page_rows, in0);
           const uint64_t s1 = fp4_scales_behind<D>(keys.page_rows, in1);
@@ -912,8 +955,9 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
       auto find = [&](int t) __attribute__((always_inline)) {
         const bool cached = t < keys.n_ct;
         const int r0 = (cached ? t : t - keys.n_ct) * kPN;
-        gone = keys.find(cached, r0, k0, v0, rows0) ? 1 : 0;
-        gone |= keys.find(cached, r0 + 16, k1, v1, rows1) ? 2 : 0;
+        uint32_t in_page = 0;
+        gone = keys.find<false>(cached, r0, k0, v0, rows0, in_page) ? 1 : 0;
+        gone |= keys.find<false>(cached, r0 + 16, k1, v1, rows1, in_page) ? 2 : 0;
         const int sk = __builtin_amdgcn_readfirstlane(cached ? keys.p_sr : keys.k_sl);
         sv = __builtin_amdgcn_readfirstlane(cached ? keys.p_sr : keys.v_sl);
         send_rows<RB, F32, true>(k0, rows0, sk, base, 0, 0, HP, lane);
@@ -978,7 +1022,7 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
         uint64_t k, v;
         int rows;
         uint32_t in_page = 0;
-        const bool gone = keys.find(cached, r0, k, v, rows, in_page);
+        const bool gone = keys.find<(M == kFp4)>(cached, r0, k, v, rows, in_page);
         if (lane == 0) flags[4 * st + wave] = gone ? 1u : 0u;
         const int sk = __builtin_amdgcn_readfirstlane(cached ? keys.p_sr : keys.k_sl);
         const int sv = __builtin_amdgcn_readfirstlane(cached ? keys.p_sr : keys.v_sl);
