@@ -76,22 +76,56 @@ __global__ __launch_bounds__(kThreads) void paged_key_weights_kernel(WeightArgs 
     return;
   }
 
+  // Queries on their way into LDS: this thread's chunks of rows row0.., and a row's lse. The
+  // first ones are read before all else, then the page numbers, whatever the length: what a
+  // workgroup waits for at its start are two reads one after the other, not four (a chunk of 83
+  // over 32,768 rows of 24 heads in bf16: 50.0 us, 41 so).
+  constexpr int NQ = QT * CR / kThreads;
+  static_assert(QT * CR % kThreads == 0 && QT <= kThreads, "whole shares");
+  u32x4 qx[NQ];
+  float lx;
+  auto read_queries = [&](int row0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < NQ; ++e) {
+      const int u = e * kThreads + int(threadIdx.x), row = min(row0 + u / CR, a.R - 1);
+      const int t = int(uint32_t(row) / uint32_t(a.group)), h = hk * a.group + row - t * a.group;
+      qx[e] = *reinterpret_cast<const u32x4*>(a.q + b * a.q_sb + t * a.q_sl + h * a.q_sh + 16 * (u % CR));
+    }
+    const int row = min(row0 + int(threadIdx.x) % QT, a.R - 1);
+    const int t = int(uint32_t(row) / uint32_t(a.group)), h = hk * a.group + row - t * a.group;
+    lx = a.lse[(int64_t(b) * a.Lq + t) * a.H + h];
+  };
+  auto write_queries = [&](int row0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < NQ; ++e) {
+      const int u = e * kThreads + int(threadIdx.x), r = u / CR, c = u % CR;
+      *reinterpret_cast<u32x4*>(tile + r * RB + 16 * (c ^ swz<RB>(r))) = qx[e];
+    }
+    // A query that saw no key, and one past the last, gives nothing.
+    const bool none = row0 + int(threadIdx.x) % QT >= a.R || lx == -INFINITY;
+    if (int(threadIdx.x) < QT) stat[threadIdx.x] = none ? INFINITY : lx * 1.4426950408889634f;
+  };
+  read_queries(0);  // (there are some: without any there are no rows either, see len)
+
   // This lane's keys: half of the dims of each, chunks 8 (s / 4) + 4 g + s % 4, which in
   // 4 bits are whole blocks. Rows without a page or past the length read a query instead
-  // (2 or 4 D bytes) and are not written.
+  // (2 or 4 D bytes) and are not written. (4-bit rows are converted here: kept as codes they
+  // take fewer registers, but 1,500 queries then take 134 us for 118.)
   u32x4 kf[NK][KS];
   bool there[NK];
-  uint32_t entry[NK];
+  int page[NK];
+  auto entry_of = [&](uint32_t r) __attribute__((always_inline)) {
+    return a.page_magic ? uint32_t((uint64_t(r >> 4) * a.page_magic) >> 32) : r >> 4;
+  };
+#pragma unroll
+  for (int x = 0; x < NK; ++x)
+    page[x] = a.table[b * a.t_sb + entry_of(uint32_t(min(key0 + 32 * x + nl, rows - 1)))];
 #pragma unroll
   for (int x = 0; x < NK; ++x) {
     const int r = key0 + 32 * x + nl;
-    there[x] = r < len;
-    const uint32_t x16 = uint32_t(r) >> 4;
-    entry[x] = a.page_magic ? uint32_t((uint64_t(x16) * a.page_magic) >> 32) : x16;
-    const int page = there[x] ? a.table[b * a.t_sb + entry[x]] : -1;
-    there[x] = uint32_t(page) < uint32_t(a.n_pages);
-    const uint32_t in_page = uint32_t(r) - entry[x] * uint32_t(a.page_rows);
-    const char* const head = a.pk + int64_t(page) * a.p_sp + hk * a.p_sh;
+    there[x] = r < len && uint32_t(page[x]) < uint32_t(a.n_pages);
+    const uint32_t in_page = uint32_t(r) - entry_of(uint32_t(r)) * uint32_t(a.page_rows);
+    const char* const head = a.pk + int64_t(page[x]) * a.p_sp + hk * a.p_sh;
     if constexpr (FP4) {
       const char* const codes = there[x] ? head + in_page * uint32_t(D / 2) : a.q;
       const char* const scales = there[x] ? head + uint32_t(a.page_rows) * (D / 2) + in_page * uint32_t(D / 32) : a.q;
@@ -115,27 +149,11 @@ __global__ __launch_bounds__(kThreads) void paged_key_weights_kernel(WeightArgs 
   float sum[NK] = {};
   const uint32_t base = lds_addr(tile);
   for (int row0 = 0; row0 < a.R; row0 += QT) {
-    if (row0) __syncthreads();  // the last rows are read
-#pragma unroll
-    for (int u = int(threadIdx.x); u < QT * CR; u += kThreads) {
-      const int r = u / CR, c = u % CR, row = row0 + r;
-      u32x4 x{0, 0, 0, 0};
-      if (row < a.R) {
-        const int t = int(uint32_t(row) / uint32_t(a.group)), h = hk * a.group + row - t * a.group;
-        x = *reinterpret_cast<const u32x4*>(a.q + b * a.q_sb + t * a.q_sl + h * a.q_sh + 16 * c);
-      }
-      *reinterpret_cast<u32x4*>(tile + r * RB + 16 * (c ^ swz<RB>(r))) = x;
+    if (row0) {
+      read_queries(row0);
+      __syncthreads();  // the last rows are read
     }
-    if (int(threadIdx.x) < QT) {
-      const int row = row0 + int(threadIdx.x);
-      float l = INFINITY;  // gives nothing
-      if (row < a.R) {
-        const int t = int(uint32_t(row) / uint32_t(a.group)), h = hk * a.group + row - t * a.group;
-        const float x = a.lse[(int64_t(b) * a.Lq + t) * a.H + h];
-        l = x == -INFINITY ? INFINITY : x * 1.4426950408889634f;  // (it saw no key)
-      }
-      stat[threadIdx.x] = l;
-    }
+    write_queries(row0);
     __syncthreads();
 #pragma unroll 1
     for (int m0 = 0; m0 < QT && row0 + m0 < a.R; m0 += 32) {
