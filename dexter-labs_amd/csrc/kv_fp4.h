@@ -11,7 +11,7 @@
 // The scale is 2^e for the least e with every magnitude of the block at most
 // 7 * 2^e, so that the rounding to 6, the largest code, is off by at most the
 // half step 2^e that any code above 4 may be off by. Relative to the values' norm,
-// of normal data: 0.115. e keeps to [-127, 125] for bf16 and [-23, 13] for f16, where
+// of normal data: 0.112. e keeps to [-127, 125] for bf16 and [-23, 13] for f16, where
 // all of a block's values are numbers of that type.
 //
 // A pool is bytes [2, P, H, R * (D / 2 + D / 32)]: of each page and head first the

@@ -27,6 +27,7 @@ namespace dx {
 namespace {
 
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
+constexpr float kNone = 0x1.fffffep127f;  // for a log-sum-exp: of a query that gives nothing
 
 struct WeightArgs {
   const char* q; int64_t q_sb, q_sl, q_sh;  // bytes
@@ -101,9 +102,9 @@ __global__ __launch_bounds__(kThreads) void paged_key_weights_kernel(WeightArgs 
       const int u = e * kThreads + int(threadIdx.x), r = u / CR, c = u % CR;
       *reinterpret_cast<u32x4*>(tile + r * RB + 16 * (c ^ swz<RB>(r))) = qx[e];
     }
-    // A query that saw no key, and one past the last, gives nothing.
+    // A query that saw no key, and one past the last, gives nothing, whatever its scores.
     const bool none = row0 + int(threadIdx.x) % QT >= a.R || lx == -INFINITY;
-    if (int(threadIdx.x) < QT) stat[threadIdx.x] = none ? INFINITY : lx * 1.4426950408889634f;
+    if (int(threadIdx.x) < QT) stat[threadIdx.x] = none ? kNone : lx * 1.4426950408889634f;
   };
   read_queries(0);  // (there are some: without any there are no rows either, see len)
 
@@ -176,20 +177,30 @@ __global__ __launch_bounds__(kThreads) void paged_key_weights_kernel(WeightArgs 
         }
       }
       // Register r: query m0 + 8 (r / 4) + 4 g + r % 4. Their sum as a tree, then one
-      // addition: of many queries the running sum takes a rounding per 32.
+      // addition: of many queries the running sum takes a rounding per 32. (An infinite score
+      // less kNone is no 0: where there is one of those, its terms are taken out.)
+      auto add_up = [&](auto some) __attribute__((always_inline)) {
 #pragma unroll
-      for (int x = 0; x < NK; ++x) {
-        float part[4];
+        for (int x = 0; x < NK; ++x) {
+          float part[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const f32x4 l = *reinterpret_cast<const f32x4*>(&stat[m0 + 8 * u + 4 * g]);
-          float p[4];
+          for (int u = 0; u < 4; ++u) {
+            const f32x4 l = *reinterpret_cast<const f32x4*>(&stat[m0 + 8 * u + 4 * g]);
+            float p[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) p[e] = fast_exp2(__builtin_fmaf(s[x][4 * u + e], a.scale_log2, -l[e]));
-          part[u] = (p[0] + p[1]) + (p[2] + p[3]);
+            for (int e = 0; e < 4; ++e) {
+              p[e] = fast_exp2(__builtin_fmaf(s[x][4 * u + e], a.scale_log2, -l[e]));
+              if constexpr (decltype(some)::value) p[e] = l[e] == kNone ? 0.f : p[e];
+            }
+            part[u] = (p[0] + p[1]) + (p[2] + p[3]);
+          }
+          sum[x] += (part[0] + part[1]) + (part[2] + part[3]);
         }
-        sum[x] += (part[0] + part[1]) + (part[2] + part[3]);
-      }
+      };
+      if (__ballot(stat[m0 + nl] == kNone))
+        add_up(std::integral_constant<bool, true>{});
+      else
+        add_up(std::integral_constant<bool, false>{});
     }
   }
 #pragma unroll

@@ -470,9 +470,10 @@ def kv_page_gather(pages: torch.Tensor, block_table: torch.Tensor, rows: torch.T
     ``[B, H, N]`` move with their rows and are 0 behind them.
 
     ``rows`` is what ``kv_keep_rows`` returned: in place it has to be ascending with ``rows[b,
-    h, i] >= i``. Entries below 0, past a table or without a page move nothing. Pages that
-    ``dst_table`` names and ``block_table`` does not at the same place must not be read by any
-    sequence of the call. ``head_dim`` is needed for pages in 4 bits.
+    h, i] >= i``. Entries below 0, past a table or without a page move nothing, nor does a row
+    that is where it belongs. A page that rows move into must not be another sequence's, nor
+    one that the call reads, but for the page that both tables name at the same place of one
+    sequence. ``head_dim`` is needed for pages in 4 bits.
     """
     return select("cache", "page_gather", pages, rows)(pages, block_table, rows, dst_table, weights,
                                                        head_dim)

@@ -86,15 +86,16 @@ def paged_key_weights(q, lse, weights, pages, block_table, cache_lens, softmax_s
         raise ValueError(f"{what}: lse must be float32 {[b, q_len, heads]} on {device}")
     t_sb, width = _table(block_table, b, device, "block_table")
     _check_i32(cache_lens, (b,), device, "cache_lens")
-    if weights is not None:
-        _check_weights(weights, (b, kv_heads, width * rows), device, what)
+    shape = (b, kv_heads, width * rows)
+    w_sb, w_sh = kv_heads * shape[2], shape[2]
+    add = weights is not None
+    if add:
+        w_sb, w_sh = _check_weights(weights, shape, device, what)
     if _elsewhere(device):
         with _on(device):
             return paged_key_weights(q, lse, weights, pages, block_table, cache_lens, softmax_scale)
-    add = weights is not None
     if not add:
-        weights = torch.empty((b, kv_heads, width * rows), device=device)
-    w_sb, w_sh = _check_weights(weights, (b, kv_heads, width * rows), device, what)
+        weights = torch.empty(shape, device=device)
     if weights.numel() == 0 or (add and q.numel() == 0):
         return weights
     scale = float(softmax_scale) if softmax_scale is not None else 1.0 / math.sqrt(dim)
@@ -140,7 +141,7 @@ def kv_keep_rows(weights, cache_lens, keep, recent=0):
     if rows.numel() == 0:
         return rows
     rc = _lib.load().dx_kv_keep_rows(weights.data_ptr(), sb, sh, width, cache_lens.data_ptr(), keep,
-                                     recent, rows.data_ptr(), b, heads, _lib.stream_handle(device))
+                                     min(recent, keep), rows.data_ptr(), b, heads, _lib.stream_handle(device))
     if rc:
         _lib.check(rc, what)
     return rows

@@ -4,7 +4,7 @@ The format (``csrc/kv_fp4.h``): E2M1 codes, 32 to a power-of-two scale, so that 
 a head takes ``D / 2 + D / 32`` bytes (68 at D 128, where 16 bits take 256). It is the
 one that this hardware converts by itself, exactly: attention reads the rows as the
 values that were stored and rounds nothing more. What storing rounds is the user's
-choice (of normal data 11.5% of its norm).
+choice (of normal data 11.2% of its norm).
 
 A pool is uint8 ``[2, P, H, R * (D / 2 + D / 32)]``; pages, tables and lengths are those
 of ``paged.py``, whose checks these operators share. No counterpart in the reference.

@@ -187,6 +187,33 @@ def test_queries_that_saw_no_key_give_nothing(device, built_lib):
     assert got.shape == (0, 2, 32)
 
 
+@pytest.mark.parametrize("in4", [False, True])
+@pytest.mark.parametrize("lq", [7, 40, 100])
+def test_what_gives_nothing_may_be_no_number(device, built_lib, in4, lq):
+    """Queries that saw no key hold NaN and infinities: the weights are those without them."""
+    lens, rows, heads, dim = [300, 64], 16, 2, 128
+    count, tables, _ = _tables(lens, rows, 5)
+    pages = _rand((2, count, rows, heads, dim), torch.bfloat16, 6)
+    pool = (fp4.pack(*fp4.quantise(pages)) if in4 else pages).to(device)
+    q = _rand((2, lq, heads, dim), torch.bfloat16, 7).to(device)
+    lse = torch.full((2, lq, heads), 9.0, device=device)
+    for t in {lq - 1, lq // 2, 1}:
+        lse[0, t] = -math.inf
+    kw = dict(pages=pool, block_table=_i32(tables, device), cache_lens=_i32(lens, device))
+    want = ops.paged_key_weights(q, lse, **kw)
+    bad = q.clone()
+    bad[0, lq - 1], bad[0, lq // 2, 0], bad[0, 1, 1] = math.nan, math.inf, -math.inf
+    assert bool(torch.isfinite(want).all()) and float(want[0, :, :300].min()) > 0
+    assert torch.equal(ops.paged_key_weights(bad, lse, **kw), want)
+    # An infinite key: its weight is what the queries that count give it, the last ones of a
+    # tile's rows no more than others.
+    if not in4:
+        pool[0, tables[1][0], 0] = math.inf
+        q[1] = q[1].abs()
+        got = ops.paged_key_weights(q, lse, **kw)
+        assert bool((got[1, :, 0] == math.inf).all())
+
+
 def test_weights_sum_to_the_queries(device, built_lib):
     """With no new keys, each query's probabilities over the cached rows add up to 1."""
     lens, rows, lq, heads, kv, dim = [1000, 37], 64, 83, 4, 2, 128
