@@ -79,41 +79,50 @@ __global__ __launch_bounds__(kKeepThreads) void kv_keep_rows_kernel(KeepArgs a) 
     return;
   }
 
-  // A wave has a run of `steps` 64 rows, as integers in LDS, 0 past the end (its own, so no
-  // barrier), four of which are read together. Longer sequences than fit are read again each
-  // time.
-  const int steps = (m + 4 * kKeepThreads - 1) / (4 * kKeepThreads) * 4;
-  const int from = wave * steps * 64 + lane;
-  extern __shared__ uint32_t held[];
-  const bool hold = steps * kKeepThreads <= a.held;
-  auto read = [&](uint32_t (&x)[4], int s) __attribute__((always_inline)) {
-    float f[4];
+  // A wave has a run of `steps` 256 rows, as integers in LDS, 0 past the end (its own, so no
+  // barrier), of which a lane has four that lie side by side. Longer sequences than fit are
+  // read again each time.
+  const int steps = (m + 4 * kKeepThreads - 1) / (4 * kKeepThreads);
+  const int from = wave * steps * 256 + 4 * lane;
+  extern __shared__ __attribute__((aligned(16))) uint32_t held[];
+  const bool hold = 4 * steps * kKeepThreads <= a.held;
+  const bool wide = (reinterpret_cast<uintptr_t>(w) & 15u) == 0 && m >= 4;
+  // Rows row.. of the sequence, whatever stands there instead past its end.
+  auto load = [&](int row) __attribute__((always_inline)) {
+    if (wide) return *reinterpret_cast<const f32x4*>(w + min(row, (m & ~3) - 4));
+    f32x4 f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) f[j] = from + (s + j) * 64 < m ? w[from + (s + j) * 64] : 0.f;
+    for (int j = 0; j < 4; ++j) f[j] = w[min(row + j, m - 1)];
+    return f;
+  };
+  auto ranks = [&](f32x4 f, int row) __attribute__((always_inline)) {
+    if (wide && row < m && row + 4 > m) {  // the last, that are no four
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = from + (s + j) * 64 < m ? rank_of(f[j]) : 0u;
+      for (int j = 0; j < 3; ++j) f[j] = w[min(row + j, m - 1)];
+    }
+    u32x4 x;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = row + j < m ? rank_of(f[j]) : 0u;
+    return x;
   };
   auto each = [&](auto&& fn) __attribute__((always_inline)) {
 #pragma unroll 1
-    for (int s = 0; s < steps; s += 4) {
-      uint32_t x[4];
-      if (hold) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = held[from + (s + j) * 64];
-      } else {
-        read(x, s);
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) fn(x[j], from + (s + j) * 64);
+    for (int s = 0; s < steps; ++s) {
+      const int row = from + 256 * s;
+      fn(hold ? *reinterpret_cast<const u32x4*>(held + row) : ranks(load(row), row), row);
     }
   };
   if (hold) {
-#pragma unroll 2
-    for (int s = 0; s < steps; s += 4) {
-      uint32_t x[4];
-      read(x, s);
+    constexpr int N = 4;  // loads under way
+#pragma unroll 1
+    for (int s = 0; s < steps; s += N) {
+      f32x4 f[N];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) held[from + (s + j) * 64] = x[j];
+      for (int j = 0; j < N; ++j) f[j] = load(from + 256 * (s + j));
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (s + j < steps)
+          *reinterpret_cast<u32x4*>(held + from + 256 * (s + j)) = ranks(f[j], from + 256 * (s + j));
     }
   }
 
@@ -124,11 +133,10 @@ __global__ __launch_bounds__(kKeepThreads) void kv_keep_rows_kernel(KeepArgs a) 
     const uint32_t digits = shift ? kBins - 1 : (1u << 10) - 1;
     for (int i = tid; i < kBins; i += kKeepThreads) hist[i] = 0;
     __syncthreads();
-    each([&](uint32_t v, int) __attribute__((always_inline)) {
-      if (v != 0u && (v & mask) == prefix) {
-        const uint32_t d = (v >> shift) & digits;
-        atomicAdd(&hist[d], 1u);
-      }
+    each([&](u32x4 v, int) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (v[j] != 0u && (v[j] & mask) == prefix) atomicAdd(&hist[(v[j] >> shift) & digits], 1u);
     });
     __syncthreads();
     // From the largest digit down: the first whose rows and all above reach `want`. Lanes
@@ -161,31 +169,44 @@ __global__ __launch_bounds__(kKeepThreads) void kv_keep_rows_kernel(KeepArgs a) 
     if (shift == 0) break;
   }
 
-  // Rows above it, and the first `want` of those at it.
+  // Rows above it, and the first `want` of those at it. Two counts of a step's 256 rows
+  // in one number: those above it in the low half, those at it in the high one.
+  auto count = [&](u32x4 v) __attribute__((always_inline)) {
+    uint32_t n = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) n += (v[j] > prefix ? 1u : 0u) + (v[j] == prefix ? 1u << 16 : 0u);
+    return n;
+  };
   uint32_t n_above = 0, n_at = 0;
-  each([&](uint32_t v, int) __attribute__((always_inline)) {
-    n_above += uint32_t(__popcll(__ballot(v > prefix)));
-    n_at += uint32_t(__popcll(__ballot(v == prefix)));
+  each([&](u32x4 v, int) __attribute__((always_inline)) {
+    const uint32_t n = count(v);
+    n_above += n & 0xffffu;
+    n_at += n >> 16;
   });
-  if (lane == 0) {
+  n_above = scan64(n_above);
+  n_at = scan64(n_at);
+  if (lane == 63) {
     above[wave] = n_above;
     at[wave] = n_at;
   }
   __syncthreads();
-  uint32_t pos = 0, seen = 0;  // kept, and met at it, before this wave's run
+  uint32_t pos = 0, seen = 0;  // above, and at it, before this wave's next step
   for (int i = 0; i < wave; ++i) {
     pos += above[i];
     seen += at[i];
   }
-  pos += min(seen, want);
-  const uint64_t below = (uint64_t(1) << lane) - 1;
-  each([&](uint32_t v, int i) __attribute__((always_inline)) {
-    const uint64_t same = __ballot(v == prefix);
-    const bool take = v > prefix || (v == prefix && seen + uint32_t(__popcll(same & below)) < want);
-    const uint64_t taken = __ballot(take);
-    if (take) out[pos + uint32_t(__popcll(taken & below))] = i;
-    pos += uint32_t(__popcll(taken));
-    seen += uint32_t(__popcll(same));
+  each([&](u32x4 v, int row) __attribute__((always_inline)) {
+    const uint32_t n = count(v), upto = scan64(n), before = upto - n;
+    uint32_t s = seen + (before >> 16), p = pos + (before & 0xffffu) + min(s, want);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const bool same = v[j] == prefix;
+      if (v[j] > prefix || (same && s < want)) out[p++] = row + j;
+      s += same ? 1u : 0u;
+    }
+    const uint32_t all = uint32_t(__builtin_amdgcn_readlane(int(upto), 63));
+    pos += all & 0xffffu;
+    seen += all >> 16;
   });
 }
 
