@@ -178,7 +178,9 @@ __global__ __launch_bounds__(kThreads) void paged_key_weights_kernel(WeightArgs 
       }
       // Register r: query m0 + 8 (r / 4) + 4 g + r % 4. Their sum as a tree, then one
       // addition: of many queries the running sum takes a rounding per 32. (An infinite score
-      // less kNone is no 0: where there is one of those, its terms are taken out.)
+      // or NaN less kNone is no 0: where a query that saw no key is among them, such terms are
+      // taken out. What stands behind the last query is that one again, whose own term is as
+      // infinite then.)
       auto add_up = [&](auto some) __attribute__((always_inline)) {
 #pragma unroll
         for (int x = 0; x < NK; ++x) {
@@ -197,7 +199,7 @@ __global__ __launch_bounds__(kThreads) void paged_key_weights_kernel(WeightArgs 
           sum[x] += (part[0] + part[1]) + (part[2] + part[3]);
         }
       };
-      if (__ballot(stat[m0 + nl] == kNone))
+      if (__ballot(stat[m0 + nl] == kNone && row0 + m0 + nl < a.R))
         add_up(std::integral_constant<bool, true>{});
       else
         add_up(std::integral_constant<bool, false>{});
