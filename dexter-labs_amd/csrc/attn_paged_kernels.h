@@ -332,6 +332,7 @@ struct Tile {
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[x][r] = fast_exp2(__builtin_fmaf(s[x][r], c, -mb));
   }
+  template <bool AHEAD>
   __device__ __forceinline__ void pv(uint32_t va, const f32x16 (&s)[NS]) {
     if constexpr (F32) {
       float part[4] = {0.f, 0.f, 0.f, 0.f};
@@ -379,13 +380,17 @@ struct Tile {
       // V fragments are read W ahead of their products, the first ones before the packing:
       // left alone the compiler reads each right before its product, which then waits
       // out the LDS latency (2 x 1,500 causal queries, 16 heads of 8, over 400 to 1,000 rows:
-      // 72.4 us a call so, 65.7 with them).
+      // 72.4 us a call so, 65.7 with them). Not over a prefix, whose many tiles of one length
+      // leave a SIMD's other wave to fill the wait (16 x 83 over 8,217 rows, 24 heads: 218.1 us so,
+      // 221 read ahead; in 4 bits 203.0 and 206.6).
       constexpr int N = 2 * NS * DT, W = 4;
       u32x4 vf[W];
-      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (AHEAD) {
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int i = 0; i < W; ++i) vf[i] = v_frag(va, i / DT, i % DT);
-      __builtin_amdgcn_sched_barrier(0);
+        for (int i = 0; i < W; ++i) vf[i] = v_frag(va, i / DT, i % DT);
+        __builtin_amdgcn_sched_barrier(0);
+      }
       u32x4 pk[2 * NS];
       float part[2] = {0.f, 0.f};
 #pragma unroll
@@ -400,6 +405,12 @@ struct Tile {
             part[e & 1] += s[u / 2][8 * (u % 2) + 2 * e] + s[u / 2][8 * (u % 2) + 2 * e + 1];
         }
       l += part[0] + part[1];
+      if constexpr (!AHEAD) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          acc[i % DT] = Mfma<T>::run(v_frag(va, i / DT, i % DT), pk[i / DT], acc[i % DT]);
+        return;
+      }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
@@ -942,7 +953,7 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
           }
         }
-        ti.pv(va, s);
+        ti.template pv<!PREFIX>(va, s);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         if (more && tile_at(i + 1) >= keys.n_ct) send_v();
       }
@@ -990,7 +1001,7 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
           Ti::clear_poison(base + Sh::tile, 0, Sh::tile, lane);
           asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
-        ti.pv(va, s);
+        ti.template pv<!PREFIX>(va, s);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         if (more) send_v();
       }
@@ -1108,7 +1119,7 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
           ti.take_poison(v0, s, seen, lane);
           clear();
         }
-        ti.pv(va + st, s);
+        ti.template pv<!PREFIX>(va + st, s);
         if (i + 1 < nt) take_tile(i + 1);
       }
     }
