@@ -15,6 +15,12 @@
 // queries, all rows of a (sequence, K/V head), pass through LDS for four waves. 64 keys
 // a wave halve the LDS reads per product, which at 32 would take the LDS as long as the
 // products take the matrix units.
+//
+// What it takes: a chunk of 83 over 32,768 rows of 24 heads (D 128) 44 us in bf16, 4.6 TB/s,
+// 32 us in 4 bits; one token of 32 prompts of 300 to 3,000 rows in 4 bits 15.4 us, of which
+// the host's part is 15; 2 x 1,500 queries, 16 heads over 8, over 4,000 to 10,000 rows 120
+// us, 600 TFLOP/s, exponentials and products in turn. Long workgroups that walk several blocks
+// of keys gained nothing at 3 to 1,000 workgroups per compute unit.
 #include "attn_common.h"
 #include "attn_tile.h"
 #include "kv_fp4.h"
