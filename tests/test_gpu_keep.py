@@ -396,3 +396,64 @@ def test_a_captured_eviction(device, built_lib):
         torch.cuda.synchronize()
         assert torch.equal(step(pools[1], ws[1]), at)
         assert torch.equal(pools[0], pools[1]) and torch.equal(ws[0], ws[1])
+
+
+@pytest.mark.parametrize("in4", [False, True])
+def test_pools_past_4_gb(device, built_lib, in4):
+    """Pages whose offsets pass 32 bits, against the same pages in a small pool."""
+    rows, heads, dim, k = 128, 8, 128, 150
+    row = 68 if in4 else 256
+    count = (1 << 32) // (rows * heads * row) + 40
+    shape = (heads, rows * row) if in4 else (rows, heads, dim)
+    small = _rand((2, 3, rows, heads, dim), torch.bfloat16, 1)
+    small = (fp4.pack(*fp4.quantise(small)) if in4 else small).to(device)
+    large = torch.empty(2, count, *shape, dtype=small.dtype, device=device)
+    at = [count - 1, 2, count - 9]
+    large[:, at] = small
+    q = _rand((1, 5, heads, dim), torch.bfloat16, 2).to(device)
+    lse = torch.full((1, 5, heads), 4.0, device=device)
+    got = []
+    for pool, table in ((small, [[0, 1, 2]]), (large, [at])):
+        kw = dict(block_table=_i32(table, device), cache_lens=_i32([330], device))
+        w = ops.paged_key_weights(q, lse, pages=pool, **kw)
+        rows_kept = ops.kv_keep_rows(w, kw["cache_lens"], k, 20)
+        ops.kv_page_gather(pool, kw["block_table"], rows_kept, None, w, dim)
+        got.append((w, rows_kept, pool[:, table[0]]))
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+    assert bool((got[0][0] > 0).any()) and int(got[0][1].max()) == 329
+
+
+@pytest.mark.parametrize("in4", [False, True])
+def test_two_streams_at_once(device, built_lib, in4):
+    """Attention, weights, choice and move of two caches on streams of their own: each as alone."""
+    lens, rows, heads, dim, lq = [900, 40, 600], 16, 4, 128, 50
+    count, tables, _ = _tables(lens, rows, 4)
+    kw = dict(block_table=_i32(tables, device), cache_lens=_i32(lens, device))
+    attend = ops.paged_attention_fp4 if in4 else ops.paged_attention
+
+    def run(q, pool):
+        out, lse = attend(q, q, q, pages=pool, return_lse=True, **kw)
+        w = ops.paged_key_weights(q, lse, pages=pool, **kw)
+        kept = ops.kv_keep_rows(w, kw["cache_lens"], 100, 10)
+        ops.kv_page_gather(pool, kw["block_table"], kept, None, w, dim)
+        return out, lse, kept, w, pool
+    inputs = []
+    for i in range(2):
+        pages = _rand((2, count, rows, heads, dim), torch.bfloat16, 10 + i)
+        pool = (fp4.pack(*fp4.quantise(pages)) if in4 else pages).to(device)
+        inputs.append((_rand((3, lq, heads, dim), torch.bfloat16, 20 + i).to(device), pool))
+    want = [run(q, pool.clone()) for q, pool in inputs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(4):
+        pools = [pool.clone() for _, pool in inputs]
+        torch.cuda.synchronize()
+        got = []
+        for s, (q, _), pool in zip(streams, inputs, pools):
+            with torch.cuda.stream(s):
+                got.append(run(q, pool))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            for x, y in zip(a, b):
+                assert torch.equal(x, y)
