@@ -19,6 +19,7 @@ struct Record { int item, slot, parts, pad; };
 struct Line {
   float* o;     // [slot][32 RW rows][D]: unnormalised sums
   float* ml;    // [slot][32 RW rows]: {m, l}
+  float* le;    // [slot][32 RW rows]: second sums (null: none)
   Record* rec;
   int splits;   // key ranges per item; 0: the line is cut into pieces
   int by_item;  // the records are, and there are some
@@ -41,7 +42,7 @@ struct PagedArgs {
   float scale_log2;             // signed
   int own_n;                    // workgroups for the own line at most, where it alone is cut
   Line own, pre;
-  float* lse;                   // [B, Lq, H], or null
+  float* lse;                   // [B, Lq, H]; null without
 };
 
 constexpr int64_t kMaxItemCost = 16;  // kItemCost at most
@@ -67,5 +68,7 @@ hipError_t launch_paged_f16_lse(const PagedArgs& a, const PagedPlan& p, int D, h
 hipError_t launch_paged_f32_lse(const PagedArgs& a, const PagedPlan& p, int D, hipStream_t st);
 hipError_t launch_paged_bf16_fp4(const PagedArgs& a, const PagedPlan& p, int D, hipStream_t st);
 hipError_t launch_paged_f16_fp4(const PagedArgs& a, const PagedPlan& p, int D, hipStream_t st);
+hipError_t launch_paged_bf16_fp4_lse(const PagedArgs& a, const PagedPlan& p, int D, hipStream_t st);
+hipError_t launch_paged_f16_fp4_lse(const PagedArgs& a, const PagedPlan& p, int D, hipStream_t st);
 
 }  // namespace dx

@@ -103,9 +103,10 @@ PagedPlan plan_paged(int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hkv, 
   return p;
 }
 
-int64_t slot_bytes(int rw, int64_t D) { return 32 * int64_t(rw) * (D * 4 + 8); }
-int64_t plan_bytes(const PagedPlan& p, int64_t D) {
-  return p.own_slots * slot_bytes(p.rw_own, D) + p.pre_slots * slot_bytes(p.rw_pre, D) +
+// two: partials have a second sum (log-sum-exps in 16 bits).
+int64_t slot_bytes(int rw, int64_t D, bool two) { return 32 * int64_t(rw) * (D * 4 + (two ? 12 : 8)); }
+int64_t plan_bytes(const PagedPlan& p, int64_t D, bool two) {
+  return p.own_slots * slot_bytes(p.rw_own, D, two) + p.pre_slots * slot_bytes(p.rw_pre, D, two) +
          (p.own_recs + p.pre_recs) * int64_t(sizeof(Record));
 }
 
@@ -193,7 +194,8 @@ int paged_entry(const char* what, const dx_paged_call* call, Form form) {
 
   const PagedPlan p = plan_paged(c.B, c.Lq, c.Lk, c.H, c.Hkv, c.D, c.dtype, c.width * c.page_rows,
                                  c.prefix_width * c.page_rows, prefix, device_cus());
-  const int64_t need = plan_bytes(p, c.D);
+  const bool two = form.with_lse && c.dtype != DX_F32;
+  const int64_t need = plan_bytes(p, c.D, two);
   if (need > c.workspace_bytes || (need > 0 && !c.workspace)) {
     set_error("%s: workspace of %lld bytes, %lld needed", what, (long long)(c.workspace ? c.workspace_bytes : 0),
               (long long)need);
@@ -247,13 +249,19 @@ int paged_entry(const char* what, const dx_paged_call* call, Form form) {
   a.pre.o = reinterpret_cast<float*>(take(p.pre_slots * 32 * p.rw_pre * c.D * 4));
   a.own.ml = reinterpret_cast<float*>(take(p.own_slots * 32 * p.rw_own * 8));
   a.pre.ml = reinterpret_cast<float*>(take(p.pre_slots * 32 * p.rw_pre * 8));
+  if (two) {
+    a.own.le = reinterpret_cast<float*>(take(p.own_slots * 32 * p.rw_own * 4));
+    a.pre.le = reinterpret_cast<float*>(take(p.pre_slots * 32 * p.rw_pre * 4));
+  }
   a.own.rec = reinterpret_cast<Record*>(take(p.own_recs * int64_t(sizeof(Record))));
   a.pre.rec = reinterpret_cast<Record*>(take(p.pre_recs * int64_t(sizeof(Record))));
   const hipStream_t st = static_cast<hipStream_t>(c.stream);
   const int D = int(c.D);
   const bool bf16 = c.dtype == DX_BF16;
   hipError_t e;
-  if (form.fp4)
+  if (form.fp4 && form.with_lse)
+    e = bf16 ? launch_paged_bf16_fp4_lse(a, p, D, st) : launch_paged_f16_fp4_lse(a, p, D, st);
+  else if (form.fp4)
     e = bf16 ? launch_paged_bf16_fp4(a, p, D, st) : launch_paged_f16_fp4(a, p, D, st);
   else if (form.with_lse)
     e = c.dtype == DX_F32 ? launch_paged_f32_lse(a, p, D, st)
@@ -275,17 +283,31 @@ int paged_entry(const char* what, const dx_paged_call* call, Form form) {
 
 using namespace dx;
 
-extern "C" int64_t dx_paged_attention_workspace_bytes(int dtype, int64_t B, int64_t Lq, int64_t Lk,
-                                                      int64_t H, int64_t Hkv, int64_t D,
-                                                      int64_t page_rows, int64_t width,
-                                                      int has_prefix, int64_t prefix_width) {
+namespace {
+int64_t workspace_bytes(int dtype, int64_t B, int64_t Lq, int64_t Lk, int64_t H, int64_t Hkv, int64_t D,
+                        int64_t page_rows, int64_t width, int has_prefix, int64_t prefix_width, bool lse) {
   const int bad = check_sizes("paged_attention", B, Lq, Lk, H, Hkv, D, dtype, page_rows, width,
                               prefix_width);
   if (bad) return -bad;
   if (B == 0 || Lq == 0) return 0;
   const PagedPlan p = plan_paged(B, Lq, Lk, H, Hkv, D, dtype, width * page_rows,
                                  prefix_width * page_rows, has_prefix != 0, device_cus());
-  return plan_bytes(p, D);
+  return plan_bytes(p, D, lse && dtype != DX_F32);
+}
+}  // namespace
+
+extern "C" int64_t dx_paged_attention_workspace_bytes(int dtype, int64_t B, int64_t Lq, int64_t Lk,
+                                                      int64_t H, int64_t Hkv, int64_t D,
+                                                      int64_t page_rows, int64_t width,
+                                                      int has_prefix, int64_t prefix_width) {
+  return workspace_bytes(dtype, B, Lq, Lk, H, Hkv, D, page_rows, width, has_prefix, prefix_width, false);
+}
+
+extern "C" int64_t dx_paged_attention_lse_workspace_bytes(int dtype, int64_t B, int64_t Lq, int64_t Lk,
+                                                          int64_t H, int64_t Hkv, int64_t D,
+                                                          int64_t page_rows, int64_t width,
+                                                          int has_prefix, int64_t prefix_width) {
+  return workspace_bytes(dtype, B, Lq, Lk, H, Hkv, D, page_rows, width, has_prefix, prefix_width, true);
 }
 
 extern "C" int dx_paged_attention(const dx_paged_call* call) {

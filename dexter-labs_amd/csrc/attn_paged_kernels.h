@@ -96,8 +96,14 @@ template <typename T> struct Elem { static constexpr int bytes = 2; };
 template <> struct Elem<float> { static constexpr int bytes = 4; };
 
 // What a launch reads and writes besides: kLse, each query's log-sum-exp; kFp4, cached
-// rows in 4 bits (kv_fp4.h), and the log-sum-exp where it is asked for.
-enum Mode { kPlain, kLse, kFp4 };
+// rows in 4 bits (kv_fp4.h); kFp4Lse, both.
+enum Mode { kPlain, kLse, kFp4, kFp4Lse };
+constexpr bool in_fp4(Mode m) { return m == kFp4 || m == kFp4Lse; }
+constexpr bool with_lse(Mode m) { return m == kLse || m == kFp4Lse; }
+// Whether a row has two sums: that of its probabilities as they enter the product, rounded to
+// 16 bits, divides the result, and a log-sum-exp, a result in 32, takes them as they were. In fp32
+// nothing is rounded, and one serves both.
+template <typename T, Mode M> constexpr bool two_sums = with_lse(M) && Elem<T>::bytes == 2;
 
 // Tile rows of RB bytes in LDS: 16-byte chunk c of row r sits at c ^ kswz(r)
 // (K) or c ^ vswz(r) (V). K: the swizzles of attn_fwd.hip and attn_wide.hip,
@@ -133,10 +139,10 @@ template <typename T, int D, int RW> struct Shape {
   static constexpr int stream = stages * 2 * tile;
   // Results on their way between waves: [wave][D' / 8 vectors][64 lanes] of 16
   // bytes, a vector's row padded by 16 (reads across vectors then hit all
-  // banks), and {m, l} of 32 rows. D' = D, or half of it where that fits.
+  // banks), {m, l} of 32 rows, and their second sums. D' = D, or half of it where that fits.
   static constexpr int DP = D > 128 ? 128 : D;
   static constexpr int vec = 1040;
-  static constexpr int area = DP / 8 * vec + 256;
+  static constexpr int ml = DP / 8 * vec, le = ml + 256, area = le + 128;
   static constexpr int body = KW * stream > RW * KW * area ? KW * stream : RW * KW * area;
   // Behind them: which 16-row groups of each stage's tile have no page, and
   // whether a wave's sums hold what is no number.
@@ -253,13 +259,13 @@ struct Tile {
   static constexpr bool F32 = Elem<T>::bytes == 4;
   static constexpr int RB = D * Elem<T>::bytes, KS = RB / 32, DT = D / 32;
   f32x16 acc[DT];
-  float m, l;
+  float m, l, le;  // le: the second sum (two_sums)
 
   __device__ __forceinline__ void reset() {
 #pragma unroll
     for (int d = 0; d < DT; ++d) acc[d] = f32x16{};
     m = -INFINITY;
-    l = 0.f;
+    l = le = 0.f;
   }
   // S^T = K Q^T of the tile, K fragments read W ahead of the products that use
   // them: left alone the compiler reads each right before its product, which
@@ -329,6 +335,7 @@ struct Tile {
       if (!__all(m == -INFINITY)) {
         const float corr = m == -INFINITY ? 0.f : fast_exp2((m - m_new) * c);
         l *= corr;
+        if constexpr (two_sums<T, M>) le *= corr;
 #pragma unroll
         for (int d = 0; d < DT; ++d) acc[d] *= corr;
       }
@@ -380,10 +387,9 @@ struct Tile {
       // the peak rate, or a second product of what the rounding left. l sums the rounded ones, so
       // that a row's weights still add up to 1. Against 64 bits, relative to the
       // outputs' norm: 0.0023 in bf16 and 2.9e-4 in f16, of which the result's own rounding
-      // is 0.0017 and 2.1e-4.
-      // With a log-sum-exp, a result in 32 bits, l sums them as they were before that rounding
-      // (2^-9 of each in bf16), and a row's weights add up to 1 but for what their roundings
-      // come to.
+      // is 0.0017 and 2.1e-4. (Divided by the sum of the unrounded ones, a row that one key
+      // carries is off by that key's rounding, 2^-9 of it: the maximum is followed at a distance, so
+      // its probability is not 1.) le sums them as they were, for a log-sum-exp alone.
       //
       // V fragments are read W ahead of their products, the first ones before the packing:
       // left alone the compiler reads each right before its product, which then waits
@@ -400,19 +406,19 @@ struct Tile {
         __builtin_amdgcn_sched_barrier(0);
       }
       u32x4 pk[2 * NS];
-      float part[2] = {0.f, 0.f};
+      float part[2] = {0.f, 0.f}, exact[2] = {0.f, 0.f};
 #pragma unroll
       for (int u = 0; u < 2 * NS; ++u)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const uint32_t p = Mfma<T>::pack(s[u / 2][8 * (u % 2) + 2 * e], s[u / 2][8 * (u % 2) + 2 * e + 1]);
           pk[u][e] = p;
-          if constexpr (M == kPlain)
-            part[e & 1] = Mfma<T>::sum2(p, part[e & 1]);
-          else
-            part[e & 1] += s[u / 2][8 * (u % 2) + 2 * e] + s[u / 2][8 * (u % 2) + 2 * e + 1];
+          part[e & 1] = Mfma<T>::sum2(p, part[e & 1]);
+          if constexpr (two_sums<T, M>)
+            exact[e & 1] += s[u / 2][8 * (u % 2) + 2 * e] + s[u / 2][8 * (u % 2) + 2 * e + 1];
         }
       l += part[0] + part[1];
+      if constexpr (two_sums<T, M>) le += exact[0] + exact[1];
       if constexpr (!AHEAD) {
 #pragma unroll
         for (int i = 0; i < N; ++i)
@@ -722,7 +728,7 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
   using Ti = Tile<T, D, TK / 32, M>;
   // Single row waves over 4 bits: a key's dims go to lanes by blocks (CodedKeys), 8 dims
   // of product s being chunk chunk_of(s) + 4 g of the row; else chunk 2 s + g.
-  constexpr bool kByBlocks = M == kFp4 && RW == 1;
+  constexpr bool kByBlocks = in_fp4(M) && RW == 1, kTwoSums = two_sums<T, M>;
   auto chunk_of = [](int s) { return kByBlocks ? 8 * (s / 4) + s % 4 : 2 * s; };
   constexpr bool F32 = Ti::F32;
   constexpr int KS = Ti::KS;
@@ -1020,10 +1026,10 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
       uint32_t* const flags = reinterpret_cast<uint32_t*>(smem + Sh::flags) + stream * 2 * 4;
       // Cached rows in 4 bits go through registers: take_tile writes what send_tile read to the
       // stage that is sent to, any time before the barrier that publishes it.
-      Coded<T, D, M == kFp4 ? WR : 16> kc, vc;
+      Coded<T, D, in_fp4(M) ? WR : 16> kc, vc;
       bool coming = false;
       auto take_tile = [&](int i) __attribute__((always_inline)) {
-        if constexpr (M == kFp4) {
+        if constexpr (in_fp4(M)) {
           if (!coming) return;
           const uint32_t to = base + (i & 1) * 2 * Sh::tile;
           kc.template store<true>(to, wave * WR, lane);
@@ -1041,12 +1047,12 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
         uint64_t k, v;
         int rows;
         uint32_t in_page = 0;
-        const bool gone = keys.find<(M == kFp4)>(cached, r0, k, v, rows, in_page);
+        const bool gone = keys.find<in_fp4(M)>(cached, r0, k, v, rows, in_page);
         if (lane == 0) flags[4 * st + wave] = gone ? 1u : 0u;
         const int sk = __builtin_amdgcn_readfirstlane(cached ? keys.p_sr : keys.k_sl);
         const int sv = __builtin_amdgcn_readfirstlane(cached ? keys.p_sr : keys.v_sl);
         const uint32_t to = base + st * 2 * Sh::tile + tr * RB;
-        if constexpr (M == kFp4) {
+        if constexpr (in_fp4(M)) {
           coming = cached;
           if (cached) {
             const uint64_t sc = fp4_scales_behind<D>(keys.page_rows, in_page);
@@ -1145,6 +1151,7 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
     const bool whole = first && t1 == weight && splits <= 1;
     const float mref = ti.m == -INFINITY ? -INFINITY : ti.m * c;
     const float lsum = xor32_sum(ti.l);
+    const float lexact = kTwoSums ? xor32_sum(ti.le) : 0.f;
     Args& a = *reread(args);
     const int nrows = PREFIX ? a.B * a.R : a.R;
 #pragma unroll
@@ -1160,8 +1167,10 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
             *reinterpret_cast<f32x4*>(area + (4 * d + u) * Sh::vec + 16 * lane) =
                 f32x4{v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]};
           }
-        if (g == 0)
-          *reinterpret_cast<f32x2*>(area + Sh::DP / 8 * Sh::vec + 8 * nl) = f32x2{mref, lsum};
+        if (g == 0) {
+          *reinterpret_cast<f32x2*>(area + Sh::ml + 8 * nl) = f32x2{mref, lsum};
+          if constexpr (kTwoSums) *reinterpret_cast<float*>(area + Sh::le + 4 * nl) = lexact;
+        }
       }
       __syncthreads();
       constexpr int CD = Sh::DP / 8;  // 8-value chunks of a row in this pass
@@ -1175,16 +1184,19 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
           float mm = -INFINITY;
 #pragma unroll
           for (int s = 0; s < KW; ++s) {
-            ml[s] = *reinterpret_cast<const f32x2*>(area + s * RW * Sh::area + CD * Sh::vec + 8 * (r % 32));
+            ml[s] = *reinterpret_cast<const f32x2*>(area + s * RW * Sh::area + Sh::ml + 8 * (r % 32));
             mm = fmaxf(mm, ml[s][0]);
           }
           const float ref = mm == -INFINITY ? 0.f : mm;
-          float l = 0.f;
+          float l = 0.f, le = 0.f;
           f32x4 o[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
           for (int s = 0; s < KW; ++s) {
             const float wt = fast_exp2(ml[s][0] - ref);
             l = __builtin_fmaf(ml[s][1], wt, l);
+            if constexpr (kTwoSums)
+              le = __builtin_fmaf(*reinterpret_cast<const float*>(area + s * RW * Sh::area + Sh::le + 4 * (r % 32)),
+                                  wt, le);
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
               const f32x4 v = *reinterpret_cast<const f32x4*>(area + s * RW * Sh::area + ch * Sh::vec +
@@ -1201,8 +1213,8 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
             const uint32_t rr = uint32_t(row0 + r);
             const int qo = int(rr / uint32_t(a.group));
             const int ho = hk * a.group + int(rr - uint32_t(qo) * uint32_t(a.group));
-            if constexpr (M != kPlain)
-              if (a.lse && col == 0) a.lse[(int64_t(b) * a.Lq + qo) * a.H + ho] = log_sum(mm, l);
+            if constexpr (with_lse(M))
+              if (col == 0) a.lse[(int64_t(b) * a.Lq + qo) * a.H + ho] = log_sum(mm, kTwoSums ? le : l);
             char* const op = a.out + b * a.o_sb + qo * a.o_sl + ho * a.o_sh + col * Elem<T>::bytes;
             if constexpr (F32) {
               reinterpret_cast<f32x4*>(op)[0] = o[0] * inv;
@@ -1217,8 +1229,10 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
             f32x4* const po = reinterpret_cast<f32x4*>((PREFIX ? a.pre.o : a.own.o) + at_row * D + col);
             po[0] = o[0];
             po[1] = o[1];
-            if (col == 0)
+            if (col == 0) {
               *reinterpret_cast<f32x2*>((PREFIX ? a.pre.ml : a.own.ml) + at_row * 2) = f32x2{mm, l};
+              if constexpr (kTwoSums) (PREFIX ? a.pre.le : a.own.le)[at_row] = le;
+            }
           }
         }
       }
@@ -1337,6 +1351,8 @@ template <typename T, int D, int RWP, int RWO, Mode M>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
   __shared__ f32x4 sums[3][64][2];
   __shared__ f32x2 stats[3][64];
+  __shared__ float exact[3][64];  // of second sums
+  constexpr bool kTwoSums = two_sums<T, M>;
   const Record rec = a.own.rec[blockIdx.x];
   if (rec.parts == 0) return;
   const uint32_t n_rt = uint32_t(a.R + 32 * RWO - 1) / (32 * RWO);
@@ -1349,11 +1365,12 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
   const int row = int(rt) * 32 * RWO + in_item;
   if (int(rt) * 32 * RWO + int(blockIdx.y) * 8 >= a.R) return;  // no row of this workgroup exists
   const bool valid = row < a.R;
-  float m = -INFINITY, l = 0.f;
+  float m = -INFINITY, l = 0.f, le = 0.f;
   f32x4 o[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-  auto add = [&](const f32x2 ml, const f32x4 (&v)[2], float ref) __attribute__((always_inline)) {
+  auto add = [&](const f32x2 ml, float e, const f32x4 (&v)[2], float ref) __attribute__((always_inline)) {
     const float wt = fast_exp2(ml[0] - ref);
     l = __builtin_fmaf(ml[1], wt, l);
+    if constexpr (kTwoSums) le = __builtin_fmaf(e, wt, le);
 #pragma unroll
     for (int x = 0; x < 2; ++x)
 #pragma unroll
@@ -1362,6 +1379,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
   auto rescale = [&](float mm) __attribute__((always_inline)) {
     const float ref = mm == -INFINITY ? 0.f : mm, keep = fast_exp2(m - ref);
     l *= keep;
+    if constexpr (kTwoSums) le *= keep;
     o[0] *= keep;
     o[1] *= keep;
     m = mm;
@@ -1386,17 +1404,20 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
     // This wave's parts, four at a time: their loads do not wait for one another.
     for (int p0 = wave; p0 < parts; p0 += 16) {
       f32x2 ml[4];
+      float e[4];
       f32x4 v[4][2];
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         const int p = p0 + 4 * x, q = p - pre_parts;
         ml[x] = f32x2{-INFINITY, 0.f};
+        e[x] = 0.f;
         v[x][0] = v[x][1] = f32x4{0.f, 0.f, 0.f, 0.f};
         if (p < parts) {
           const bool pre = RWP > 0 && q < 0;
           const int64_t at = pre ? pre_row + int64_t(p) * (32 * RWP)
                                  : own_row + int64_t(broken ? (q ? 2 * q - 1 : 0) : q) * (32 * RWO);
           ml[x] = *reinterpret_cast<const f32x2*>((pre ? a.pre.ml : a.own.ml) + at * 2);
+          if constexpr (kTwoSums) e[x] = (pre ? a.pre.le : a.own.le)[at];
           const f32x4* const from = reinterpret_cast<const f32x4*>((pre ? a.pre.o : a.own.o) + at * D + 8 * ch);
           v[x][0] = from[0];
           v[x][1] = from[1];
@@ -1407,11 +1428,12 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
       for (int x = 0; x < 4; ++x) mm = fmaxf(mm, ml[x][0]);
       const float ref = rescale(mm);
 #pragma unroll
-      for (int x = 0; x < 4; ++x) add(ml[x], v[x], ref);
+      for (int x = 0; x < 4; ++x) add(ml[x], e[x], v[x], ref);
     }
   }
   if (wave > 0) {
     stats[wave - 1][lane] = f32x2{m, l};
+    if constexpr (kTwoSums) exact[wave - 1][lane] = le;
     sums[wave - 1][lane][0] = o[0];
     sums[wave - 1][lane][1] = o[1];
   }
@@ -1422,11 +1444,11 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
   for (int x = 0; x < 3; ++x) mm = fmaxf(mm, stats[x][lane][0]);
   const float ref = rescale(mm);
 #pragma unroll
-  for (int x = 0; x < 3; ++x) add(stats[x][lane], sums[x][lane], ref);
+  for (int x = 0; x < 3; ++x) add(stats[x][lane], kTwoSums ? exact[x][lane] : 0.f, sums[x][lane], ref);
   const float inv = 1.0f / l;  // no visible key: 0 * inf = NaN
   const int qi = int(uint32_t(row) / uint32_t(a.group)), hq = hk * a.group + row - qi * a.group;
-  if constexpr (M != kPlain)
-    if (a.lse && ch == 0) a.lse[(int64_t(b) * a.Lq + qi) * a.H + hq] = log_sum(m, l);
+  if constexpr (with_lse(M))
+    if (ch == 0) a.lse[(int64_t(b) * a.Lq + qi) * a.H + hq] = log_sum(m, kTwoSums ? le : l);
   char* const op = a.out + b * a.o_sb + qi * a.o_sl + hq * a.o_sh + 8 * ch * Elem<T>::bytes;
   if constexpr (Elem<T>::bytes == 4) {
     reinterpret_cast<f32x4*>(op)[0] = o[0] * inv;

@@ -317,8 +317,7 @@ def paged_attention(
 
     With ``return_lse`` also each query's log-sum-exp, fp32 ``[B, L, H]``: ``ln`` of the
     sum of ``exp(softmax_scale * q.k)`` over the keys it sees, ``-inf`` where it sees none
-    (``paged_key_weights`` takes it). In 16 bits the result's last bits may then differ:
-    the weights are divided by a sum of what they were before their rounding.
+    (``paged_key_weights`` takes it). The result is the same, bit for bit.
     """
     impl = select("attention", "paged", q, k, v)
     more = {"return_lse": True} if return_lse else {}

@@ -17,7 +17,7 @@ import torch
 
 LIB_NAME = "libdexter_gfx950.so"
 LIB_PATH = Path(__file__).resolve().parents[2] / LIB_NAME
-ABI_VERSION = 14
+ABI_VERSION = 15
 
 DX_OK, DX_EINVAL, DX_ELAUNCH, DX_EFULL, DX_EWORKSPACE = 0, 1, 2, 3, 4
 DX_BF16, DX_F16, DX_F32, DX_I32, DX_I64, DX_FP4 = 0, 1, 2, 3, 4, 5
@@ -174,6 +174,7 @@ _SIGNATURES: dict[str, tuple[type, list]] = {
     "dx_paged_attention_workspace_bytes": (_l, [
         _i, _l, _l, _l, _l, _l, _l,  # dtype, B, Lq, Lk, H, Hkv, D
         _l, _l, _i, _l]),          # rows per page, table width, has prefix, prefix width
+    "dx_paged_attention_lse_workspace_bytes": (_l, [_i, _l, _l, _l, _l, _l, _l, _l, _l, _i, _l]),
     "dx_paged_attention": (_i, [_p]),          # a packed dx_paged_call (PAGED_CALL)
     "dx_shared_prefix_attention": (_i, [_p]),
     "dx_paged_attention_lse": (_i, [_p, _p]),  # call, lse

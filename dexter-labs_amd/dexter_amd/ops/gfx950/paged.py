@@ -202,10 +202,11 @@ def _attn_accepts(q, k, v, *args, **kwargs) -> bool:
 
 @functools.lru_cache(maxsize=1024)
 def _workspace_bytes(device_index, code, b, q_len, kv_len, heads, kv_heads, dim, rows, width,
-                     has_prefix, p_width) -> int:
+                     has_prefix, p_width, with_lse) -> int:
     """Of a shape on the current device (``device_index``): the library's own answer."""
-    n = _lib.load().dx_paged_attention_workspace_bytes(
-        code, b, q_len, kv_len, heads, kv_heads, dim, rows, width, has_prefix, p_width)
+    lib = _lib.load()
+    ask = lib.dx_paged_attention_lse_workspace_bytes if with_lse else lib.dx_paged_attention_workspace_bytes
+    n = ask(code, b, q_len, kv_len, heads, kv_heads, dim, rows, width, has_prefix, p_width)
     if n < 0:
         _lib.check(-n, "paged attention workspace")
     return n
@@ -300,7 +301,7 @@ def _attend(what, q, k, v, pages, prefix, block_table, cache_lens, block_boundar
         starts_ptr = starts.data_ptr()
     code = _lib.dtype_code(dtype)
     ws_bytes = _workspace_bytes(device.index, code, b, q_len, kv_len, heads, kv_heads, dim, rows,
-                                width, int(prefix is not None), p_width)
+                                width, int(prefix is not None), p_width, return_lse)
     # From torch's allocator, on the current stream: no other call holds it.
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device) if ws_bytes else None
     o_row = heads * dim

@@ -48,7 +48,8 @@
  *   dx_kv_page_append_fp4, dx_kv_page_read_fp4, dx_paged_attention_fp4,
  *   dx_shared_prefix_attention_fp4
  *                            the same with the cache in 4 bits (no counterpart)
- *   dx_paged_attention_lse, dx_shared_prefix_attention_lse, dx_paged_key_weights,
+ *   dx_paged_attention_lse, dx_shared_prefix_attention_lse,
+ *   dx_paged_attention_lse_workspace_bytes, dx_paged_key_weights,
  *   dx_kv_keep_rows, dx_kv_page_gather
  *                            a cache that keeps the rows which attention weighs
  *                            most (no counterpart)
@@ -93,7 +94,7 @@ const char* dx_last_error(void);
 
 /* ABI revision of this header; the Python loader checks it. */
 int dx_abi_version(void);
-#define DX_ABI_VERSION 14
+#define DX_ABI_VERSION 15
 
 /*
  * Launch-schedule overrides, for measurement and tests only: process-wide,
@@ -572,13 +573,17 @@ int64_t dx_paged_attention_workspace_bytes(int dtype, int64_t B, int64_t Lq, int
 /*
  * dx_paged_attention and dx_shared_prefix_attention that also write each query's
  * log-sum-exp: lse (float [B, Lq, H], contiguous, not NULL) = ln of the sum of
- * exp(scale q.k) over the keys it sees, -inf where it sees none. In 16 bits the
- * weights are divided by the sum of the probabilities as they were before their
- * rounding, so out may differ from the other entry points' in its last bits.
- * Workspace as theirs.
+ * exp(scale q.k) over the keys it sees, -inf where it sees none. out is theirs, bit
+ * for bit. In 16 bits the log-sum-exp's sum is one of its own, over the
+ * probabilities as they were before their rounding, and a call's workspace is
+ * dx_paged_attention_lse_workspace_bytes(...), as large or larger.
  */
 int dx_paged_attention_lse(const dx_paged_call* call, void* lse);
 int dx_shared_prefix_attention_lse(const dx_paged_call* call, void* lse);
+int64_t dx_paged_attention_lse_workspace_bytes(int dtype, int64_t B, int64_t Lq, int64_t Lk,
+                                               int64_t H, int64_t Hkv, int64_t D,
+                                               int64_t page_rows, int64_t width,
+                                               int has_prefix, int64_t prefix_width);
 
 /*
  * A KV cache's pages in 4 bits. A pool is bytes [2, n_pages, H, page_rows *
@@ -618,7 +623,8 @@ int dx_kv_page_read_fp4(const void* pages, int64_t p_plane, int64_t p_sp, int64_
  * (and the prefix) in a 4-bit pool: pages, p_plane, p_sp and p_sh of the call are
  * its bytes and byte strides, p_sr is not read; q, k, v and out are of dtype,
  * DX_BF16 or DX_F16. lse may be NULL. The rows' values are exact in dtype and
- * enter the products as they are. Workspace as theirs.
+ * enter the products as they are. Workspace as theirs; without lse as
+ * dx_paged_attention's.
  */
 int dx_paged_attention_fp4(const dx_paged_call* call, void* lse);
 int dx_shared_prefix_attention_fp4(const dx_paged_call* call, void* lse);
