@@ -81,8 +81,8 @@ class PagedKVCache:
         self.prefix_len = torch.zeros(1, **i32)
         self.status = torch.zeros(1, **i32)
         # What the rows received: of every layer, a sequence's tail behind its length is 0.
-        self.weights = (torch.zeros(layers, batch, heads, self.width * page_rows, device=device)
-                        if track_weights else None)
+        self.weights = (torch.zeros(layers, batch, heads, self.width * page_rows, device=device,
+                                    dtype=torch.float32) if track_weights else None)
 
     def _copy_pages(self, src: list[int], dst: list[int]) -> None:
         pools = self.pools

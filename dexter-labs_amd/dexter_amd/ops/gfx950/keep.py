@@ -95,7 +95,7 @@ def paged_key_weights(q, lse, weights, pages, block_table, cache_lens, softmax_s
         with _on(device):
             return paged_key_weights(q, lse, weights, pages, block_table, cache_lens, softmax_scale)
     if not add:
-        weights = torch.empty(shape, device=device)
+        weights = torch.empty(shape, device=device, dtype=torch.float32)
     if weights.numel() == 0 or (add and q.numel() == 0):
         return weights
     scale = float(softmax_scale) if softmax_scale is not None else 1.0 / math.sqrt(dim)

@@ -288,7 +288,7 @@ def _attend(what, q, k, v, pages, prefix, block_table, cache_lens, block_boundar
             return _attend(what, q, k, v, pages, prefix, block_table, cache_lens, block_boundaries,
                            softmax_scale, causal, return_lse, fp4)
     out = torch.empty((b, q_len, heads, dim), device=device, dtype=dtype)
-    lse = torch.empty((b, q_len, heads), device=device) if return_lse else None
+    lse = torch.empty((b, q_len, heads), device=device, dtype=torch.float32) if return_lse else None
     if b == 0 or q_len == 0:
         return (out, lse) if return_lse else out
     scale = float(softmax_scale) if softmax_scale is not None else 1.0 / math.sqrt(dim)
