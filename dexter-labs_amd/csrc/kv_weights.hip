@@ -67,8 +67,16 @@ __global__ __launch_bounds__(kThreads) void paged_key_weights_kernel(WeightArgs 
   using F = Form<T, D, FP4>;
   constexpr int RB = F::RB, KS = F::KS, NK = F::NK, QT = F::QT, CR = RB / 16;
   constexpr bool F32 = F::es == 4;
-  __shared__ __attribute__((aligned(16))) char tile[QT * RB];
-  __shared__ __attribute__((aligned(16))) float stat[QT];
+  // One array, the tile at a multiple of RB in it: chunks are addressed by XOR into a row's start.
+  struct Shared {
+    __attribute__((aligned(512))) char tile[QT * RB];
+    __attribute__((aligned(16))) float stat[QT];
+  };
+  __shared__ Shared shared;
+  static_assert(512 % RB == 0 && alignof(Shared) % RB == 0 && __builtin_offsetof(Shared, tile) == 0,
+                "a row's chunks by XOR");
+  char* const tile = shared.tile;
+  float* const stat = shared.stat;
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6), lane = int(threadIdx.x) & 63;
   const int g = lane >> 5, nl = lane & 31;
   const int bh = int(blockIdx.y), b = bh / a.Hkv, hk = bh - b * a.Hkv;
