@@ -275,8 +275,9 @@ class PagedKVCache:
         if need:
             to = torch.tensor([t + [-1] * (self.width - len(t)) for t in tables], dtype=torch.int32)
             to = to.to(self.block_table.device)
-        for pool, weights in zip(self.pools, self.weights):
-            rows = ops.kv_keep_rows(weights, self.cache_lens, keep, recent)
+        # Every layer's rows are chosen before any layer's move: what can fail comes first.
+        picked = [ops.kv_keep_rows(weights, self.cache_lens, keep, recent) for weights in self.weights]
+        for pool, weights, rows in zip(self.pools, self.weights, picked):
             ops.kv_page_gather(pool, self.block_table, rows, to, weights, self.head_dim)
         for _ in range(need):
             self._take()
