@@ -248,18 +248,21 @@ class PagedKVCache:
         if self.weights is not None:
             self.weights.zero_()
 
-    def evict(self, keep: int, recent: int = 0) -> int:
-        """Bring every sequence that holds more than ``keep`` rows down to ``keep``: its last
-        ``recent`` rows (at most ``keep``) and the heaviest before them, in their order, each
-        layer and head by its own weights. Returns how many sequences that was. Rows stay
-        where their pages are the sequence's alone; the others' go to new pages
-        (``RuntimeError`` with nothing changed when there are too few)."""
+    def evict(self, keep: int, recent: int = 0, seq: int | None = None) -> int:
+        """Bring every sequence (or ``seq`` alone) that holds more than ``keep`` rows down to
+        ``keep``: its last ``recent`` rows (at most ``keep``) and the heaviest before them, in
+        their order, each layer and head by its own weights. Returns how many sequences that
+        was. Rows stay where their pages are the sequence's alone; the others' go to new pages
+        (``RuntimeError`` with nothing changed when there are too few: all sequences' new pages
+        are found before any old one is free, so on a full pool that sequences share, evict
+        them one by one, which frees pages for the next and leaves the last sharer in place)."""
         if self.weights is None:
             raise RuntimeError("evict needs PagedKVCache(track_weights=True)")
         if keep < 0 or recent < 0:
             raise ValueError(f"cannot keep {keep} rows, {recent} of them the last")
         self._outside_a_capture("evict")
-        long = [b for b, length in enumerate(self.lengths) if length > keep]
+        which = range(self.batch) if seq is None else [range(self.batch)[seq]]
+        long = [b for b in which if self.lengths[b] > keep]
         if not long:
             return 0
         count = -(-keep // self.page_rows)
@@ -276,9 +279,11 @@ class PagedKVCache:
             to = torch.tensor([t + [-1] * (self.width - len(t)) for t in tables], dtype=torch.int32)
             to = to.to(self.block_table.device)
         # Every layer's rows are chosen before any layer's move: what can fail comes first.
-        picked = [ops.kv_keep_rows(weights, self.cache_lens, keep, recent) for weights in self.weights]
-        for pool, weights, rows in zip(self.pools, self.weights, picked):
-            ops.kv_page_gather(pool, self.block_table, rows, to, weights, self.head_dim)
+        at = slice(which[0], which[-1] + 1)
+        layers = [weights[at] for weights in self.weights]
+        picked = [ops.kv_keep_rows(weights, self.cache_lens[at], keep, recent) for weights in layers]
+        for pool, weights, rows in zip(self.pools, layers, picked):
+            ops.kv_page_gather(pool, self.block_table[at], rows, to[at], weights, self.head_dim)
         for _ in range(need):
             self._take()
         for b in long:
