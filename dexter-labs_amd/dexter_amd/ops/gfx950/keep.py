@@ -190,9 +190,10 @@ def kv_page_gather(pages, block_table, rows, dst_table=None, weights=None, head_
     if _elsewhere(device):
         with _on(device):
             return kv_page_gather(pages, block_table, rows, dst_table, weights, head_dim)
+    rows = rows.contiguous()  # (held until the launch)
     rc = _lib.load().dx_kv_page_gather(
         pages.data_ptr(), s0, s1, s2, s3, code, pages.shape[1], page_rows, block_table.data_ptr(),
-        s_sb, width, to.data_ptr(), d_sb, d_width, rows.contiguous().data_ptr(), keep, w_ptr, w_sb,
+        s_sb, width, to.data_ptr(), d_sb, d_width, rows.data_ptr(), keep, w_ptr, w_sb,
         w_sh, w_width, b, heads, head_dim, _lib.stream_handle(device))
     if rc:
         _lib.check(rc, what)
