@@ -10,8 +10,9 @@ of page numbers and a length of its own:
   step is one of the whole batch, ``n`` rows for every sequence. Lengths come to differ
   through ``free`` and ``fork``; ``SelfAttention`` then takes a rotary table per sequence.
 * ``fork(src, dst)`` makes sequence ``dst`` a copy of ``src`` by sharing its pages: no
-  bytes move. The partly filled last page is copied when one of the two next writes
-  to it (``kv_page_copy``, one launch for all layers).
+  rows move. The partly filled last page is copied when one of the two next writes
+  to it (``kv_page_copy``, one launch for all layers). Row weights, where a cache tracks
+  them, are copied at once.
 * ``hold_prefix(seq)`` turns the history of one sequence into a prefix of the whole
   batch (several candidate futures of one episode): it is kept once, and attention
   computes it once for all sequences (``shared_prefix_attention``). Until then it
@@ -25,7 +26,11 @@ of page numbers and a length of its own:
   ``evict(keep, recent)`` brings every longer sequence down to ``keep`` rows: the last
   ``recent`` and the heaviest before them, each layer and head by its own weights. Rows carry
   their positions in their rotated keys: the caller goes on counting positions from where
-  the sequence was, not from its new length. A prefix keeps all of its rows.
+  the sequence was, not from its new length. A prefix keeps all of its rows. A row receives
+  weight from the steps after its own, nothing from the chunk that it was written with: let
+  ``recent`` cover the last chunk at least. (After one chunk, all weights are 0, and the
+  lowest rows would be kept.) ``weights`` are 4 bytes for each row that a table has room
+  for, layer and head: ``max_rows`` bounds them.
 
 Which page is whose is decided on the host, before anything is launched:
 ``reserve(n)`` finds pages for the next ``n`` rows of every sequence or raises
@@ -252,7 +257,8 @@ class PagedKVCache:
         """Bring every sequence (or ``seq`` alone) that holds more than ``keep`` rows down to
         ``keep``: its last ``recent`` rows (at most ``keep``) and the heaviest before them, in
         their order, each layer and head by its own weights. Returns how many sequences that
-        was. Rows stay where their pages are the sequence's alone; the others' go to new pages
+        was. Between steps only: rows that are appended but not committed are nobody's yet, and
+        are lost. Rows stay where their pages are the sequence's alone; the others' go to new pages
         (``RuntimeError`` with nothing changed when there are too few: all sequences' new pages
         are found before any old one is free, so on a full pool that sequences share, evict
         them one by one, which frees pages for the next and leaves the last sharer in place)."""

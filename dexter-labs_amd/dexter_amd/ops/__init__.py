@@ -456,7 +456,9 @@ def kv_keep_rows(weights: torch.Tensor, cache_lens: torch.Tensor, keep: int,
 
     Of the ``n = min(cache_lens[b], N)`` rows of sequence ``b``, ``c = min(n, keep)``: the last
     ``min(recent, c)`` and those with the largest weights before them; of equal ones the
-    lowest, and NaN counts as ``-inf``.
+    lowest, and NaN counts as ``-inf``. It knows no table: where a sequence has dropped pages,
+    give their rows a weight of ``-inf``, and keep no more rows than the others are and no
+    ``recent`` ones among them. A row that is kept without a page cannot move.
     """
     return select("cache", "keep_rows", weights)(weights, cache_lens, keep, recent)
 
@@ -468,9 +470,10 @@ def kv_page_gather(pages: torch.Tensor, block_table: torch.Tensor, rows: torch.T
     ``dst_table`` names (default: ``block_table``'s own, in place), in both planes; ``weights``
     ``[B, H, N]`` move with their rows and are 0 behind them.
 
-    ``rows`` is what ``kv_keep_rows`` returned: in place it has to be ascending with ``rows[b,
-    h, i] >= i``. Entries below 0, past a table or without a page move nothing, nor does a row
-    that is where it belongs. A page that rows move into must not be another sequence's, nor
+    ``rows`` is what ``kv_keep_rows`` returned. For a move in place, and wherever ``weights`` are
+    given (theirs is always in place), it has to be ascending with ``rows[b, h, i] >= i``. Entries
+    below 0, past a table or without a page move nothing (what stood in row ``i``'s place stays
+    there), nor does a row that is where it belongs. A page that rows move into must not be another sequence's, nor
     one that the call reads, but for the page that both tables name at the same place of one
     sequence. ``head_dim`` is needed for pages in 4 bits.
     """

@@ -662,7 +662,9 @@ int dx_paged_key_weights(const dx_weights_call* call);
  * per head: the last min(recent, c) of them and the c - min(recent, c) others with
  * the largest weights[b][h] (float [B, H, width]), c = min(n, keep); of equal ones
  * the lowest rows, and NaN counts as -inf. rows (int32 [B, H, keep]): their
- * numbers in order, then -1. No workspace.
+ * numbers in order, then -1. It knows no table: rows that lie in no page are
+ * the caller's to give -inf, and to keep out of the last `recent` and of c. No
+ * workspace.
  */
 int dx_kv_keep_rows(const void* weights, int64_t w_sb, int64_t w_sh, int64_t width,
                     const void* lens, int64_t keep, int64_t recent, void* rows,
@@ -671,11 +673,13 @@ int dx_kv_keep_rows(const void* weights, int64_t w_sb, int64_t w_sh, int64_t wid
 /*
  * Row i of sequence b's head h in the pages dst_table becomes row rows[b][h][i]
  * (int32 [B, H, keep], contiguous) of the pages src_table, in both planes; entries
- * that are negative, past a table or without a page move nothing. dst_table may
- * name the source's own pages at their places, where rows[b][h][i] >= i and
- * ascending (as dx_kv_keep_rows gives them), or pages that no sequence of the call
- * reads. weights (float [B, H, w_width], may be NULL) move with their rows, and are 0
- * behind them. dtype: the pool's, or DX_FP4 (byte strides, p_sr not read).
+ * that are negative, past a table or without a page move nothing, and what stood
+ * in row i's place stays there. dst_table may name the source's own pages at their
+ * places, or pages that no sequence of the call reads. weights (float [B, H,
+ * w_width], may be NULL) move with their rows, in place whatever dst_table is, and
+ * are 0 behind them. With weights, and with pages in place, rows[b][h][i] >= i and
+ * ascending, as dx_kv_keep_rows gives them. dtype: the pool's, or DX_FP4 (byte
+ * strides, p_sr not read).
  */
 int dx_kv_page_gather(void* pages, int64_t p_plane, int64_t p_sp, int64_t p_sr, int64_t p_sh,
                       int dtype, int64_t n_pages, int64_t page_rows, const void* src_table,
