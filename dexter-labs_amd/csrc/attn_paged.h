@@ -18,8 +18,7 @@ struct Record { int item, slot, parts, pad; };
 // A line of work: its partials and records.
 struct Line {
   float* o;     // [slot][32 RW rows][D]: unnormalised sums
-  float* ml;    // [slot][32 RW rows]: {m, l}
-  float* le;    // [slot][32 RW rows]: second sums (null: none)
+  float* ml;    // [slot][32 RW rows]: {m, l}; with two sums behind them, per slot, [32 RW rows]
   Record* rec;
   int splits;   // key ranges per item; 0: the line is cut into pieces
   int by_item;  // the records are, and there are some

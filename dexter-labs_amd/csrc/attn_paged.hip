@@ -247,12 +247,8 @@ int paged_entry(const char* what, const dx_paged_call* call, Form form) {
   };
   a.own.o = reinterpret_cast<float*>(take(p.own_slots * 32 * p.rw_own * c.D * 4));
   a.pre.o = reinterpret_cast<float*>(take(p.pre_slots * 32 * p.rw_pre * c.D * 4));
-  a.own.ml = reinterpret_cast<float*>(take(p.own_slots * 32 * p.rw_own * 8));
-  a.pre.ml = reinterpret_cast<float*>(take(p.pre_slots * 32 * p.rw_pre * 8));
-  if (two) {
-    a.own.le = reinterpret_cast<float*>(take(p.own_slots * 32 * p.rw_own * 4));
-    a.pre.le = reinterpret_cast<float*>(take(p.pre_slots * 32 * p.rw_pre * 4));
-  }
+  a.own.ml = reinterpret_cast<float*>(take(p.own_slots * 32 * p.rw_own * (two ? 12 : 8)));
+  a.pre.ml = reinterpret_cast<float*>(take(p.pre_slots * 32 * p.rw_pre * (two ? 12 : 8)));
   a.own.rec = reinterpret_cast<Record*>(take(p.own_recs * int64_t(sizeof(Record))));
   a.pre.rec = reinterpret_cast<Record*>(take(p.pre_recs * int64_t(sizeof(Record))));
   const hipStream_t st = static_cast<hipStream_t>(c.stream);

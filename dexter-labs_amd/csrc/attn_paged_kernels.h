@@ -102,7 +102,9 @@ constexpr bool in_fp4(Mode m) { return m == kFp4 || m == kFp4Lse; }
 constexpr bool with_lse(Mode m) { return m == kLse || m == kFp4Lse; }
 // Whether a row has two sums: that of its probabilities as they enter the product, rounded to
 // 16 bits, divides the result, and a log-sum-exp, a result in 32, takes them as they were. In fp32
-// nothing is rounded, and one serves both.
+// nothing is rounded, and one serves both. us a call without and with the second: 16 x 83 queries,
+// 24 heads, over a prefix of 8,217 rows 206 and 210, in 4 bits 204 and 209; 32 tokens, 8 K/V
+// heads, over 300 to 3,000 rows in 4 bits 29.7 and 30.2.
 template <typename T, Mode M> constexpr bool two_sums = with_lse(M) && Elem<T>::bytes == 2;
 
 // Tile rows of RB bytes in LDS: 16-byte chunk c of row r sits at c ^ kswz(r)
@@ -120,8 +122,8 @@ template <int RB, bool F32> __device__ __forceinline__ constexpr int vswz(int r)
 
 constexpr int kThreads = kPagedThreads, kWaves = kThreads / 64;
 
-// A workgroup's shape for RW row waves.
-template <typename T, int D, int RW> struct Shape {
+// A workgroup's shape for RW row waves (TWO: rows with two sums).
+template <typename T, int D, int RW, bool TWO = false> struct Shape {
   static constexpr int RB = D * Elem<T>::bytes;      // bytes of a row
   // Four waves and half of a CU's LDS, so that two workgroups share a CU and one
   // starts, ends or waits while the other computes. One row wave: streams of one
@@ -142,7 +144,7 @@ template <typename T, int D, int RW> struct Shape {
   // banks), {m, l} of 32 rows, and their second sums. D' = D, or half of it where that fits.
   static constexpr int DP = D > 128 ? 128 : D;
   static constexpr int vec = 1040;
-  static constexpr int ml = DP / 8 * vec, le = ml + 256, area = le + 128;
+  static constexpr int ml = DP / 8 * vec, le = ml + 256, area = le + (TWO ? 128 : 0);
   static constexpr int body = KW * stream > RW * KW * area ? KW * stream : RW * KW * area;
   // Behind them: which 16-row groups of each stage's tile have no page, and
   // whether a wave's sums hold what is no number.
@@ -723,12 +725,13 @@ __device__ __forceinline__ void send_rows(uint64_t from, int rows, int step, uin
 template <typename T, int D, int RW, bool PREFIX, bool SHARED, Mode M>
 __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uint32_t n,
                                          uint32_t total, uint32_t line_fresh) {
-  using Sh = Shape<T, D, RW>;
+  constexpr bool kTwoSums = two_sums<T, M>;
+  using Sh = Shape<T, D, RW, kTwoSums>;
   constexpr int RB = Sh::RB, KW = Sh::KW, TK = Sh::TK, CR = RB / 16, RPP = 64 / CR;
   using Ti = Tile<T, D, TK / 32, M>;
   // Single row waves over 4 bits: a key's dims go to lanes by blocks (CodedKeys), 8 dims
   // of product s being chunk chunk_of(s) + 4 g of the row; else chunk 2 s + g.
-  constexpr bool kByBlocks = in_fp4(M) && RW == 1, kTwoSums = two_sums<T, M>;
+  constexpr bool kByBlocks = in_fp4(M) && RW == 1;
   auto chunk_of = [](int s) { return kByBlocks ? 8 * (s / 4) + s % 4 : 2 * s; };
   constexpr bool F32 = Ti::F32;
   constexpr int KS = Ti::KS;
@@ -1230,8 +1233,14 @@ __device__ __forceinline__ void run_line(Args* args, char* smem, uint32_t w, uin
             po[0] = o[0];
             po[1] = o[1];
             if (col == 0) {
-              *reinterpret_cast<f32x2*>((PREFIX ? a.pre.ml : a.own.ml) + at_row * 2) = f32x2{mm, l};
-              if constexpr (kTwoSums) (PREFIX ? a.pre.le : a.own.le)[at_row] = le;
+              float* const ml_of = PREFIX ? a.pre.ml : a.own.ml;
+              if constexpr (kTwoSums) {
+                float* const to = ml_of + int64_t(slot) * (3 * 32 * RW);
+                *reinterpret_cast<f32x2*>(to + 2 * r) = f32x2{mm, l};
+                to[2 * 32 * RW + r] = le;
+              } else {
+                *reinterpret_cast<f32x2*>(ml_of + at_row * 2) = f32x2{mm, l};
+              }
             }
           }
         }
@@ -1416,8 +1425,16 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
           const bool pre = RWP > 0 && q < 0;
           const int64_t at = pre ? pre_row + int64_t(p) * (32 * RWP)
                                  : own_row + int64_t(broken ? (q ? 2 * q - 1 : 0) : q) * (32 * RWO);
-          ml[x] = *reinterpret_cast<const f32x2*>((pre ? a.pre.ml : a.own.ml) + at * 2);
-          if constexpr (kTwoSums) e[x] = (pre ? a.pre.le : a.own.le)[at];
+          const float* const ml_of = pre ? a.pre.ml : a.own.ml;
+          if constexpr (kTwoSums) {
+            constexpr uint32_t kRowsP = 32 * (RWP ? RWP : 1), kRowsO = 32 * RWO;  // of a slot
+            const uint32_t rows = pre ? kRowsP : kRowsO, r = uint32_t(at) & (rows - 1);
+            const float* const slot = ml_of + (at - r) * 3;
+            ml[x] = *reinterpret_cast<const f32x2*>(slot + 2 * r);
+            e[x] = slot[2 * rows + r];
+          } else {
+            ml[x] = *reinterpret_cast<const f32x2*>(ml_of + at * 2);
+          }
           const f32x4* const from = reinterpret_cast<const f32x4*>((pre ? a.pre.o : a.own.o) + at * D + 8 * ch);
           v[x][0] = from[0];
           v[x][1] = from[1];
@@ -1462,7 +1479,9 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
 
 template <typename T, int D, int RWP, int RWO, Mode M>
 hipError_t launch_form(const PagedArgs& a, const PagedPlan& p, hipStream_t st) {
-  constexpr int lds_own = Shape<T, D, RWO>::lds, lds_pre = RWP ? Shape<T, D, RWP ? RWP : 1>::lds : 0;
+  constexpr bool kTwoSums = two_sums<T, M>;
+  constexpr int lds_own = Shape<T, D, RWO, kTwoSums>::lds;
+  constexpr int lds_pre = RWP ? Shape<T, D, RWP ? RWP : 1, kTwoSums>::lds : 0;
   constexpr int lds = lds_own > lds_pre ? lds_own : lds_pre;
   const void* fn = reinterpret_cast<const void*>(&paged_attn_kernel<T, D, RWP, RWO, M>);
   hipError_t e = opt_in_lds(fn, lds);
