@@ -42,8 +42,8 @@
 // arithmetic, and rows past the end (or of a table entry that names no page)
 // come back as zeros from the descriptor's bound.
 //
-// What it takes (medians; bf16, D 128 where not said; kernel alone, the join 4-8 us
-// more where not said):
+// What it takes (medians; bf16, D 128 where not said; kernel alone under the profiler, the
+// join 4-8 us more where not said; in a running stream the causal prompts take 10% less):
 //   32 tokens, 8 K/V heads, 300 to 3,000 cached rows each   48 us, 4.4 TB/s
 //   the same at D 256                                        84 us, 5.1 TB/s
 //   83 queries, 24 heads, 32,768 cached rows                 84 us, 4.8 TB/s
@@ -56,14 +56,14 @@
 //   2 x 1,500 causal, 8 K/V heads, 400 to 1,000 rows         74 us, 446 TFLOP/s (no join)
 //   the same at D 256                                        165 us, 398 TFLOP/s (join 23)
 //   4 x 99 in fp32, 24 heads, 0 to 1,245 rows                62 us, 48 TFLOP/s
-// and over cached rows in 4 bits:
-//   32 tokens, 8 K/V heads, 300 to 3,000 cached rows each   26 us, 2.2 TB/s
-//   83 queries, 24 heads, 32,768 cached rows                 71 us, 472 TFLOP/s
-//   2 x 1,500 causal in f16, 8 K/V heads, 400 to 1,000 rows  82 us, 403 TFLOP/s (no join)
-//   16 x 83, 24 heads, 0 to 332 rows, prefix of 8,217        203 us, 680 TFLOP/s (join 20)
+// and over cached rows in 4 bits, with log-sum-exps:
+//   32 tokens, 8 K/V heads, 300 to 3,000 cached rows each   28 us, 2.0 TB/s
+//   83 queries, 24 heads, 32,768 cached rows                 74 us, 455 TFLOP/s
+//   2 x 1,500 causal in f16, 8 K/V heads, 400 to 1,000 rows  86 us, 383 TFLOP/s (no join)
+//   16 x 83, 24 heads, 0 to 332 rows, prefix of 8,217        204 us, 678 TFLOP/s (join 21)
 // Four bits, many keys to a row tile: bound by the chain code -> value -> LDS -> product,
 // which takes the place of the DMA: 83 queries' tile takes 5,400 cycles of a wave, a
-// quarter of them the conversion, and matrix units are busy 25%.
+// quarter of them the conversion, and matrix units are busy 21% of the launch.
 // Many keys to a row tile: bound by memory. Otherwise by the chain of a tile (scores,
 // softmax, product) in the few waves that registers allow, and by the 4 to 8 us from
 // a workgroup's start to its first product: lengths, table, keys and queries, one

@@ -10,7 +10,9 @@
 // LDS (up to 32,768 rows): they are read once. (In registers the unrolled passes over 32
 // of them are 30 KB of code, which takes longer to fetch than to run.) Bound by one compute
 // unit's passes over a head's weights, four steps that wait for each other: 8,192 of 32,768
-// rows for 96 heads take 21.5 us (15.7 MB: 0.7 TB/s), 1,024 of 300 to 3,000 for 256 heads 8.7.
+// rows for 96 heads take 22 us (15.7 MB: 0.7 TB/s; 23.6 with other weights each time), 1,024 of
+// 300 to 3,000 for 256 heads 8.7 (9.1). Past 32,768 rows each pass reads the weights again, one load
+// at a time: 8,192 of 40,000 for 96 heads 40 us, of 65,536 62, of 131,072 for 24 heads 111.
 // A second histogram for odd lanes, to halve what meets in one digit, changed nothing.
 //
 // kv_page_gather. Row i of a head becomes row rows[i], which is i at least and ascending in
@@ -19,8 +21,9 @@
 // later steps read lies behind the rows that this one writes. So it may run in place, on the
 // pages it reads. Bound by memory: kept rows are read and written once; the next step's loads
 // are under way while one is stored, and the lookups of 1,024 rows are made at once. 8,192 of
-// 32,768 rows of 24 heads (bf16, D 128, in place): 49 us, 4.1 TB/s; of four such sequences 241
-// us, 3.4 TB/s; 1,024 of 300 to 3,000 rows of 32 x 8 heads in 4 bits to new pages: 16 us.
+// 32,768 rows of 24 heads (bf16, D 128, in place): 47 us, 4.3 TB/s, when the same rows come again,
+// and 77 with others, 2.7; of four such sequences 244 us, 3.3 TB/s; 1,024 of 300 to 3,000 rows of 32
+// x 8 heads in 4 bits to new pages: 17 and 22 us.
 #include "attn_common.h"
 #include "kv_fp4.h"
 

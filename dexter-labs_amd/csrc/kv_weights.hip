@@ -16,11 +16,14 @@
 // a wave halve the LDS reads per product, which at 32 would take the LDS as long as the
 // products take the matrix units.
 //
-// What it takes: a chunk of 83 over 32,768 rows of 24 heads (D 128) 44 us in bf16, 4.6 TB/s,
-// 32 us in 4 bits; one token of 32 prompts of 300 to 3,000 rows in 4 bits 15.4 us, of which
-// the host's part is 15; 2 x 1,500 queries, 16 heads over 8, over 4,000 to 10,000 rows 120
-// us, 600 TFLOP/s, exponentials and products in turn. Long workgroups that walk several blocks
-// of keys gained nothing at 3 to 1,000 workgroups per compute unit.
+// What it takes (in a captured stream): a chunk of 83 over 32,768 rows of 24 heads (D 128) 43 us
+// in bf16 when the same rows come again, 4.7 TB/s, and 58 with others, 3.6; 32 us in 4 bits; 199
+// in fp32, whose products are a thirteenth of the rate; one token of 32 prompts of 300 to 3,000
+// rows 14.5 us in 4 bits, most of it first loads, and 30 in 16; 2 x 1,500 queries, 16 heads
+// over 8, over 4,000 to 10,000 rows 120 us, 600 TFLOP/s, exponentials and products in turn, and 158
+// over a table of twice the width: workgroups that find no row there take a place among the
+// others, and CUs get uneven shares. Long workgroups that walk several blocks of keys gained
+// nothing at 3 to 1,000 workgroups per compute unit.
 #include "attn_common.h"
 #include "attn_tile.h"
 #include "kv_fp4.h"
@@ -94,7 +97,7 @@ __global__ __launch_bounds__(kThreads) void paged_key_weights_kernel(WeightArgs 
   // Queries on their way into LDS: this thread's chunks of rows row0.., and a row's lse. The
   // first ones are read before all else, then the page numbers, whatever the length: what a
   // workgroup waits for at its start are two reads one after the other, not four (a chunk of 83
-  // over 32,768 rows of 24 heads in bf16: 50.0 us, 41 so).
+  // over 32,768 rows of 24 heads in bf16, the same rows again: 50 us in the other order).
   constexpr int NQ = QT * CR / kThreads;
   static_assert(QT * CR % kThreads == 0 && QT <= kThreads, "whole shares");
   u32x4 qx[NQ];
